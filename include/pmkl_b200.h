@@ -263,6 +263,144 @@ int pmkl_causal_attention_bwd_static(const void *dout, const void *q, const void
 int pmkl_warp_softmax_fwd(void *dst, const void *src, int elements, int stride, int rows, int in_dtype,
                           int out_dtype, int is_log, void *stream);
 
+/*
+ * Serving attention from a paged cache of keys and values in 8 bits.  Three
+ * operators of this library (no reference counterpart) make a step after the
+ * projections: pmkl_paged_plan gives the step's new tokens their places in the
+ * cache, pmkl_paged_append writes their keys and values there,
+ * pmkl_paged_attention attends with their queries.
+ *
+ * The cache.  k_cache and v_cache hold `num_blocks` pages of `block_size` rows
+ * for each of `kv_heads` heads, [num_blocks, kv_heads, block_size, hidden]
+ * 8-bit floats (e4m3: 4 exponent and 3 mantissa bits, largest value 448) at
+ * block * s[0] + head * s[1] + row * s[2] + col (s = k_strides / v_strides;
+ * NULL = contiguous).  k_scale and v_scale are contiguous
+ * [num_blocks, kv_heads] fp32: a stored value x stands for x * scale of its
+ * page and head.  Row r of request b is row r % block_size of page
+ * block_table[b][r / block_size]; the slot of a row is page * block_size + row
+ * in its page.
+ *
+ * Tokens of a step are packed by request: request b has the rows
+ * query_starts[b] <= t < query_starts[b + 1] of q, k, v, o.
+ */
+
+/* Kernel selection for pmkl_paged_attention. */
+typedef enum pmkl_paged_kernel {
+    PMKL_PAGED_AUTO = 0,
+    PMKL_PAGED_SIMT = 1, /* CUDA cores: any dtype, hidden 1..256, any block size */
+} pmkl_paged_kernel;
+
+/* Why paged_plan left a request out (status[b]). */
+typedef enum pmkl_plan_status {
+    PMKL_PLAN_OK = 0,
+    PMKL_PLAN_NO_BLOCKS = 1,   /* the free list has not enough pages */
+    PMKL_PLAN_NO_COLUMNS = 2,  /* the block table is too narrow */
+    PMKL_PLAN_NO_TOKENS = 3,   /* its tokens go past max_tokens */
+} pmkl_plan_status;
+
+/*
+ * Pages, block table and slot map for a step's new tokens, from the requests'
+ * lengths, all on the device: one launch, no synchronisation, sizes on the
+ * host only as upper limits, so that it can be captured in a graph.
+ *
+ *   cached_lens, new_lens : [batch] int32, rows in the cache and rows to add
+ *                           (negative values count as 0).
+ *   block_table           : [batch] rows of max_blocks int32, table_stride
+ *                           elements apart; entries of the rows in the cache
+ *                           are read, entries of new pages are written, others
+ *                           stay.
+ *   free_blocks, free_count : the free pages, free_blocks[0 .. *free_count - 1]
+ *                           (int32; free_capacity elements are allocated, which
+ *                           limits the count).  The i-th page taken is
+ *                           free_blocks[*free_count - 1 - i], pages being taken
+ *                           in the requests' order.
+ *   max_tokens            : length of slot_map.
+ *   seq_lens              : [batch] out, cached + new (cached where left out).
+ *   query_starts          : [batch + 1] out, running sums of new_lens.
+ *   slot_map              : [max_tokens] int64 out, the slot of each new token;
+ *                           -1 for tokens of requests left out and past the
+ *                           last token.
+ *   free_count_out        : [1] out, free pages left; may not be free_count.
+ *   status                : [batch] int32 out, a pmkl_plan_status.
+ *
+ * A request whose tokens do not end within max_tokens or whose pages do not
+ * fit max_blocks is left out and takes no page.  Of the others request b gets
+ * its pages when the pages that the requests up to b need together are there
+ * (requests that need none always pass).  The sum of new_lens must stay below
+ * 2^31.
+ */
+int pmkl_paged_plan(const int32_t *cached_lens, const int32_t *new_lens, int32_t *block_table, int64_t table_stride,
+                    const int32_t *free_blocks, const int32_t *free_count, int free_capacity, int batch,
+                    int max_blocks, int block_size, int64_t max_tokens, int32_t *seq_lens, int32_t *query_starts,
+                    int64_t *slot_map, int32_t *free_count_out, int32_t *status, void *stream);
+
+/*
+ * Writes new keys and values into the cache as 8-bit floats.
+ *
+ *   k, v     : [tokens, kv_heads, hidden] of `dtype`, element strides
+ *              (token, head) kv_strides_k / kv_strides_v, NULL = contiguous,
+ *              hidden contiguous.
+ *   slot_map : [tokens] int64; tokens with a slot outside the cache (-1) are
+ *              skipped.
+ *
+ * Tokens whose slots follow one another in one page form a run; a page is
+ * written by at most one run of a call (pmkl_paged_plan's slot maps are so;
+ * two runs in one page race on its scale).  The scale of the page and head
+ * becomes the smallest power of two s of 2^-64 .. 2^64 with max |x| <= 448 s
+ * over the run's finite values, or stays, where the page held rows before the
+ * run and its scale is larger; where it grows, the rows of the page before the
+ * run are rounded again by the ratio.  A run from row 0 starts the page anew.
+ * Values are stored as e4m3(x / s), to the nearest, ties to even, beyond 448
+ * as 448; NaN stays NaN.
+ */
+int pmkl_paged_append(const void *k, const void *v, const int64_t *k_new_strides, const int64_t *v_new_strides,
+                      const int64_t *slot_map, int tokens, int kv_heads, int hidden, int dtype, void *k_cache,
+                      void *v_cache, const int64_t *k_strides, const int64_t *v_strides, float *k_scale,
+                      float *v_scale, int num_blocks, int block_size, void *stream);
+
+/*
+ * Attention of a step's queries over the cache.
+ *
+ *   q, o         : [tokens, heads, hidden] of `dtype`, element strides (token,
+ *                  head) q_strides / o_strides, NULL = contiguous, hidden
+ *                  contiguous.  Query head h reads K/V head h / (heads /
+ *                  kv_heads).
+ *   lse          : [tokens, heads] fp32 out, log of the sum of exp(s) over the
+ *                  visible keys, s = scale * q.k; may be NULL.
+ *   block_table  : as in pmkl_paged_plan; only entries of pages that hold rows
+ *                  of a request are read.  Keys in a page outside the cache
+ *                  count as not there.
+ *   seq_lens     : [batch] int32 rows in the cache, the step's own included.
+ *   query_starts : [batch + 1] int32; NULL: one token a request (tokens ==
+ *                  batch).
+ *   max_query_len: no request has more tokens in the step (rows past it are
+ *                  not written).
+ *   is_causal    : token i of a request's n sees the keys up to its own place,
+ *                  seq_len - n + i; otherwise all of them.
+ *   scale        : score scale; <= 0 for 1/sqrt(hidden).
+ *   workspace    : device scratch of at least
+ *                  pmkl_paged_attention_workspace_size(...) bytes, 256-byte
+ *                  aligned; contents on entry do not matter.
+ *
+ * A row that sees no key gets o = 0 and lse = -inf, and so do rows of q past
+ * query_starts[batch].  Rows of a page behind seq_len may hold anything, NaN
+ * included.  Scales are positive; the scale of a page of values outside
+ * 2^-64 .. 2^64 counts as the nearer of the two.  Scores, softmax and sums
+ * are fp32, o is rounded once.
+ */
+int pmkl_paged_attention(const void *q, const int64_t *q_strides, const void *k_cache, const void *v_cache,
+                         const int64_t *k_strides, const int64_t *v_strides, const float *k_scale,
+                         const float *v_scale, const int32_t *block_table, int64_t table_stride,
+                         const int32_t *seq_lens, const int32_t *query_starts, void *o, const int64_t *o_strides,
+                         float *lse, int tokens, int batch, int heads, int kv_heads, int hidden, int num_blocks,
+                         int block_size, int max_blocks, int max_query_len, int dtype, int is_causal, float scale,
+                         void *workspace, size_t workspace_bytes, int kernel, void *stream);
+
+/* Workspace bytes of pmkl_paged_attention for these sizes (0 for an empty
+ * problem).  Host only. */
+size_t pmkl_paged_attention_workspace_size(int tokens, int batch, int heads, int kv_heads, int hidden,
+                                           int max_query_len, int dtype);
+
 /* Human-readable name of a pmkl_status value (static storage). */
 const char *pmkl_status_string(int status);
 

@@ -77,6 +77,16 @@ def capi() -> ctypes.CDLL:
         L.pmkl_causal_attention_bwd_workspace_size_ex.argtypes = [i32] * 6
         L.pmkl_warp_softmax_fwd.restype = i32
         L.pmkl_warp_softmax_fwd.argtypes = [vp, vp] + [i32] * 6 + [vp]
+        i64, sz = ctypes.c_int64, ctypes.c_size_t
+        L.pmkl_paged_plan.restype = i32
+        L.pmkl_paged_plan.argtypes = [vp] * 3 + [i64, vp, vp] + [i32] * 4 + [i64] + [vp] * 6
+        L.pmkl_paged_append.restype = i32
+        L.pmkl_paged_append.argtypes = [vp, vp, i64p, i64p, vp] + [i32] * 4 + [vp, vp, i64p, i64p, vp, vp, i32, i32, vp]
+        L.pmkl_paged_attention.restype = i32
+        L.pmkl_paged_attention.argtypes = [vp, i64p, vp, vp, i64p, i64p, vp, vp, vp, i64, vp, vp, vp, i64p, vp] + [
+            i32] * 11 + [f32, vp, sz, i32, vp]
+        L.pmkl_paged_attention_workspace_size.restype = sz
+        L.pmkl_paged_attention_workspace_size.argtypes = [i32] * 7
         L.pmkl_status_string.restype = ctypes.c_char_p
         L.pmkl_status_string.argtypes = [i32]
         L.pmkl_version.restype = i32

@@ -3,8 +3,8 @@
 * ``libpmkl_b200.so`` -- the CUDA kernels and the C ABI of
   ``include/pmkl_b200.h``, compiled by nvcc for sm_100a only
   (``-gencode arch=compute_100a,code=sm_100a``) into ``pmkl_b200/lib/``.
-* ``pmkl_pytorch_ext`` -- the torch binding (``torch_ext/fused_self_attention.cpp``),
-  compiled with torch's extension builder into ``pmkl_b200/torch_ext/_build/``
+* ``pmkl_pytorch_ext`` -- the torch binding (``torch_ext/fused_self_attention.cpp``
+  and ``torch_ext/paged.h``), compiled with torch's extension builder into ``pmkl_b200/torch_ext/_build/``
   and linked against ``libpmkl_b200.so`` through an ``$ORIGIN`` rpath.
 
 Both land inside the source tree so that they travel with it; nothing is
@@ -78,7 +78,8 @@ def build_ext(force: bool = False, verbose: bool = False) -> Path:
     EXT_BUILD_DIR.mkdir(parents=True, exist_ok=True)
     so = EXT_BUILD_DIR / f"{EXT_NAME}.so"
     src = EXT_SRC_DIR / "fused_self_attention.cpp"
-    newest = max(src.stat().st_mtime, (INCLUDE / "pmkl_b200.h").stat().st_mtime, LIB_PATH.stat().st_mtime)
+    newest = max(src.stat().st_mtime, (EXT_SRC_DIR / "paged.h").stat().st_mtime,
+                 (INCLUDE / "pmkl_b200.h").stat().st_mtime, LIB_PATH.stat().st_mtime)
     if so.is_file() and not force and so.stat().st_mtime >= newest:
         return so
     cuda_home = Path(cpp.CUDA_HOME or "/usr/local/cuda")

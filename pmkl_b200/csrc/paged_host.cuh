@@ -1,0 +1,215 @@
+// paged_host.cuh -- host side of the paged 8-bit cache's operators: argument
+// checks, kernel selection and launches.  Included by pmkl_b200.cu, whose
+// device checks and launch helpers it uses.
+#pragma once
+
+#include "paged_append.cuh"
+#include "paged_attention_simt.cuh"
+#include "paged_plan.cuh"
+
+namespace pmkl_b200 {
+namespace {
+
+// Calls f with a null pointer of the element type that `dtype` names.
+template <typename F>
+int with_dtype(int dtype, F f) {
+    if (dtype == PMKL_DTYPE_F32) return f(static_cast<float *>(nullptr));
+    if (dtype == PMKL_DTYPE_F16) return f(static_cast<__half *>(nullptr));
+    return f(static_cast<__nv_bfloat16 *>(nullptr));
+}
+
+unsigned blocks_for(long long units, long long per_block, int blocks_per_sm) {
+    const long long need = (units + per_block - 1) / per_block;
+    const long long cap = static_cast<long long>(sm_count()) * blocks_per_sm;
+    return static_cast<unsigned>(need < cap ? need : cap);
+}
+
+// Strides of the cache [num_blocks][kv_heads][block_size][hidden].
+bool cache_view(paged::CacheView *c, const void *base, const float *scale, const int64_t *given, int kv_heads,
+                int block, int hidden) {
+    c->base = static_cast<uint8_t *>(const_cast<void *>(base));
+    c->scale = const_cast<float *>(scale);
+    const long long s[3] = {static_cast<long long>(kv_heads) * block * hidden, static_cast<long long>(block) * hidden,
+                            hidden};
+    for (int i = 0; i < 3; ++i) {
+        if (given && given[i] < 0) return false;
+        c->s[i] = given ? given[i] : s[i];
+    }
+    return true;
+}
+
+// (token, head) strides of a packed [tokens][heads][hidden] tensor.
+bool packed_strides(long long (&st)[2], const int64_t *given, int heads, int hidden) {
+    const long long s[2] = {static_cast<long long>(heads) * hidden, hidden};
+    for (int i = 0; i < 2; ++i) {
+        if (given && given[i] < 0) return false;
+        st[i] = given ? given[i] : s[i];
+    }
+    return true;
+}
+
+int paged_plan_impl(const paged::PlanArgs &a, cudaStream_t stream) {
+    paged::PlanArgs p = a;
+    // 1024 slots a CTA and at least one CTA; every CTA forms the running sums
+    // of all requests, so more CTAs than SMs would only repeat them.
+    const unsigned grid = p.max_tokens > 0 ? blocks_for(p.max_tokens, 1024, 1) : 1;
+    p.tokens_per_cta = (p.max_tokens + grid - 1) / grid;
+    paged::paged_plan_kernel<<<grid, paged::kPlanThreads, 0, stream>>>(p);
+    return launch_status();
+}
+
+int paged_append_impl(const paged::AppendArgs &p, int dtype, cudaStream_t stream) {
+    const long long units = static_cast<long long>(p.tokens) * p.kv_heads * 2;
+    return with_dtype(dtype, [&](auto *t) -> int {
+        using T = std::remove_pointer_t<decltype(t)>;
+        paged::paged_append_kernel<T>
+            <<<blocks_for(units, paged::kAppendThreads / 32, 16), paged::kAppendThreads, 0, stream>>>(p);
+        return launch_status();
+    });
+}
+
+int paged_attention_impl(const paged::AttnArgs &p, int dtype, int kernel, cudaStream_t stream) {
+    (void)kernel;
+    const long long units = static_cast<long long>(p.batch) * p.max_q * p.H;
+    return with_dtype(dtype, [&](auto *t) -> int {
+        using T = std::remove_pointer_t<decltype(t)>;
+        paged::paged_attention_simt_kernel<T>
+            <<<blocks_for(units > 0 ? units : 1, 1, 16), paged::kSimtThreads, 0, stream>>>(p);
+        return launch_status();
+    });
+}
+
+}  // namespace
+}  // namespace pmkl_b200
+
+extern "C" {
+
+int pmkl_paged_plan(const int32_t *cached_lens, const int32_t *new_lens, int32_t *block_table, int64_t table_stride,
+                    const int32_t *free_blocks, const int32_t *free_count, int free_capacity, int batch,
+                    int max_blocks, int block_size, int64_t max_tokens, int32_t *seq_lens, int32_t *query_starts,
+                    int64_t *slot_map, int32_t *free_count_out, int32_t *status, void *stream) {
+    if (batch < 0 || max_blocks < 0 || block_size < 1 || max_tokens < 0 || free_capacity < 0 || table_stride < 0)
+        return PMKL_ERR_INVALID_SHAPE;
+    if (batch > 1 && table_stride < max_blocks) return PMKL_ERR_INVALID_SHAPE;
+    if (max_tokens > 0x7FFFFFFFLL) return PMKL_ERR_INVALID_SHAPE;
+    if (!free_count || !free_count_out || !query_starts) return PMKL_ERR_NULL_POINTER;
+    if (free_capacity > 0 && !free_blocks) return PMKL_ERR_NULL_POINTER;
+    if (max_tokens > 0 && !slot_map) return PMKL_ERR_NULL_POINTER;
+    if (batch > 0 && (!cached_lens || !new_lens || !seq_lens || !status || (max_blocks > 0 && !block_table)))
+        return PMKL_ERR_NULL_POINTER;
+    if (free_count == free_count_out) return PMKL_ERR_INVALID_SHAPE;
+    const int dev_rc = current_device_ok();
+    if (dev_rc != PMKL_OK) return dev_rc;
+    paged::PlanArgs p{};
+    p.cached = cached_lens;
+    p.fresh = new_lens;
+    p.table = block_table;
+    p.table_stride = table_stride;
+    p.free_blocks = free_blocks;
+    p.free_count = free_count;
+    p.free_capacity = free_capacity;
+    p.batch = batch;
+    p.max_blocks = max_blocks;
+    p.block = block_size;
+    p.max_tokens = max_tokens;
+    p.seq_lens = seq_lens;
+    p.query_starts = query_starts;
+    p.slots = reinterpret_cast<long long *>(slot_map);
+    p.free_out = free_count_out;
+    p.status = status;
+    return paged_plan_impl(p, static_cast<cudaStream_t>(stream));
+}
+
+int pmkl_paged_append(const void *k, const void *v, const int64_t *k_new_strides, const int64_t *v_new_strides,
+                      const int64_t *slot_map, int tokens, int kv_heads, int hidden, int dtype, void *k_cache,
+                      void *v_cache, const int64_t *k_strides, const int64_t *v_strides, float *k_scale,
+                      float *v_scale, int num_blocks, int block_size, void *stream) {
+    if (tokens < 0 || kv_heads < 0 || hidden < 0 || num_blocks < 0 || block_size < 1) return PMKL_ERR_INVALID_SHAPE;
+    if (!dtype_valid(dtype)) return PMKL_ERR_INVALID_DTYPE;
+    if (tokens == 0 || kv_heads == 0 || hidden == 0 || num_blocks == 0) return PMKL_OK;
+    if (hidden > 256) return PMKL_ERR_UNSUPPORTED;
+    if (!k || !v || !slot_map || !k_cache || !v_cache || !k_scale || !v_scale) return PMKL_ERR_NULL_POINTER;
+    paged::AppendArgs p{};
+    p.x[0] = k;
+    p.x[1] = v;
+    if (!packed_strides(p.x_st[0], k_new_strides, kv_heads, hidden) ||
+        !packed_strides(p.x_st[1], v_new_strides, kv_heads, hidden) ||
+        !cache_view(&p.cache[0], k_cache, k_scale, k_strides, kv_heads, block_size, hidden) ||
+        !cache_view(&p.cache[1], v_cache, v_scale, v_strides, kv_heads, block_size, hidden))
+        return PMKL_ERR_INVALID_SHAPE;
+    const int dev_rc = current_device_ok();
+    if (dev_rc != PMKL_OK) return dev_rc;
+    p.slots = reinterpret_cast<const long long *>(slot_map);
+    p.tokens = tokens;
+    p.kv_heads = kv_heads;
+    p.hidden = hidden;
+    p.block = block_size;
+    p.num_slots = static_cast<long long>(num_blocks) * block_size;
+    return paged_append_impl(p, dtype, static_cast<cudaStream_t>(stream));
+}
+
+size_t pmkl_paged_attention_workspace_size(int tokens, int batch, int heads, int kv_heads, int hidden,
+                                           int max_query_len, int dtype) {
+    if (tokens <= 0 || batch <= 0 || heads <= 0 || kv_heads <= 0 || hidden <= 0 || max_query_len <= 0 ||
+        heads % kv_heads != 0 || !dtype_valid(dtype))
+        return 0;
+    return 0;
+}
+
+int pmkl_paged_attention(const void *q, const int64_t *q_strides, const void *k_cache, const void *v_cache,
+                         const int64_t *k_strides, const int64_t *v_strides, const float *k_scale,
+                         const float *v_scale, const int32_t *block_table, int64_t table_stride,
+                         const int32_t *seq_lens, const int32_t *query_starts, void *o, const int64_t *o_strides,
+                         float *lse, int tokens, int batch, int heads, int kv_heads, int hidden, int num_blocks,
+                         int block_size, int max_blocks, int max_query_len, int dtype, int is_causal, float scale,
+                         void *workspace, size_t workspace_bytes, int kernel, void *stream) {
+    if (tokens < 0 || batch < 0 || heads < 0 || kv_heads < 0 || hidden < 0 || num_blocks < 0 || block_size < 1 ||
+        max_blocks < 0 || max_query_len < 0 || table_stride < 0)
+        return PMKL_ERR_INVALID_SHAPE;
+    if (!dtype_valid(dtype)) return PMKL_ERR_INVALID_DTYPE;
+    if (kernel != PMKL_PAGED_AUTO && kernel != PMKL_PAGED_SIMT) return PMKL_ERR_UNSUPPORTED;
+    if (heads > 0 && (kv_heads == 0 || heads % kv_heads != 0)) return PMKL_ERR_INVALID_SHAPE;
+    if (batch > 1 && table_stride < max_blocks) return PMKL_ERR_INVALID_SHAPE;
+    if (!query_starts && tokens != batch) return PMKL_ERR_INVALID_SHAPE;
+    if (tokens == 0 || heads == 0 || hidden == 0) return PMKL_OK;
+    if (hidden > 256) return PMKL_ERR_UNSUPPORTED;
+    if (!q || !o) return PMKL_ERR_NULL_POINTER;
+    if (batch > 0 && !seq_lens) return PMKL_ERR_NULL_POINTER;
+    if (batch > 0 && max_blocks > 0 && !block_table) return PMKL_ERR_NULL_POINTER;
+    if (num_blocks > 0 && (!k_cache || !v_cache || !k_scale || !v_scale)) return PMKL_ERR_NULL_POINTER;
+    const size_t need =
+        pmkl_paged_attention_workspace_size(tokens, batch, heads, kv_heads, hidden, max_query_len, dtype);
+    if (need > 0) {
+        if (!workspace) return PMKL_ERR_NULL_POINTER;
+        if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return PMKL_ERR_MISALIGNED;
+        if (workspace_bytes < need) return PMKL_ERR_WORKSPACE;
+    }
+    paged::AttnArgs p{};
+    if (!packed_strides(p.q_st, q_strides, heads, hidden) || !packed_strides(p.o_st, o_strides, heads, hidden) ||
+        !cache_view(&p.k, k_cache, k_scale, k_strides, kv_heads, block_size, hidden) ||
+        !cache_view(&p.v, v_cache, v_scale, v_strides, kv_heads, block_size, hidden))
+        return PMKL_ERR_INVALID_SHAPE;
+    const int dev_rc = current_device_ok();
+    if (dev_rc != PMKL_OK) return dev_rc;
+    p.q = q;
+    p.o = o;
+    p.table = block_table;
+    p.table_stride = table_stride;
+    p.seq_lens = seq_lens;
+    p.query_starts = query_starts;
+    p.lse = lse;
+    p.tokens = tokens;
+    p.batch = batch;
+    p.H = heads;
+    p.Hkv = kv_heads;
+    p.D = hidden;
+    p.num_blocks = num_blocks;
+    p.block = block_size;
+    p.max_blocks = max_blocks;
+    p.max_q = query_starts ? max_query_len : 1;
+    p.causal = is_causal ? 1 : 0;
+    p.scale = scale > 0.f ? scale : 1.0f / sqrtf(static_cast<float>(hidden));
+    return paged_attention_impl(p, dtype, kernel, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -1069,3 +1069,5 @@ int pmkl_tc_selftest(int which, const void *a, const void *b, float *c, int hidd
 }
 
 }  // extern "C"
+
+#include "paged_host.cuh"

@@ -174,6 +174,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> fused_self_attention_bw_ex(
     return backward_impl(dout, q, k, v, out_m, out_l, is_causal, kernel, scale, true);
 }
 
+#include "paged.h"
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("fused_self_attention_fw", &fused_self_attention_fw, "fused_self_attention_fw");
     m.def("fused_self_attention_bw", &fused_self_attention_bw, "fused_self_attention_bw");
@@ -184,6 +186,17 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("fused_self_attention_fw_ex", &fused_self_attention_fw_ex, "fused_self_attention_fw_ex",
           pybind11::arg("q"), pybind11::arg("k"), pybind11::arg("v"), pybind11::arg("is_causal"),
           pybind11::arg("out_fp32") = false, pybind11::arg("kernel") = 0, pybind11::arg("scale") = 0.0);
+    m.def("paged_plan", &paged_plan, "paged_plan", pybind11::arg("cached_lens"), pybind11::arg("new_lens"),
+          pybind11::arg("block_table"), pybind11::arg("free_blocks"), pybind11::arg("free_count"),
+          pybind11::arg("block_size"), pybind11::arg("max_tokens"));
+    m.def("paged_append", &paged_append, "paged_append", pybind11::arg("k"), pybind11::arg("v"),
+          pybind11::arg("slot_map"), pybind11::arg("k_cache"), pybind11::arg("v_cache"), pybind11::arg("k_scale"),
+          pybind11::arg("v_scale"));
+    m.def("paged_attention_fw", &paged_attention_fw, "paged_attention_fw", pybind11::arg("q"),
+          pybind11::arg("k_cache"), pybind11::arg("v_cache"), pybind11::arg("k_scale"), pybind11::arg("v_scale"),
+          pybind11::arg("block_table"), pybind11::arg("seq_lens"), pybind11::arg("query_starts") = pybind11::none(),
+          pybind11::arg("max_query_len") = 1, pybind11::arg("is_causal") = true, pybind11::arg("scale") = 0.0,
+          pybind11::arg("kernel") = 0);
     m.attr("KERNEL_AUTO") = static_cast<int>(PMKL_ATTN_AUTO);
     m.attr("KERNEL_SIMT") = static_cast<int>(PMKL_ATTN_SIMT);
     m.attr("KERNEL_TCGEN05") = static_cast<int>(PMKL_ATTN_TCGEN05);

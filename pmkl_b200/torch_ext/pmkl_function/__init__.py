@@ -26,6 +26,17 @@ takes k, v with fewer heads than q (grouped-query / multi-query attention:
 query head h reads K/V head h // (H // H_kv)) and an explicit score scale
 (<= 0: 1/sqrt(D)); its backward returns dk, dv with k's and v's head count,
 each the sum over the query heads that read it.
+
+For answering with a model, three operators over a paged cache of keys and
+values in 8 bits (no reference counterpart); a step calls them in this order:
+
+    seq_lens, query_starts, slot_map, free_count, status = paged_plan(
+        cached_lens, new_lens, block_table, free_blocks, free_count, block_size, max_tokens)
+    paged_append(k, v, slot_map, k_cache, v_cache, k_scale, v_scale)
+    out, lse = paged_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens,
+                               query_starts=None, max_query_len=1, is_causal=True, scale=0.0)
+
+See each function's text; ``examples/paged_decode.py`` runs them together.
 """
 import torch
 from torch.autograd import Function
@@ -35,6 +46,9 @@ import pmkl_pytorch_ext
 __all__ = [
     'fused_self_attention',
     'fused_self_attention_ex',
+    'paged_append',
+    'paged_attention',
+    'paged_plan',
 ]
 
 
@@ -90,3 +104,53 @@ class fused_self_attention_ex_(Function):
 
 
 fused_self_attention_ex = fused_self_attention_ex_.apply
+
+
+def paged_plan(cached_lens, new_lens, block_table, free_blocks, free_count, block_size, max_tokens):
+    """Pages, block table and slot map for a step's new tokens, on the device.
+
+    ``cached_lens``, ``new_lens``: [batch] int32, each request's rows in the
+    cache and tokens to add.  ``block_table``: [batch, pages] int32, written in
+    place where a request gets new pages.  ``free_blocks`` [n] and
+    ``free_count`` [1] int32: the free pages, taken from the end of the first
+    ``free_count``.  ``max_tokens``: length of the slot map, at least the new
+    tokens' number.
+
+    Returns ``seq_lens`` [batch] (cached + new), ``query_starts`` [batch + 1]
+    (running sums of ``new_lens``), ``slot_map`` [max_tokens] int64 (page *
+    block_size + row of each token, -1 behind the last), ``free_count`` [1] (a
+    new tensor: pages left) and ``status`` [batch]: 0, or why the request was
+    left out, with no page taken and -1 for its tokens (1 not enough free
+    pages, 2 ``block_table`` too narrow, 3 past ``max_tokens``)."""
+    return pmkl_pytorch_ext.paged_plan(cached_lens, new_lens, block_table, free_blocks, free_count, block_size,
+                                       max_tokens)
+
+
+def paged_append(k, v, slot_map, k_cache, v_cache, k_scale, v_scale):
+    """Writes new keys and values [tokens, kv_heads, hidden] into the cache.
+
+    ``k_cache``, ``v_cache``: float8_e4m3fn [pages, kv_heads, block, hidden]
+    (any strides with a contiguous last dimension); ``k_scale``, ``v_scale``:
+    float32 [pages, kv_heads], powers of two.  ``slot_map`` int64 as from
+    ``paged_plan``; tokens with a slot of -1 are skipped.  All four cache
+    tensors are updated in place: the scale of a page grows with its rows, and
+    rows written earlier are then rounded again to the larger scale."""
+    pmkl_pytorch_ext.paged_append(k, v, slot_map, k_cache, v_cache, k_scale, v_scale)
+
+
+def paged_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_starts=None, max_query_len=1,
+                    is_causal=True, scale=0.0):
+    """Attention of a step's queries [tokens, heads, hidden] over the cache.
+
+    ``seq_lens`` [batch] counts each request's rows in the cache, the step's
+    own included; request b's queries are rows ``query_starts[b]`` to
+    ``query_starts[b + 1]`` of ``q`` (without ``query_starts``: row b), at most
+    ``max_query_len`` of them, and stand at the end of its rows; with
+    ``is_causal`` each sees the keys up to its own place.  Query head h reads
+    K/V head h // (heads // kv_heads).  ``scale`` <= 0: 1/sqrt(hidden).
+
+    Returns ``out`` like q and ``lse`` [tokens, heads] float32, the log of the
+    sum of the exponentials (-inf, with ``out`` 0, where no key is visible).
+    Forward only: the cache is not differentiable."""
+    return pmkl_pytorch_ext.paged_attention_fw(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens,
+                                               query_starts, max_query_len, is_causal, scale)

@@ -1,0 +1,106 @@
+"""CPU-side checks of the paged 8-bit cache's operators: argument errors of the
+C ABI come before any device work, workspace sizes are host-only, the torch
+binding refuses CPU tensors, and the tests' plain forms agree with torch."""
+import math
+
+import pytest
+import torch
+
+import paged_ref as ref
+import pmkl_b200
+
+FAKE = 0x10000  # non-null, 256-byte aligned, never dereferenced
+
+
+def plan(batch=2, max_blocks=4, block=16, tokens=8, stride=4, cap=3, ptr=FAKE, out=0x20000):
+    return pmkl_b200.capi().pmkl_paged_plan(ptr, ptr, ptr, stride, ptr, ptr, cap, batch, max_blocks, block, tokens, ptr,
+                                            ptr, ptr, out, ptr, None)
+
+
+def test_plan_argument_errors():
+    assert plan(batch=-1) == -1
+    assert plan(block=0) == -1
+    assert plan(tokens=-1) == -1
+    assert plan(tokens=1 << 31) == -1
+    assert plan(stride=3) == -1  # rows overlap
+    assert plan(out=FAKE) == -1  # free_count_out is free_count
+    assert plan(ptr=0) == -3
+    assert plan(out=0) == -3
+
+
+def append(tokens=2, heads=1, hidden=64, dtype=2, blocks=4, block=16, ptr=FAKE, strides=None):
+    return pmkl_b200.capi().pmkl_paged_append(ptr, ptr, strides, None, ptr, tokens, heads, hidden, dtype, ptr, ptr, None,
+                                              None, ptr, ptr, blocks, block, None)
+
+
+def test_append_argument_errors():
+    import ctypes
+    assert append(tokens=-1) == -1
+    assert append(block=0) == -1
+    assert append(dtype=7) == -2
+    assert append(hidden=257) == -5
+    assert append(ptr=0) == -3
+    assert append(strides=(ctypes.c_int64 * 2)(-1, 64)) == -1
+    assert append(tokens=0, ptr=0) == 0 and append(blocks=0, ptr=0) == 0
+
+
+def attend(tokens=2, batch=2, heads=4, kv=2, hidden=64, blocks=4, block=16, width=4, stride=4, max_q=1, dtype=2, kernel=0,
+           ptr=FAKE, starts=FAKE, ws=FAKE, ws_bytes=1 << 40):
+    return pmkl_b200.capi().pmkl_paged_attention(ptr, None, ptr, ptr, None, None, ptr, ptr, ptr, stride, ptr, starts, ptr,
+                                                 None, ptr, tokens, batch, heads, kv, hidden, blocks, block, width, max_q,
+                                                 dtype, 1, 0.0, ws, ws_bytes, kernel, None)
+
+
+def test_attention_argument_errors():
+    assert attend(tokens=-1) == -1
+    assert attend(kv=3) == -1
+    assert attend(kv=0) == -1
+    assert attend(stride=3) == -1
+    assert attend(tokens=3, starts=None) == -1  # one token a request
+    assert attend(block=0) == -1
+    assert attend(dtype=5) == -2
+    assert attend(kernel=77) == -5
+    assert attend(hidden=257) == -5
+    assert attend(ptr=0) == -3
+    assert attend(tokens=0, ptr=0, batch=0) == 0
+
+
+def test_workspace_size_is_zero_for_empty_or_bad_sizes():
+    f = pmkl_b200.capi().pmkl_paged_attention_workspace_size
+    assert f(0, 2, 4, 2, 64, 1, 2) == 0
+    assert f(2, 2, 4, 3, 64, 1, 2) == 0
+    assert f(2, 2, 4, 2, 64, 1, 9) == 0
+    assert f(2, 2, 4, 2, 64, 1, 2) % 256 == 0
+
+
+def test_binding_refuses_cpu_tensors():
+    from pmkl_function import paged_append, paged_attention, paged_plan
+
+    n = torch.ones(1, dtype=torch.int32)
+    c, s = torch.zeros(1, 1, 16, 64).to(torch.float8_e4m3fn), torch.ones(1, 1)
+    x = torch.zeros(1, 1, 64)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        paged_attention(x, c, c, s, s, n[None], n)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        paged_append(x, x, torch.zeros(1, dtype=torch.int64), c, c, s, s)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        paged_plan(n, n, n[None], n, n, 16, 1)
+
+
+def test_plain_forms():
+    """The tests' own references: e4m3 rounding as torch's, attention as softmax of whole matrices."""
+    x = torch.cat([torch.linspace(-500, 500, 4001), torch.linspace(-0.02, 0.02, 4001)]).double()
+    assert torch.equal(ref.e4m3(x), x.float().clamp(-448, 448).to(torch.float8_e4m3fn).double())
+    assert ref.scale_for(448.0) == 1 and ref.scale_for(448.1) == 2 and ref.scale_for(0) == 2.0 ** -64
+    kc, ks = ref.make_cache(3, 1, 4, 8, 1)
+    vc, vs = ref.make_cache(3, 1, 4, 8, 2)
+    q = torch.randn(2, 2, 8, generator=torch.Generator().manual_seed(3))
+    o, lse, _ = ref.attention(q, kc, vc, ks, vs, [[2, 0, 1]], [10], [0, 2])
+    k = torch.cat([kc[p, 0].double() * ks[p, 0].double() for p in (2, 0, 1)])[:10]
+    v = torch.cat([vc[p, 0].double() * vs[p, 0].double() for p in (2, 0, 1)])[:10]
+    for i, keys in ((0, 9), (1, 10)):
+        s = q[i, 1].double() @ k[:keys].T / math.sqrt(8)
+        assert torch.allclose(o[i, 1], torch.softmax(s, 0) @ v[:keys]) and torch.allclose(lse[i, 1], s.logsumexp(0))
+    seq, starts, slots, left, status, table = ref.plan([5, 0], [4, 2], [[7, 8, -1], [-1] * 3], [1, 2, 3], 3, 4, 7)
+    assert (seq, starts, left, status) == ([9, 2], [0, 4, 6], 1, [0, 0])
+    assert table == [[7, 8, 3], [2, -1, -1]] and slots == [33, 34, 35, 12, 8, 9, -1]

@@ -287,7 +287,8 @@ int pmkl_warp_softmax_fwd(void *dst, const void *src, int elements, int stride, 
 /* Kernel selection for pmkl_paged_attention. */
 typedef enum pmkl_paged_kernel {
     PMKL_PAGED_AUTO = 0,
-    PMKL_PAGED_SIMT = 1, /* CUDA cores: any dtype, hidden 1..256, any block size */
+    PMKL_PAGED_SIMT = 1,   /* CUDA cores: any dtype, hidden 1..256, any block size */
+    PMKL_PAGED_STREAM = 2, /* hidden 64 or 128, block_size a multiple of 16, 16-byte aligned cache */
 } pmkl_paged_kernel;
 
 /* Why paged_plan left a request out (status[b]). */

@@ -40,7 +40,8 @@ __device__ __forceinline__ Request request_of(const AttnArgs &p, int b) {
         begin = min(max(p.query_starts[b], 0), p.tokens);
         end = min(max(p.query_starts[b + 1], begin), p.tokens);
     }
-    const long long cap = static_cast<long long>(p.max_blocks) * p.block;
+    // Room above, so that key positions rounded up to a tile stay 32-bit.
+    const long long cap = min(static_cast<long long>(p.max_blocks) * p.block, 0x7FFFFFFFLL - 4096);
     const int len = max(0, p.seq_lens[b]);
     r.first = begin;
     r.rows = min(end - begin, p.max_q);

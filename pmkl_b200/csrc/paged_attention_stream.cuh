@@ -1,0 +1,634 @@
+// paged_attention_stream.cuh -- attention of a few query rows a request over
+// the paged 8-bit cache: head size 64 or 128, pages of a multiple of 16 rows.
+//
+// The rows of a request that read one K/V head (its tokens times the query
+// heads of the group) share one pass over that head's cache, 2 D bytes a key
+// for 4 D FLOP a row: with up to a few tens of rows the cache's bytes are the
+// bound, so the kernel is built to keep loads in flight and nothing else.
+//
+//   * Work is the list of all (request, K/V head, row tile) items, each cut in
+//     tiles of 128 keys; a grid of resident CTAs takes equal shares of the
+//     list, whatever the lengths, a CTA's share beginning and ending inside an
+//     item.  Each CTA finds its share from the lengths itself.  Items that lie
+//     in one CTA are written at once; the others leave normalised partial rows
+//     and their log-sums in the workspace, joined in the list's order by a
+//     second kernel (no atomics: the same bits on every run).
+//   * A warp takes 16 keys at a time, straight from global memory into the
+//     registers that the tensor cores read, with no shared memory between: a
+//     sum over D may run in any order, so thread (g, t) = (lane / 4, lane % 4)
+//     loads 16 consecutive bytes of keys g and g + 8 and the queries are laid
+//     out to match; and output rows may come in any order, so for V it loads 16
+//     consecutive bytes of keys 2t, 2t + 1, 2t + 8, 2t + 9 and pairs up the
+//     bytes of neighbouring keys.  e4m3 values are exact in fp16, which is what
+//     the products take.
+//   * S^T = K Q^T puts keys in rows and queries in columns; its result is
+//     turned into the operand of O^T = V^T P^T by a transposing matrix move.
+//   * Queries are exact in fp16 too: each row is divided by a power of two that
+//     brings its largest value near 2^7 (16-bit types); fp32 queries and
+//     weights are split in two fp16 parts.
+//   * A page's value scale enters the exponent: w = s + log2 vs, p' = 2^(w - M)
+//     rounded to fp16 for the product, and the sum of the softmax takes p' / vs
+//     in fp32.  M is a bound that is raised only when some w passes it by 2^8
+//     (voted per warp), so most tiles reduce nothing across lanes.
+//
+// Rows behind a request's last key may hold anything: their scores are set to
+// -inf by selection and their values to zero.  A key that some rows see and
+// others do not (a later token of the same step) may hold NaN too, which the
+// product would spread as 0 * NaN: tiles at the diagonal look for NaN bytes,
+// and where there are any the product gets zeros for them and the rows that do
+// see the key get their NaN by selection.
+#pragma once
+
+#include "paged_attention_simt.cuh"
+
+namespace pmkl_b200 {
+namespace paged {
+
+constexpr int kStreamWarps = 8;
+constexpr int kStreamThreads = 32 * kStreamWarps;
+constexpr int kTileKeys = 16 * kStreamWarps;  // keys a CTA takes at a time
+constexpr int kMaxStreamCtas = 640;           // partials in the workspace: 148 SMs with up to 4 CTAs
+
+// Workspace: an item descriptor a CTA, then log-sums [2 CTAs][rows], then
+// partial rows [2 CTAs][rows][D].  A CTA's slot 2c holds the item that it
+// enters in the middle, 2c + 1 the item that it begins and does not end.
+struct StreamDesc {
+    int b, item, segments, pad;
+};
+
+struct StreamArgs {
+    AttnArgs a;
+    int vec_q;    // q rows are 16-byte aligned
+    float *part_o, *part_lse;
+    StreamDesc *desc;
+};
+
+__device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t v) {  // the low 16 bits
+    uint32_t r;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ uint32_t e4m3x2_to_h2_hi(uint32_t v) {  // the high 16 bits
+    uint32_t r;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(r) : "r"(v));
+    return r;
+}
+
+// c += a b, a 16 x 16 (rows g, g + 8), b 16 x 8 fp16, c 16 x 8 fp32.
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+        "%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t h2_bits(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float2 h2_floats(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Streaming loads: a step reads the cache once.
+template <int BYTES>
+struct Bytes {
+    uint32_t w[BYTES / 4];
+};
+__device__ __forceinline__ void load_bytes(Bytes<16> &r, const uint8_t *p) {
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3])
+                 : "l"(p));
+}
+__device__ __forceinline__ void load_bytes(Bytes<8> &r, const uint8_t *p) {
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(r.w[0]), "=r"(r.w[1]) : "l"(p));
+}
+
+template <int D, int NT>
+struct StreamCfg {
+    static constexpr int kRows = 8 * NT;
+    static constexpr int kRowPitch = D + 32;  // 4 floats behind every D / 8: a warp's float4 stores meet no bank twice
+    static constexpr int kSmemBytes = (kStreamWarps / 2) * kRows * kRowPitch * 4;
+};
+
+__host__ __device__ constexpr size_t stream_workspace(int rows, int D) {
+    return static_cast<size_t>(kMaxStreamCtas) * (sizeof(StreamDesc) + 2 * static_cast<size_t>(rows) * (D + 1) * 4);
+}
+
+// Key tiles of a request's items: all its row tiles are given the same number,
+// at least one, so that every item has a writer.
+__device__ __forceinline__ int request_tiles(const Request &r) { return max(1, (r.keys + kTileKeys - 1) / kTileKeys); }
+
+template <int ROWS>
+__device__ __forceinline__ int row_tiles(const AttnArgs &p, const Request &r) {
+    return (r.rows * (p.H / p.Hkv) + ROWS - 1) / ROWS;
+}
+
+// 16 consecutive elements of a query row as fp32.
+template <typename T>
+__device__ __forceinline__ void load_q16(float (&x)[16], const T *q, bool vec) {
+    if (vec) {
+        constexpr int N = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < 16; i += N) {
+            const uint4 u = *reinterpret_cast<const uint4 *>(q + i);
+            const T *e = reinterpret_cast<const T *>(&u);
+#pragma unroll
+            for (int j = 0; j < N; ++j) x[i + j] = Elem<T>::to_float(e[j]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = Elem<T>::to_float(q[i]);
+    }
+}
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kStreamThreads, NT == 1 ? 2 : 1) paged_attention_stream_kernel(const StreamArgs sa) {
+    using C = StreamCfg<D, NT>;
+    constexpr bool kSplit = sizeof(T) == 4;  // fp32 queries: two fp16 parts of q and of p
+    constexpr int kParts = kSplit ? 2 : 1;
+    constexpr int kSteps = D / 16;   // products of 16 along D
+    constexpr int kHalves = D / 64;  // 16-byte loads of a key row
+    constexpr int kMt = D / 16;      // 16-row tiles of O^T
+    constexpr int kVBytes = D / 8;   // bytes of a V row a thread
+    extern __shared__ float s_acc[];
+    __shared__ float s_m[kStreamWarps][C::kRows], s_l[kStreamWarps][C::kRows];
+    __shared__ long long s_sum[kStreamWarps];
+    __shared__ long long s_at;
+    __shared__ int s_b;
+    const AttnArgs &p = sa.a;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int group = p.H / p.Hkv;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    clear_tail<T>(p);
+
+    // ---- this CTA's share of the list
+    const auto weight = [&](int b) -> long long {
+        if (b >= p.batch) return 0;
+        const Request r = request_of(p, b);
+        return static_cast<long long>(row_tiles<C::kRows>(p, r)) * p.Hkv * request_tiles(r);
+    };
+    const auto block_inclusive = [&](long long v) -> long long {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += x;
+        }
+        __syncthreads();
+        if (lane == 31) s_sum[warp] = v;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kStreamWarps; ++w)
+            if (w < warp) v += s_sum[w];
+        return v;
+    };
+    const long long w0 = weight(tid);
+    long long total = w0;
+    for (int b = tid + kStreamThreads; b < p.batch; b += kStreamThreads) total += weight(b);
+    block_inclusive(total);
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kStreamWarps; ++w) total += s_sum[w];
+    // As many shares as CTAs, or as tiles where those are fewer: none is empty.
+    const long long shares = min(total, static_cast<long long>(gridDim.x));
+    const bool idle = blockIdx.x >= shares;
+    const long long u_begin = idle ? 0 : total * blockIdx.x / shares;
+    const long long u_end = idle ? 0 : total * (blockIdx.x + 1) / shares;
+    if (u_begin < u_end) {
+        long long before = 0;
+        for (int b0 = 0; b0 < p.batch; b0 += kStreamThreads) {
+            const long long w = b0 ? weight(b0 + tid) : w0;
+            const long long end = block_inclusive(w) + before;
+            if (u_begin >= end - w && u_begin < end) s_b = b0 + tid, s_at = end - w;
+            long long all = 0;
+#pragma unroll
+            for (int x = 0; x < kStreamWarps; ++x) all += s_sum[x];
+            before += all;
+            if (before > u_begin) break;
+        }
+    }
+    if (tid == 0) sa.desc[blockIdx.x].segments = 0;
+    __syncthreads();
+
+    long long u = u_begin;
+    int b = u < u_end ? s_b : 0;
+    long long b_begin = u < u_end ? s_at : 0;
+    while (u < u_end && b < p.batch) {
+        const Request r = request_of(p, b);
+        const int n_rt = row_tiles<C::kRows>(p, r), tiles = request_tiles(r);
+        const long long b_len = static_cast<long long>(n_rt) * p.Hkv * tiles;
+        if (u >= b_begin + b_len) {
+            b_begin += b_len;
+            ++b;
+            continue;
+        }
+        const int item = static_cast<int>((u - b_begin) / tiles);
+        const int tile0 = static_cast<int>((u - b_begin) - static_cast<long long>(item) * tiles);
+        const int tile1 = static_cast<int>(min(static_cast<long long>(tiles), tile0 + (u_end - u)));
+        const int h = item / n_rt, row0 = (item - h * n_rt) * C::kRows;
+        const int n_rows = min(C::kRows, r.rows * group - row0);
+        u += tile1 - tile0;
+
+        // ---- queries, as operands of S^T
+        uint32_t qf[kParts][NT][kSteps][2];
+        float q_scale[NT][2];  // of the columns 2t, 2t + 1: raw product to log2 units
+        int lim[NT][2];        // keys that they see
+        int lim_min = r.keys, lim_max = 0;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int row = row0 + n * 8 + g;
+            const bool real = row < r.rows * group;
+            const int i = row / group;
+            const T *q = static_cast<const T *>(p.q) + (r.first + (real ? i : 0)) * p.q_st[0] +
+                         (h * group + (real ? row - i * group : 0)) * p.q_st[1];
+            float x[kHalves][16];
+            float amax = 0.f;
+#pragma unroll
+            for (int hf = 0; hf < kHalves; ++hf) {
+                load_q16(x[hf], q + hf * 64 + t * 16, sa.vec_q != 0);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    if (!real) x[hf][j] = 0.f;
+                    amax = fmaxf(amax, fabsf(x[hf][j]));
+                }
+            }
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            // The power of two that brings the row's largest value to 2^7 .. 2^8.
+            const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127 - 7, -100), 126);
+            const float down = exp2_int(-e);
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int at = (s & 3) * 4 + j * 2;
+                    const float a = x[s >> 2][at] * down, c = x[s >> 2][at + 1] * down;
+                    qf[0][n][s][j] = h2_bits(a, c);
+                    if constexpr (kSplit) {
+                        const float2 hi = h2_floats(qf[0][n][s][j]);
+                        qf[kParts - 1][n][s][j] = h2_bits(a - hi.x, c - hi.y);
+                    }
+                }
+            const float up = exp2_int(e) * p.scale * 1.4426950408889634f;
+            const int seen = real ? visible(p, r, i) : r.keys;
+            q_scale[n][0] = __shfl_sync(0xffffffffu, up, 8 * t);
+            q_scale[n][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4);
+            lim[n][0] = __shfl_sync(0xffffffffu, seen, 8 * t);
+            lim[n][1] = __shfl_sync(0xffffffffu, seen, 8 * t + 4);
+        }
+        // Rows see more keys the later their token: the first and last real row bound the rest.
+        lim_min = visible(p, r, row0 / group);
+        lim_max = visible(p, r, (row0 + n_rows - 1) / group);
+
+        // ---- this warp's keys: 16 of every tile
+        float acc[kMt][NT][4];
+        float m[NT][2], l[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+            for (int x = 0; x < kMt; ++x) acc[x][n][0] = acc[x][n][1] = acc[x][n][2] = acc[x][n][3] = 0.f;
+        }
+        const int *table = p.table + b * p.table_stride;
+        const int key_end = min(tile1 * kTileKeys, lim_max);
+        int key = tile0 * kTileKeys + warp * 16;
+        // page and row of `key`, advanced by kTileKeys without a division
+        int col = key / p.block, row = key - col * p.block;
+        const int d_col = kTileKeys / p.block, d_row = kTileKeys - d_col * p.block;
+        const auto page_at = [&](int c) -> int {
+            const int x = __ldg(table + c);
+            return x >= 0 && x < p.num_blocks ? x : -1;
+        };
+        Bytes<16> kr[2][kHalves];
+        Bytes<kVBytes> vr[4];
+        const auto load_k = [&](int page, int rw) {
+            const uint8_t *at = p.k.base + page * p.k.s[0] + h * p.k.s[1] + (rw + g) * p.k.s[2] + t * 16;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int hf = 0; hf < kHalves; ++hf) load_bytes(kr[i][hf], at + i * 8 * p.k.s[2] + hf * 64);
+        };
+        const auto load_v = [&](int page, int rw) {
+            const uint8_t *at = p.v.base + page * p.v.s[0] + h * p.v.s[1] + (rw + 2 * t) * p.v.s[2] + g * kVBytes;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) load_bytes(vr[i], at + ((i & 1) + (i >> 1) * 8) * p.v.s[2]);
+        };
+        int page = -1, page_next = -1;
+        float ks = 0.f, vs = 1.f;
+        const auto load_scales = [&](int pg) {
+            ks = __ldg(p.k.scale + static_cast<long long>(pg) * p.Hkv + h);
+            vs = __ldg(p.v.scale + static_cast<long long>(pg) * p.Hkv + h);
+        };
+        const auto step_page = [&](int &c, int &rw) {
+            c += d_col;
+            rw += d_row;
+            if (rw >= p.block) rw -= p.block, ++c;
+        };
+        int col_next = col, row_next = row;
+        if (key < key_end) {
+            page = page_at(col);
+            if (page >= 0) {
+                load_scales(page);
+                load_k(page, row);
+                load_v(page, row);
+            }
+            step_page(col_next, row_next);
+            if (key + kTileKeys < key_end) page_next = page_at(col_next);
+        }
+        for (; key < key_end; key += kTileKeys) {
+            const bool there = page >= 0;
+            // S^T: 16 keys, NT x 8 queries
+            float s[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+            if (there) {
+#pragma unroll
+                for (int x = 0; x < kSteps; ++x) {
+                    const uint32_t lo = kr[0][x >> 2].w[x & 3], hi = kr[1][x >> 2].w[x & 3];
+                    const uint32_t a0 = e4m3x2_to_h2(lo), a2 = e4m3x2_to_h2_hi(lo);
+                    const uint32_t a1 = e4m3x2_to_h2(hi), a3 = e4m3x2_to_h2_hi(hi);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int part = 0; part < kParts; ++part)
+                            mma16816(s[n], a0, a1, a2, a3, qf[part][n][x][0], qf[part][n][x][1]);
+                }
+            }
+            const float ks_now = ks, vs_now = value_scale(vs);
+            const bool more = key + kTileKeys < key_end;
+            if (more && page_next >= 0) {
+                load_k(page_next, row_next);
+                load_scales(page_next);
+            }
+            if (there) {
+                // weights in log2 units, the value scale included
+                const float lv = log2f(vs_now), inv_vs = 1.f / vs_now;
+                const bool edge = key + 16 > lim_min;
+                bool raise = false;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const float f0 = q_scale[n][0] * ks_now, f1 = q_scale[n][1] * ks_now;
+                    s[n][0] = fmaf(s[n][0], f0, lv);
+                    s[n][1] = fmaf(s[n][1], f1, lv);
+                    s[n][2] = fmaf(s[n][2], f0, lv);
+                    s[n][3] = fmaf(s[n][3], f1, lv);
+                    if (edge) {
+                        if (key + g >= lim[n][0]) s[n][0] = -INFINITY;
+                        if (key + g >= lim[n][1]) s[n][1] = -INFINITY;
+                        if (key + g + 8 >= lim[n][0]) s[n][2] = -INFINITY;
+                        if (key + g + 8 >= lim[n][1]) s[n][3] = -INFINITY;
+                    }
+                    raise = raise || fmaxf(s[n][0], s[n][2]) > m[n][0] + 8.f || fmaxf(s[n][1], s[n][3]) > m[n][1] + 8.f;
+                }
+                if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            float top = fmaxf(s[n][c], s[n][c + 2]);
+#pragma unroll
+                            for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                            top = fmaxf(top, m[n][c]);
+                            const float fix = m[n][c] == top ? 1.f : exp2_fast(m[n][c] - top);
+                            m[n][c] = top;
+                            l[n][c] *= fix;
+#pragma unroll
+                            for (int x = 0; x < kMt; ++x) acc[x][n][c] *= fix, acc[x][n][c + 2] *= fix;
+                        }
+                }
+                uint32_t pf[kParts][NT][2];  // P^T, keys along the operand's rows
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const float m0 = m[n][0] == -INFINITY ? 0.f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
+                    const float p0 = exp2_fast(s[n][0] - m0), p1 = exp2_fast(s[n][1] - m1);
+                    const float p2 = exp2_fast(s[n][2] - m0), p3 = exp2_fast(s[n][3] - m1);
+                    l[n][0] = fmaf(p0 + p2, inv_vs, l[n][0]);
+                    l[n][1] = fmaf(p1 + p3, inv_vs, l[n][1]);
+                    const uint32_t a = h2_bits(p0, p1), c = h2_bits(p2, p3);
+                    pf[0][n][0] = transpose8x8(a);
+                    pf[0][n][1] = transpose8x8(c);
+                    if constexpr (kSplit) {
+                        const float2 ah = h2_floats(a), ch = h2_floats(c);
+                        pf[kParts - 1][n][0] = transpose8x8(h2_bits(p0 - ah.x, p1 - ah.y));
+                        pf[kParts - 1][n][1] = transpose8x8(h2_bits(p2 - ch.x, p3 - ch.y));
+                    }
+                }
+                if (edge) {
+                    // Rows behind the last key: zero.
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (key + 2 * t + (i & 1) + (i >> 1) * 8 >= lim_max)
+#pragma unroll
+                            for (int x = 0; x < kVBytes / 4; ++x) vr[i].w[x] = 0;
+                    // NaN in rows that some queries do not see.
+                    bool nan = false;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int x = 0; x < kVBytes / 4; ++x)
+                            nan = nan || __vcmpeq4(vr[i].w[x] & 0x7F7F7F7Fu, 0x7F7F7F7Fu) != 0;
+                    if (__any_sync(0xffffffffu, nan)) {
+                        for (int who = 0; who < 4; ++who)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int k_at = key + 2 * who + (i & 1) + (i >> 1) * 8;
+#pragma unroll
+                                for (int x = 0; x < kVBytes / 4; ++x) {
+                                    const uint32_t bytes = __shfl_sync(0xffffffffu, vr[i].w[x], (lane & 28) + who);
+                                    const uint32_t bad = __vcmpeq4(bytes & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+#pragma unroll
+                                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                        for (int c = 0; c < 2; ++c)
+                                            if (k_at < lim[n][c]) {
+                                                // dim 4x + j: tile 2x + j / 2, row half j % 2
+                                                if (bad & 0x000000FFu) acc[2 * x][n][c] = NAN;
+                                                if (bad & 0x0000FF00u) acc[2 * x][n][c + 2] = NAN;
+                                                if (bad & 0x00FF0000u) acc[2 * x + 1][n][c] = NAN;
+                                                if (bad & 0xFF000000u) acc[2 * x + 1][n][c + 2] = NAN;
+                                            }
+                                }
+                            }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int x = 0; x < kVBytes / 4; ++x)
+                                vr[i].w[x] &= ~__vcmpeq4(vr[i].w[x] & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+                    }
+                }
+                // O^T += V^T P^T
+#pragma unroll
+                for (int x = 0; x < kVBytes / 4; ++x) {
+                    const uint32_t e0 = __byte_perm(vr[0].w[x], vr[1].w[x], 0x5140);  // dims 4x, 4x + 1 of keys 2t, 2t + 1
+                    const uint32_t o0 = __byte_perm(vr[0].w[x], vr[1].w[x], 0x7362);  // dims 4x + 2, 4x + 3
+                    const uint32_t e1 = __byte_perm(vr[2].w[x], vr[3].w[x], 0x5140);  // of keys 2t + 8, 2t + 9
+                    const uint32_t o1 = __byte_perm(vr[2].w[x], vr[3].w[x], 0x7362);
+                    const uint32_t a0 = e4m3x2_to_h2(e0), a1 = e4m3x2_to_h2_hi(e0);
+                    const uint32_t a2 = e4m3x2_to_h2(e1), a3 = e4m3x2_to_h2_hi(e1);
+                    const uint32_t c0 = e4m3x2_to_h2(o0), c1 = e4m3x2_to_h2_hi(o0);
+                    const uint32_t c2 = e4m3x2_to_h2(o1), c3 = e4m3x2_to_h2_hi(o1);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int part = 0; part < kParts; ++part) {
+                            mma16816(acc[2 * x][n], a0, a1, a2, a3, pf[part][n][0], pf[part][n][1]);
+                            mma16816(acc[2 * x + 1][n], c0, c1, c2, c3, pf[part][n][0], pf[part][n][1]);
+                        }
+                }
+            }
+            page = page_next;
+            if (more) {
+                if (page >= 0) load_v(page, row_next);
+                step_page(col_next, row_next);
+                page_next = key + 2 * kTileKeys < key_end ? page_at(col_next) : -1;
+            }
+        }
+
+        // ---- join the warps
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], o);
+                if (g == 0) {
+                    s_m[warp][n * 8 + 2 * t + c] = m[n][c];
+                    s_l[warp][n * 8 + 2 * t + c] = l[n][c];
+                }
+            }
+        __syncthreads();
+        float fix[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < kStreamWarps; ++w) top = fmaxf(top, s_m[w][n * 8 + 2 * t + c]);
+                fix[n][c] = m[n][c] == -INFINITY ? 0.f : exp2_fast(m[n][c] - top);
+            }
+        // Where m is -inf nothing was added (acc is 0 and stays so); NaN passes.
+        float *mine = s_acc + (warp & (kStreamWarps / 2 - 1)) * (C::kRows * C::kRowPitch);
+#pragma unroll
+        for (int round = 0; round < 2; ++round) {
+            if ((warp >= kStreamWarps / 2) == (round == 0)) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        float4 *at = reinterpret_cast<float4 *>(mine + (n * 8 + 2 * t + c) * C::kRowPitch + g * (D / 8 + 4));
+#pragma unroll
+                        for (int x = 0; x < kMt / 2; ++x) {
+                            float4 v = make_float4(acc[2 * x][n][c] * fix[n][c], acc[2 * x][n][c + 2] * fix[n][c],
+                                                   acc[2 * x + 1][n][c] * fix[n][c], acc[2 * x + 1][n][c + 2] * fix[n][c]);
+                            if (round == 1) {
+                                const float4 o = at[x];
+                                v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+                            }
+                            at[x] = v;
+                        }
+                    }
+            }
+            __syncthreads();
+        }
+        const bool whole = tile0 == 0 && tile1 == tiles;
+        const int slot = 2 * blockIdx.x + (tile0 == 0 ? 1 : 0);
+        for (int i = tid; i < n_rows * D; i += kStreamThreads) {
+            const int rw = i / D, d = i - rw * D;
+            float top = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kStreamWarps; ++w) top = fmaxf(top, s_m[w][rw]);
+            float sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < kStreamWarps; ++w) {
+                const float mw = s_m[w][rw];
+                sum += mw == -INFINITY ? s_l[w][rw] : exp2_fast(mw - top) * s_l[w][rw];
+            }
+            float x = 0.f;
+            const float *from = s_acc + rw * C::kRowPitch + d + d / (D / 8) * 4;
+#pragma unroll
+            for (int w = 0; w < kStreamWarps / 2; ++w) x += from[w * C::kRows * C::kRowPitch];
+            x *= sum == 0.f ? 0.f : 1.f / sum;
+            const float lse2 = sum == 0.f ? -INFINITY : top + log2f(sum);
+            if (whole) {
+                const int tok = (row0 + rw) / group, head = h * group + (row0 + rw) - tok * group;
+                const long long token = r.first + tok;
+                static_cast<T *>(p.o)[token * p.o_st[0] + head * p.o_st[1] + d] = Elem<T>::from_float(x);
+                if (p.lse && d == 0) p.lse[token * p.H + head] = lse2 * 0.6931471805599453f;
+            } else {
+                sa.part_o[(static_cast<long long>(slot) * C::kRows + rw) * D + d] = x;
+                if (d == 0) sa.part_lse[slot * C::kRows + rw] = lse2;
+            }
+        }
+        if (tile0 == 0 && !whole && tid == 0) {
+            // Begun here, ended by a later CTA: the one whose share holds the item's last tile.
+            const long long last = b_begin + static_cast<long long>(item + 1) * tiles - 1;
+            long long c1 = last * shares / total;  // within one of the owner
+            while (total * (c1 + 1) / shares <= last) ++c1;
+            while (total * c1 / shares > last) --c1;
+            sa.desc[blockIdx.x] = StreamDesc{b, item, static_cast<int>(c1) - static_cast<int>(blockIdx.x) + 1, 0};
+        }
+        __syncthreads();  // the sums have been read
+    }
+}
+
+// Joins the partial rows of the items that CTA blockIdx.x of the stream kernel
+// began and did not end: row blockIdx.y of the row tile, a thread a column.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(D) paged_attention_join_kernel(const StreamArgs sa) {
+    constexpr int kRows = 8 * NT;
+    __shared__ float s_w[kMaxStreamCtas];
+    __shared__ float s_red[D / 32];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const StreamDesc desc = sa.desc[blockIdx.x];
+    if (desc.segments == 0) return;
+    const AttnArgs &p = sa.a;
+    const Request r = request_of(p, desc.b);
+    const int group = p.H / p.Hkv, n_rt = row_tiles<kRows>(p, r);
+    const int h = desc.item / n_rt, row = (desc.item - h * n_rt) * kRows + blockIdx.y;
+    if (row >= r.rows * group) return;
+    const int tid = threadIdx.x, n = desc.segments;
+    const auto slot = [&](int i) { return i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i); };
+    float top = -INFINITY;
+    for (int i = tid; i < n; i += D) {
+        const float x = sa.part_lse[slot(i) * kRows + blockIdx.y];
+        s_w[i] = x;
+        top = fmaxf(top, x);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if ((tid & 31) == 0) s_red[tid >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < D / 32; ++w) top = fmaxf(top, s_red[w]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, x = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+        const float w = exp2_fast(s_w[i] - base);
+        sum += w;
+        x = fmaf(w, sa.part_o[(static_cast<long long>(slot(i)) * kRows + blockIdx.y) * D + tid], x);
+    }
+    x *= sum == 0.f ? 0.f : 1.f / sum;
+    const int tok = row / group, head = h * group + row - tok * group;
+    const long long token = r.first + tok;
+    static_cast<T *>(p.o)[token * p.o_st[0] + head * p.o_st[1] + tid] = Elem<T>::from_float(x);
+    if (p.lse && tid == 0)
+        p.lse[token * p.H + head] = sum == 0.f ? -INFINITY : (base + log2f(sum)) * 0.6931471805599453f;
+}
+
+}  // namespace paged
+}  // namespace pmkl_b200

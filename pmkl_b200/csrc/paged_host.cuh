@@ -5,6 +5,7 @@
 
 #include "paged_append.cuh"
 #include "paged_attention_simt.cuh"
+#include "paged_attention_stream.cuh"
 #include "paged_plan.cuh"
 
 namespace pmkl_b200 {
@@ -68,8 +69,92 @@ int paged_append_impl(const paged::AppendArgs &p, int dtype, cudaStream_t stream
     });
 }
 
-int paged_attention_impl(const paged::AttnArgs &p, int dtype, int kernel, cudaStream_t stream) {
-    (void)kernel;
+// Rows of a request that share a pass over a K/V head, rounded up to the row
+// tile that the stream kernel takes: 8, 16 or 32.
+int stream_rows(int heads, int kv_heads, int max_q) {
+    const long long rows = static_cast<long long>(heads / kv_heads) * max_q;
+    return rows <= 8 ? 8 : (rows <= 16 ? 16 : 32);
+}
+
+bool stream_applies(const paged::AttnArgs &p) {
+    if ((p.D != 64 && p.D != 128) || p.block % 16 != 0) return false;
+    for (const paged::CacheView *c : {&p.k, &p.v}) {
+        if (!aligned16(c->base)) return false;
+        for (long long s : c->s)
+            if (s % 16 != 0) return false;
+    }
+    return true;
+}
+
+template <typename T, int D, int NT>
+int launch_stream(const paged::AttnArgs &a, void *workspace, cudaStream_t stream) {
+    using C = paged::StreamCfg<D, NT>;
+    static std::once_flag once[kMaxDevices];
+    static int per_sm[kMaxDevices];
+    auto kernel = paged::paged_attention_stream_kernel<T, D, NT>;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    bool ok = true;
+    std::call_once(once[dev], [&]() {
+        int n = 0;
+        ok = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes) == cudaSuccess &&
+             cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, paged::kStreamThreads, C::kSmemBytes) ==
+                 cudaSuccess;
+        per_sm[dev] = ok && n > 0 ? n : 1;
+    });
+    if (!ok) return PMKL_ERR_LAUNCH;
+    paged::StreamArgs p{};
+    p.a = a;
+    const size_t esz = sizeof(T);
+    p.vec_q = aligned16(a.q) && a.q_st[0] * esz % 16 == 0 && a.q_st[1] * esz % 16 == 0;
+    uint8_t *ws = static_cast<uint8_t *>(workspace);
+    p.desc = reinterpret_cast<paged::StreamDesc *>(ws);
+    p.part_lse = reinterpret_cast<float *>(ws + paged::kMaxStreamCtas * sizeof(paged::StreamDesc));
+    p.part_o = p.part_lse + 2 * paged::kMaxStreamCtas * C::kRows;
+    // No more CTAs than tiles that there can be.
+    const long long tiles = std::max<long long>(
+        1, (static_cast<long long>(a.max_blocks) * a.block + paged::kTileKeys - 1) / paged::kTileKeys);
+    const long long row_tiles =
+        (static_cast<long long>(a.H / a.Hkv) * a.max_q + C::kRows - 1) / C::kRows;
+    const long long items = static_cast<long long>(a.batch) * a.Hkv * row_tiles;
+    long long grid = std::min<long long>(static_cast<long long>(sm_count()) * per_sm[dev], paged::kMaxStreamCtas);
+    if (tiles < grid && items * tiles < grid) grid = std::max<long long>(1, items * tiles);
+    kernel<<<static_cast<unsigned>(grid), paged::kStreamThreads, C::kSmemBytes, stream>>>(p);
+    int rc = launch_status();
+    if (rc != PMKL_OK || tiles == 1) return rc;  // an item of one tile lies in one CTA
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(grid),
+                       static_cast<unsigned>(std::min<long long>(C::kRows, static_cast<long long>(a.H / a.Hkv) * a.max_q)));
+    cfg.blockDim = dim3(D);
+    cfg.stream = stream;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, paged::paged_attention_join_kernel<T, D, NT>, p) != cudaSuccess) {
+        cudaGetLastError();
+        return PMKL_ERR_LAUNCH;
+    }
+    return PMKL_OK;
+}
+
+int paged_attention_impl(const paged::AttnArgs &p, int dtype, int kernel, void *workspace, cudaStream_t stream) {
+    const bool can_stream = stream_applies(p);
+    if (kernel == PMKL_PAGED_STREAM && !can_stream) return PMKL_ERR_UNSUPPORTED;
+    if (can_stream && kernel != PMKL_PAGED_SIMT && p.batch > 0 && p.max_q > 0) {
+        const int rows = stream_rows(p.H, p.Hkv, p.max_q);
+        return with_dtype(dtype, [&](auto *t) -> int {
+            using T = std::remove_pointer_t<decltype(t)>;
+            if (p.D == 64)
+                return rows == 8    ? launch_stream<T, 64, 1>(p, workspace, stream)
+                       : rows == 16 ? launch_stream<T, 64, 2>(p, workspace, stream)
+                                    : launch_stream<T, 64, 4>(p, workspace, stream);
+            return rows == 8    ? launch_stream<T, 128, 1>(p, workspace, stream)
+                   : rows == 16 ? launch_stream<T, 128, 2>(p, workspace, stream)
+                                : launch_stream<T, 128, 4>(p, workspace, stream);
+        });
+    }
     const long long units = static_cast<long long>(p.batch) * p.max_q * p.H;
     return with_dtype(dtype, [&](auto *t) -> int {
         using T = std::remove_pointer_t<decltype(t)>;
@@ -153,7 +238,8 @@ size_t pmkl_paged_attention_workspace_size(int tokens, int batch, int heads, int
     if (tokens <= 0 || batch <= 0 || heads <= 0 || kv_heads <= 0 || hidden <= 0 || max_query_len <= 0 ||
         heads % kv_heads != 0 || !dtype_valid(dtype))
         return 0;
-    return 0;
+    if (hidden != 64 && hidden != 128) return 0;  // the CUDA-core kernel needs none
+    return align256(paged::stream_workspace(stream_rows(heads, kv_heads, max_query_len), hidden));
 }
 
 int pmkl_paged_attention(const void *q, const int64_t *q_strides, const void *k_cache, const void *v_cache,
@@ -167,7 +253,7 @@ int pmkl_paged_attention(const void *q, const int64_t *q_strides, const void *k_
         max_blocks < 0 || max_query_len < 0 || table_stride < 0)
         return PMKL_ERR_INVALID_SHAPE;
     if (!dtype_valid(dtype)) return PMKL_ERR_INVALID_DTYPE;
-    if (kernel != PMKL_PAGED_AUTO && kernel != PMKL_PAGED_SIMT) return PMKL_ERR_UNSUPPORTED;
+    if (kernel != PMKL_PAGED_AUTO && kernel != PMKL_PAGED_SIMT && kernel != PMKL_PAGED_STREAM) return PMKL_ERR_UNSUPPORTED;
     if (heads > 0 && (kv_heads == 0 || heads % kv_heads != 0)) return PMKL_ERR_INVALID_SHAPE;
     if (batch > 1 && table_stride < max_blocks) return PMKL_ERR_INVALID_SHAPE;
     if (!query_starts && tokens != batch) return PMKL_ERR_INVALID_SHAPE;
@@ -209,7 +295,7 @@ int pmkl_paged_attention(const void *q, const int64_t *q_strides, const void *k_
     p.max_q = query_starts ? max_query_len : 1;
     p.causal = is_causal ? 1 : 0;
     p.scale = scale > 0.f ? scale : 1.0f / sqrtf(static_cast<float>(hidden));
-    return paged_attention_impl(p, dtype, kernel, static_cast<cudaStream_t>(stream));
+    return paged_attention_impl(p, dtype, kernel, workspace, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -82,5 +82,152 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
     }
 }
 
+// The same for rows of 16-byte vectors, kept in registers between the search
+// for the largest value and the rounding, so that each value is read once.
+//
+// A CTA takes `span` neighbouring tokens of one head.  It lists the runs that
+// begin there (a run may end in the next span), and its warps take them, keys
+// and values apart, WPU warps a run: as many as it takes to hold a page's rows
+// (16 bytes a lane and vector, NV vectors a lane); where a page is larger, the
+// rows beyond are read again, from L2.  CTAs of neighbouring heads run side by
+// side, so that a token's whole row is read at about one time.
+constexpr int kSpanMax = 32;
+
+// Shares of one 16-byte vector: its largest finite magnitude, and its elements
+// divided by a power of two as 8-bit floats.
+template <typename T>
+__device__ __forceinline__ float vec_amax(const uint4 &u) {
+    const T *e = reinterpret_cast<const T *>(&u);
+    float a = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16 / static_cast<int>(sizeof(T)); ++i) a = fmaxf(a, finite_abs(Elem<T>::to_float(e[i])));
+    return a;
+}
+
+__device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d) {
+    uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+    return lo | hi << 16;
+}
+
+template <typename T>
+__device__ __forceinline__ void vec_store(uint8_t *dst, const uint4 &u, float inv) {
+    const T *e = reinterpret_cast<const T *>(&u);
+    uint32_t w[4 / sizeof(T)];
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(4 / sizeof(T)); ++i)
+        w[i] = pack_e4m3(Elem<T>::to_float(e[4 * i]) * inv, Elem<T>::to_float(e[4 * i + 1]) * inv,
+                         Elem<T>::to_float(e[4 * i + 2]) * inv, Elem<T>::to_float(e[4 * i + 3]) * inv);
+    if constexpr (sizeof(T) == 4)
+        *reinterpret_cast<uint32_t *>(dst) = w[0];
+    else
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
+}
+
+template <typename T, int WPU, int NV>
+__global__ void __launch_bounds__(kAppendThreads) paged_append_vec_kernel(const AppendArgs p, int span) {
+    constexpr int kWarps = kAppendThreads / 32, kUnits = kWarps / WPU, kElems = 16 / sizeof(T);
+    __shared__ int s_lead[kSpanMax];
+    __shared__ int s_count;
+    __shared__ float s_max[kWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int h = blockIdx.x % p.kv_heads;
+    const int t0 = blockIdx.x / p.kv_heads * span;
+    if (warp == 0) {
+        const int t = t0 + lane;
+        bool lead = false;
+        if (lane < span && t < p.tokens) {
+            const long long slot = p.slots[t];
+            lead = slot >= 0 && slot < p.num_slots && (t == 0 || slot % p.block == 0 || p.slots[t - 1] != slot - 1);
+        }
+        const unsigned int leads = __ballot_sync(0xffffffffu, lead);
+        if (lead) s_lead[__popc(leads & ((1u << lane) - 1))] = t;
+        if (lane == 0) s_count = __popc(leads);
+    }
+    __syncthreads();
+    const int units = s_count * 2;
+    // Lanes: one vector of a row each, as many rows at a time as fit the unit's lanes.
+    const int per_row = p.hidden / kElems, rows_w = 32 / per_row;
+    const int my_row = lane / per_row, col = (lane - my_row * per_row) * kElems;
+    const bool active = my_row < rows_w;
+    const int sub = warp % WPU, row_first = sub * rows_w + my_row, row_step = rows_w * WPU;
+    for (int u0 = 0; u0 < units; u0 += kUnits) {
+        const int u = u0 + warp / WPU;
+        const bool real = u < units;
+        const int t = real ? s_lead[u >> 1] : t0, side = u & 1;
+        const long long slot = real ? p.slots[t] : 0;
+        const long long page = slot / p.block;
+        const int row = static_cast<int>(slot - page * p.block);
+        const CacheView &c = p.cache[side];
+        float *scale = c.scale + page * p.kv_heads + h;
+        float held = 0.f;
+        if (real && row > 0) held = *scale;
+        int n = real ? 1 : 0;
+        if (real) {
+            const int most = min(p.block - row, p.tokens - t);
+            for (bool all = true; all && n < most; ) {
+                const int i = n + lane;
+                const bool in = i < most && p.slots[t + i] == slot + i;
+                const unsigned int out = __ballot_sync(0xffffffffu, !in);
+                n += out ? __ffs(out) - 1 : 32;
+                all = out == 0;
+            }
+        }
+        const T *x = static_cast<const T *>(p.x[side]) + t * p.x_st[side][0] + h * p.x_st[side][1] + col;
+        const long long x_row = p.x_st[side][0];
+        uint8_t *dst = c.base + page * c.s[0] + h * c.s[1] + col;
+
+        uint4 v[NV];
+        float amax = 0.f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int i = row_first + k * row_step;
+            v[k] = make_uint4(0, 0, 0, 0);
+            if (active && i < n) v[k] = *reinterpret_cast<const uint4 *>(x + i * x_row);
+        }
+        for (int i = row_first + NV * row_step; active && i < n; i += row_step)
+            amax = fmaxf(amax, vec_amax<T>(*reinterpret_cast<const uint4 *>(x + i * x_row)));
+#pragma unroll
+        for (int k = 0; k < NV; ++k) amax = fmaxf(amax, vec_amax<T>(v[k]));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        if constexpr (WPU > 1) {
+            if (lane == 0) s_max[warp] = amax;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < WPU; ++w) amax = fmaxf(amax, s_max[warp - sub + w]);
+            __syncthreads();
+        }
+        if (!real) continue;
+        float s = exp2_int(scale_exponent(amax));
+        if (row > 0) {
+            if (held >= s) {
+                s = held;
+            } else {
+                const float ratio = held / s;
+                for (int i = row_first; active && i < row; i += row_step) {
+                    uint8_t *at = dst + i * c.s[2];
+                    uint32_t *w = reinterpret_cast<uint32_t *>(at);
+#pragma unroll
+                    for (int k = 0; k < static_cast<int>(4 / sizeof(T)); ++k) {
+                        const uint32_t b = w[k];
+                        w[k] = pack_e4m3(e4m3_to_float(b & 255u) * ratio, e4m3_to_float(b >> 8 & 255u) * ratio,
+                                         e4m3_to_float(b >> 16 & 255u) * ratio, e4m3_to_float(b >> 24) * ratio);
+                    }
+                }
+            }
+        }
+        if (sub == 0 && lane == 0) *scale = s;
+        const float inv = 1.f / s;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int i = row_first + k * row_step;
+            if (active && i < n) vec_store<T>(dst + (row + i) * c.s[2], v[k], inv);
+        }
+        for (int i = row_first + NV * row_step; active && i < n; i += row_step)
+            vec_store<T>(dst + (row + i) * c.s[2], *reinterpret_cast<const uint4 *>(x + i * x_row), inv);
+    }
+}
+
 }  // namespace paged
 }  // namespace pmkl_b200

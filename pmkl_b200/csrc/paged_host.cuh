@@ -59,10 +59,46 @@ int paged_plan_impl(const paged::PlanArgs &a, cudaStream_t stream) {
     return launch_status();
 }
 
+template <typename T, int WPU, int NV>
+int launch_append_vec(const paged::AppendArgs &p, cudaStream_t stream) {
+    // Tokens a CTA: 32 (two pages of 16 rows, four runs with keys and values),
+    // fewer where that would leave SMs without a CTA.
+    const long long share = static_cast<long long>(p.tokens) * p.kv_heads / (4LL * sm_count());
+    const int span = static_cast<int>(std::min<long long>(paged::kSpanMax, std::max<long long>(2, share)));
+    const long long grid = (static_cast<long long>(p.tokens) + span - 1) / span * p.kv_heads;
+    if (grid > 0x7FFFFFFFLL) return PMKL_ERR_INVALID_SHAPE;
+    paged::paged_append_vec_kernel<T, WPU, NV>
+        <<<static_cast<unsigned>(grid), paged::kAppendThreads, 0, stream>>>(p, span);
+    return launch_status();
+}
+
+// Rows of whole 16-byte vectors, at most a warp's width of them, at 16-byte
+// addresses; 8-bit rows at multiples of what a lane stores.
+template <typename T>
+bool append_vec_applies(const paged::AppendArgs &p) {
+    constexpr int kElems = 16 / sizeof(T);
+    if (p.hidden % kElems != 0 || p.hidden / kElems > 32) return false;
+    for (int i = 0; i < 2; ++i) {
+        if (!aligned16(p.x[i]) || p.x_st[i][0] % kElems != 0 || p.x_st[i][1] % kElems != 0) return false;
+        if (reinterpret_cast<uintptr_t>(p.cache[i].base) % kElems != 0) return false;
+        for (long long s : p.cache[i].s)
+            if (s % kElems != 0) return false;
+    }
+    return true;
+}
+
 int paged_append_impl(const paged::AppendArgs &p, int dtype, cudaStream_t stream) {
-    const long long units = static_cast<long long>(p.tokens) * p.kv_heads * 2;
     return with_dtype(dtype, [&](auto *t) -> int {
         using T = std::remove_pointer_t<decltype(t)>;
+        if (append_vec_applies<T>(p)) {
+            // A warp holds 4 KiB of a page's rows in 8 vectors a lane.
+            const long long bytes = static_cast<long long>(p.block) * p.hidden * sizeof(T);
+            if (bytes <= 4096) return launch_append_vec<T, 1, 8>(p, stream);
+            if (bytes <= 8192) return launch_append_vec<T, 2, 8>(p, stream);
+            if (bytes <= 16384) return launch_append_vec<T, 4, 8>(p, stream);
+            return launch_append_vec<T, 4, 16>(p, stream);
+        }
+        const long long units = static_cast<long long>(p.tokens) * p.kv_heads * 2;
         paged::paged_append_kernel<T>
             <<<blocks_for(units, paged::kAppendThreads / 32, 16), paged::kAppendThreads, 0, stream>>>(p);
         return launch_status();

@@ -289,6 +289,7 @@ typedef enum pmkl_paged_kernel {
     PMKL_PAGED_AUTO = 0,
     PMKL_PAGED_SIMT = 1,   /* CUDA cores: any dtype, hidden 1..256, any block size */
     PMKL_PAGED_STREAM = 2, /* hidden 64 or 128, block_size a multiple of 16, 16-byte aligned cache */
+    PMKL_PAGED_TCGEN05 = 3, /* the same, fp16/bf16 queries: for many rows a K/V head */
 } pmkl_paged_kernel;
 
 /* Why paged_plan left a request out (status[b]). */

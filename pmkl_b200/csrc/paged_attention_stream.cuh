@@ -58,7 +58,7 @@ struct StreamDesc {
 
 struct StreamArgs {
     AttnArgs a;
-    int vec_q;    // q rows are 16-byte aligned
+    int vec_q, vec_o;  // rows of q, of o are 16-byte aligned
     float *part_o, *part_lse;
     StreamDesc *desc;
 };
@@ -123,8 +123,8 @@ struct StreamCfg {
     static constexpr int kSmemBytes = (kStreamWarps / 2) * kRows * kRowPitch * 4;
 };
 
-__host__ __device__ constexpr size_t stream_workspace(int rows, int D) {
-    return static_cast<size_t>(kMaxStreamCtas) * (sizeof(StreamDesc) + 2 * static_cast<size_t>(rows) * (D + 1) * 4);
+__host__ __device__ constexpr size_t partial_workspace(int ctas, int rows, int D) {
+    return static_cast<size_t>(ctas) * (sizeof(StreamDesc) + 2 * static_cast<size_t>(rows) * (D + 1) * 4);
 }
 
 // Key tiles of a request's items: all its row tiles are given the same number,
@@ -585,11 +585,11 @@ __global__ void __launch_bounds__(kStreamThreads, NT == 1 ? 2 : 1) paged_attenti
     }
 }
 
-// Joins the partial rows of the items that CTA blockIdx.x of the stream kernel
-// began and did not end: row blockIdx.y of the row tile, a thread a column.
-template <typename T, int D, int NT>
+// Joins the partial rows of the item that CTA blockIdx.x of the kernel before
+// began and did not end: rows blockIdx.y, blockIdx.y + gridDim.y, ... of its
+// row tile, a thread a column.
+template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(D) paged_attention_join_kernel(const StreamArgs sa) {
-    constexpr int kRows = 8 * NT;
     __shared__ float s_w[kMaxStreamCtas];
     __shared__ float s_red[D / 32];
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -597,37 +597,40 @@ __global__ void __launch_bounds__(D) paged_attention_join_kernel(const StreamArg
     if (desc.segments == 0) return;
     const AttnArgs &p = sa.a;
     const Request r = request_of(p, desc.b);
-    const int group = p.H / p.Hkv, n_rt = row_tiles<kRows>(p, r);
-    const int h = desc.item / n_rt, row = (desc.item - h * n_rt) * kRows + blockIdx.y;
-    if (row >= r.rows * group) return;
+    const int group = p.H / p.Hkv, n_rt = row_tiles<ROWS>(p, r);
+    const int h = desc.item / n_rt, row0 = (desc.item - h * n_rt) * ROWS;
+    const int n_rows = min(ROWS, r.rows * group - row0);
     const int tid = threadIdx.x, n = desc.segments;
     const auto slot = [&](int i) { return i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i); };
-    float top = -INFINITY;
-    for (int i = tid; i < n; i += D) {
-        const float x = sa.part_lse[slot(i) * kRows + blockIdx.y];
-        s_w[i] = x;
-        top = fmaxf(top, x);
-    }
+    for (int rw = blockIdx.y; rw < n_rows; rw += gridDim.y) {
+        __syncthreads();  // the row before is done
+        float top = -INFINITY;
+        for (int i = tid; i < n; i += D) {
+            const float x = sa.part_lse[slot(i) * ROWS + rw];
+            s_w[i] = x;
+            top = fmaxf(top, x);
+        }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if ((tid & 31) == 0) s_red[tid >> 5] = top;
-    __syncthreads();
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if ((tid & 31) == 0) s_red[tid >> 5] = top;
+        __syncthreads();
 #pragma unroll
-    for (int w = 0; w < D / 32; ++w) top = fmaxf(top, s_red[w]);
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, x = 0.f;
+        for (int w = 0; w < D / 32; ++w) top = fmaxf(top, s_red[w]);
+        const float base = top == -INFINITY ? 0.f : top;
+        float sum = 0.f, x = 0.f;
 #pragma unroll 8
-    for (int i = 0; i < n; ++i) {
-        const float w = exp2_fast(s_w[i] - base);
-        sum += w;
-        x = fmaf(w, sa.part_o[(static_cast<long long>(slot(i)) * kRows + blockIdx.y) * D + tid], x);
+        for (int i = 0; i < n; ++i) {
+            const float w = exp2_fast(s_w[i] - base);
+            sum += w;
+            x = fmaf(w, sa.part_o[(static_cast<long long>(slot(i)) * ROWS + rw) * D + tid], x);
+        }
+        x *= sum == 0.f ? 0.f : 1.f / sum;
+        const int row = row0 + rw, tok = row / group, head = h * group + row - tok * group;
+        const long long token = r.first + tok;
+        static_cast<T *>(p.o)[token * p.o_st[0] + head * p.o_st[1] + tid] = Elem<T>::from_float(x);
+        if (p.lse && tid == 0)
+            p.lse[token * p.H + head] = sum == 0.f ? -INFINITY : (base + log2f(sum)) * 0.6931471805599453f;
     }
-    x *= sum == 0.f ? 0.f : 1.f / sum;
-    const int tok = row / group, head = h * group + row - tok * group;
-    const long long token = r.first + tok;
-    static_cast<T *>(p.o)[token * p.o_st[0] + head * p.o_st[1] + tid] = Elem<T>::from_float(x);
-    if (p.lse && tid == 0)
-        p.lse[token * p.H + head] = sum == 0.f ? -INFINITY : (base + log2f(sum)) * 0.6931471805599453f;
 }
 
 }  // namespace paged

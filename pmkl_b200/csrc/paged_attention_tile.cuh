@@ -1,0 +1,589 @@
+// paged_attention_tile.cuh -- attention of many query rows a request over the
+// paged 8-bit cache on the tcgen05 tensor cores: fp16/bf16 queries, head size
+// 64 or 128, pages of a multiple of 16 rows.
+//
+// The rows that read one K/V head (tokens times the group's query heads) are
+// taken 128 at a time, and the list of (request, K/V head, row tile) items, cut
+// in tiles of 128 keys, is shared out evenly over resident CTAs as in the
+// stream kernel; a row tile's key tiles end with the last key that it sees.
+//
+// A CTA has three warpgroups, which divide its registers between them
+// (setmaxnreg); two CTAs an SM fill each other's gaps:
+//   * warps 4-7 bring the cache in: pages looked up, 8-bit values loaded 16
+//     bytes a thread, a tile ahead in registers, made fp16 (every e4m3 value is
+//     one) and stored as the 128-byte-swizzled tiles that the products read.
+//     No scale is multiplied in: they go with the scores;
+//   * warp 8 issues tcgen05.mma: S = Q K^T, then O += P V with P from tensor
+//     memory.  Products of one thread run in order, so S of the next tile may
+//     be issued over P, and its completion tells that P V is done;
+//   * warps 0-3, a thread a row: the running maximum and sum.  A page's key
+//     scale and the row's factor make one factor for 16 scores, its value scale
+//     enters the exponent (as in the stream kernel); O is rescaled only when
+//     the reference rises by more than 2^8.  They also load the queries and
+//     write the results.
+// Tensor memory (256 columns a CTA): S [0, 128), O [128, 128 + D); P takes S's
+// upper half: scores 64..127 are held in registers when it is written.
+//
+// NaN and rows behind the last key: as in the stream kernel.  Values in tiles
+// at the diagonal are searched for NaN; where there is one, the product gets
+// zeros and the rows that see the key note its columns.
+#pragma once
+
+#include "paged_attention_stream.cuh"
+#include "sm100_ptx.cuh"
+
+namespace pmkl_b200 {
+namespace paged {
+
+constexpr int kTileRows = 128;
+constexpr int kTileThreads = 384;
+// Registers a thread: at launch, and what each warpgroup sets; the three come
+// to the launch's total (the host checks that the build has it).
+constexpr int kTileLaunchRegs = 80, kTileSoftmaxRegs = 120, kTileLoadRegs = 96, kTileIssueRegs = 24;
+static_assert(kTileSoftmaxRegs + kTileLoadRegs + kTileIssueRegs == 3 * kTileLaunchRegs, "register split");
+constexpr int kMaxTileCtas = 320;  // partials in the workspace: 148 SMs with 2 CTAs
+
+template <int D>
+struct TileCfg {
+    static constexpr int kBoxes = D / 64;
+    static constexpr int kTileBytes = kBoxes * 128 * 128;
+    static constexpr int kSmemBytes = 3 * kTileBytes + 1024;
+    static constexpr uint32_t kTmemCols = 256, kColS = 0, kColP = 64, kColO = 128;
+};
+
+struct TileShared {
+    uint64_t q_full, k_full, k_empty, v_full, v_empty, s_full, p_full, o_full, drained;
+    uint32_t tmem;
+    int abort_flag;
+    float2 scale[2][8];  // of 16 keys: key scale, log2 of the value scale (-inf: no page)
+    float inv_vs[2][8];
+    int nan[2];          // the tile's values held NaN, tile number of the CTA + 1
+    long long sum[kTileThreads / 32];
+    long long at;
+    int b;
+};
+
+// One stretch of an item's key tiles.
+struct Segment {
+    Request r;
+    int b, h, item, row0, n_rows, tile0, tile1, tiles;
+    int lim_min, lim_max;  // keys that the first and last row see
+};
+
+// The share of a CTA in the list of items; every warp walks it by itself.
+struct Share {
+    long long total, shares, u, u_end, b_begin;
+    int b;
+};
+
+__device__ __forceinline__ int tile_count(const AttnArgs &p, const Request &r, int row0, int rows, int group) {
+    return max(1, (visible(p, r, (min(row0 + kTileRows, rows) - 1) / group) + 127) / 128);
+}
+
+// Key tiles of all row tiles of a request, for one K/V head.
+__device__ __forceinline__ long long head_tiles(const AttnArgs &p, const Request &r, int group) {
+    const int rows = r.rows * group;
+    long long n = 0;
+    for (int row0 = 0; row0 < rows; row0 += kTileRows) n += tile_count(p, r, row0, rows, group);
+    return n;
+}
+
+__device__ __forceinline__ bool next_segment(const AttnArgs &p, Share &w, Segment &s) {
+    const int group = p.H / p.Hkv;
+    while (w.u < w.u_end && w.b < p.batch) {
+        s.r = request_of(p, w.b);
+        const long long per_head = head_tiles(p, s.r, group), all = per_head * p.Hkv;
+        if (w.u >= w.b_begin + all) {
+            w.b_begin += all;
+            ++w.b;
+            continue;
+        }
+        const int rows = s.r.rows * group;
+        s.b = w.b;
+        s.h = static_cast<int>((w.u - w.b_begin) / per_head);
+        long long left = (w.u - w.b_begin) - s.h * per_head;
+        int rt = 0;
+        s.tiles = tile_count(p, s.r, 0, rows, group);
+        while (left >= s.tiles) {
+            left -= s.tiles;
+            ++rt;
+            s.tiles = tile_count(p, s.r, rt * kTileRows, rows, group);
+        }
+        s.row0 = rt * kTileRows;
+        s.n_rows = min(kTileRows, rows - s.row0);
+        s.item = s.h * ((rows + kTileRows - 1) / kTileRows) + rt;
+        s.tile0 = static_cast<int>(left);
+        s.tile1 = static_cast<int>(min(static_cast<long long>(s.tiles), left + (w.u_end - w.u)));
+        s.lim_min = visible(p, s.r, s.row0 / group);
+        s.lim_max = visible(p, s.r, (s.row0 + s.n_rows - 1) / group);
+        w.u += s.tile1 - s.tile0;
+        return true;
+    }
+    return false;
+}
+
+// tcgen05.wait::ld that the values pass through, so that no use of them is
+// moved before it.
+__device__ __forceinline__ void tmem_arrived(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                   "+r"(r[15])
+                 :
+                 : "memory");
+    asm volatile(""
+                 : "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                   "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                   "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+
+// Largest of 16 scores.
+__device__ __forceinline__ float max16(const uint32_t *r) {
+    float m = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+#pragma unroll
+    for (int i = 2; i < 16; i += 2) m = ptx::fmax3(m, __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+    return m;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(const StreamArgs sa) {
+    using namespace ptx;
+    using C = TileCfg<D>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ TileShared sh;
+    uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t *sQ = smem, *sK = smem + C::kTileBytes, *sV = smem + 2 * C::kTileBytes;
+    const AttnArgs &p = sa.a;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int group = p.H / p.Hkv;
+    volatile int *abort_flag = &sh.abort_flag;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    clear_tail<T>(p);
+
+    // ---- set-up: barriers, tensor memory, this CTA's share
+    if (tid == 0) {
+        mbar_init(&sh.q_full, 128);
+        mbar_init(&sh.k_full, 128);
+        mbar_init(&sh.k_empty, 1);
+        mbar_init(&sh.v_full, 128);
+        mbar_init(&sh.v_empty, 1);
+        mbar_init(&sh.s_full, 1);
+        mbar_init(&sh.p_full, 128);
+        mbar_init(&sh.o_full, 1);
+        mbar_init(&sh.drained, 1);
+        sh.nan[0] = sh.nan[1] = 0;
+        // Once any CTA has given up a wait, later CTAs skip their work.
+        sh.abort_flag = (*reinterpret_cast<volatile unsigned int *>(&g_device_error) != 0u) ? 1 : 0;
+        sa.desc[blockIdx.x].segments = 0;
+        fence_mbarrier_init();
+    }
+    if (warp == 8) {
+        tmem_alloc(&sh.tmem, C::kTmemCols);
+        tmem_relinquish();
+    }
+    const auto weight = [&](int b) -> long long {
+        return b < p.batch ? head_tiles(p, request_of(p, b), group) * p.Hkv : 0;
+    };
+    const auto block_inclusive = [&](long long v) -> long long {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += x;
+        }
+        __syncthreads();
+        if (lane == 31) sh.sum[warp] = v;
+        __syncthreads();
+        for (int w = 0; w < warp; ++w) v += sh.sum[w];
+        return v;
+    };
+    Share mine{};
+    {
+        const long long w0 = weight(tid);
+        long long part = w0;
+        for (int b = tid + kTileThreads; b < p.batch; b += kTileThreads) part += weight(b);
+        block_inclusive(part);
+        for (int w = 0; w < kTileThreads / 32; ++w) mine.total += sh.sum[w];
+        // As many shares as CTAs, or as tiles where those are fewer: none is empty.
+        mine.shares = min(mine.total, static_cast<long long>(gridDim.x));
+        const bool idle = blockIdx.x >= mine.shares;
+        mine.u = idle ? 0 : mine.total * blockIdx.x / mine.shares;
+        mine.u_end = idle ? 0 : mine.total * (blockIdx.x + 1) / mine.shares;
+        if (mine.u < mine.u_end) {
+            long long before = 0;
+            for (int b0 = 0; b0 < p.batch; b0 += kTileThreads) {
+                const long long w = b0 ? weight(b0 + tid) : w0;
+                const long long end = block_inclusive(w) + before;
+                if (mine.u >= end - w && mine.u < end) sh.b = b0 + tid, sh.at = end - w;
+                for (int x = 0; x < kTileThreads / 32; ++x) before += sh.sum[x];
+                if (before > mine.u) break;
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+    const bool skip = *abort_flag != 0;
+    if (mine.u < mine.u_end) mine.b = sh.b, mine.b_begin = sh.at;
+
+    Segment s;
+    if (warp >= 8) {
+        // ------------------------------------------------------------ products
+        reg_dealloc<kTileIssueRegs>();
+        if (warp == 8 && lane == 0 && !skip) {
+            constexpr uint32_t kIdescS = idesc_f16(128, 128, 0, 0, 0);
+            constexpr uint32_t kIdescO = idesc_f16(128, D, 0, 0, 1);
+            const uint32_t q_addr = smem_u32(sQ), k_addr = smem_u32(sK), v_addr = smem_u32(sV);
+            uint32_t it = 0, seg = 0;
+            bool ok = true;
+            while (ok && next_segment(p, mine, s)) {
+                ok = mbar_wait(&sh.q_full, seg & 1, abort_flag);
+                for (int j = s.tile0; ok && j < s.tile1; ++j, ++it) {
+                    if (!(ok = mbar_wait(&sh.k_full, it & 1, abort_flag))) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        const uint32_t off = (kk >> 2) * (128 * 128) + (kk & 3) * 32;
+                        mma_ss(tmem + C::kColS, smem_desc_sw128(q_addr + off, 16, 1024),
+                               smem_desc_sw128(k_addr + off, 16, 1024), kIdescS, kk > 0 ? 1u : 0u);
+                    }
+                    mma_commit(&sh.s_full);
+                    mma_commit(&sh.k_empty);
+                    if (!(ok = mbar_wait(&sh.v_full, it & 1, abort_flag))) break;
+                    if (!(ok = mbar_wait(&sh.p_full, it & 1, abort_flag))) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int kk = 0; kk < 8; ++kk)
+                        mma_ts(tmem + C::kColO, tmem + C::kColP + kk * 8,
+                               smem_desc_sw128(v_addr + kk * 16 * 128, 128 * 128, 1024), kIdescO,
+                               (j > s.tile0 || kk > 0) ? 1u : 0u);
+                    mma_commit(&sh.v_empty);
+                }
+                if (ok) mma_commit(&sh.o_full);
+                ++seg;
+            }
+            // Every product has ended before tensor memory is given back.
+            mma_commit(&sh.drained);
+            volatile int never = 0;
+            mbar_wait(&sh.drained, 0, &never);
+        }
+    } else if (warp >= 4) {
+        // ------------------------------------------------------------ cache to shared memory
+        reg_alloc<kTileLoadRegs>();
+        constexpr int kPerRow = D / 16;              // threads a key row
+        constexpr int kRowsPass = 128 / kPerRow;     // key rows a pass
+        constexpr int kPasses = 128 / kRowsPass;
+        const int t = tid - 128, sub = t / kPerRow, chunk = t % kPerRow;
+        uint32_t it = 0;
+        bool ok = !skip;
+        while (ok && next_segment(p, mine, s)) {
+            const int *table = p.table + s.b * p.table_stride;
+            // Page (-1: none) and row of the tile's 16-key groups, lane i of 8 the i-th.
+            const auto find = [&](int j, int &page, int &row) {
+                const int key = j * 128 + (lane & 7) * 16;
+                page = -1, row = 0;
+                if (key < s.lim_max) {
+                    const int c = key / p.block;
+                    row = key - c * p.block;
+                    const int x = __ldg(table + c);
+                    page = x >= 0 && x < p.num_blocks ? x : -1;
+                }
+            };
+            const auto load = [&](const CacheView &c, int page, int row, int key_end, uint4 (&v)[kPasses]) {
+#pragma unroll
+                for (int i = 0; i < kPasses; ++i) {
+                    const int key = i * kRowsPass + sub;
+                    const int pg = __shfl_sync(0xffffffffu, page, key >> 4), rw = __shfl_sync(0xffffffffu, row, key >> 4);
+                    v[i] = make_uint4(0, 0, 0, 0);
+                    if (pg >= 0 && key < key_end) {
+                        Bytes<16> x;
+                        load_bytes(x, c.base + pg * c.s[0] + s.h * c.s[1] + (rw + (key & 15)) * c.s[2] + chunk * 16);
+                        v[i] = make_uint4(x.w[0], x.w[1], x.w[2], x.w[3]);
+                    }
+                }
+            };
+            const auto store = [&](uint8_t *tile, const uint4 (&v)[kPasses]) {
+#pragma unroll
+                for (int i = 0; i < kPasses; ++i) {
+                    const int key = i * kRowsPass + sub;
+                    uint8_t *box = tile + (chunk >> 2) * (128 * 128) + key * 128;
+                    const int c = (chunk & 3) * 2, x = key & 7;
+                    const uint4 a = make_uint4(e4m3x2_to_h2(v[i].x), e4m3x2_to_h2_hi(v[i].x), e4m3x2_to_h2(v[i].y),
+                                               e4m3x2_to_h2_hi(v[i].y));
+                    const uint4 b = make_uint4(e4m3x2_to_h2(v[i].z), e4m3x2_to_h2_hi(v[i].z), e4m3x2_to_h2(v[i].w),
+                                               e4m3x2_to_h2_hi(v[i].w));
+                    // The second box's threads store their halves in the other order: no bank meets twice.
+                    const bool swap = (chunk >> 2) != 0;
+                    *reinterpret_cast<uint4 *>(box + (((c + (swap ? 1 : 0)) ^ x) << 4)) = swap ? b : a;
+                    *reinterpret_cast<uint4 *>(box + (((c + (swap ? 0 : 1)) ^ x) << 4)) = swap ? a : b;
+                }
+            };
+            int page, row, page_n = -1, row_n = 0;
+            find(s.tile0, page, row);
+            uint4 kv[kPasses], vv[kPasses];
+            load(p.k, page, row, 128, kv);
+            for (int j = s.tile0; j < s.tile1; ++j, ++it) {
+                const int left = s.lim_max - j * 128;  // keys of this tile that some row sees
+                load(p.v, page, row, left, vv);
+                float ks = 1.f, vs = 1.f;  // no page: any factor but 0, for masked scores are -inf
+                const bool scales = warp == 4 && lane < 8;
+                if (scales && page >= 0) {
+                    ks = __ldg(p.k.scale + static_cast<long long>(page) * p.Hkv + s.h);
+                    vs = value_scale(__ldg(p.v.scale + static_cast<long long>(page) * p.Hkv + s.h));
+                }
+                if (j + 1 < s.tile1) find(j + 1, page_n, row_n);
+                if (it > 0 && !(ok = mbar_wait_warp_all(&sh.k_empty, (it - 1) & 1, abort_flag))) break;
+                store(sK, kv);
+                if (scales) {
+                    sh.scale[it & 1][lane] = make_float2(ks, page >= 0 ? log2f(vs) : -INFINITY);
+                    sh.inv_vs[it & 1][lane] = 1.f / vs;
+                }
+                fence_proxy_async_smem();
+                mbar_arrive(&sh.k_full);
+                if (j + 1 < s.tile1) load(p.k, page_n, row_n, 128, kv);
+                if (j * 128 + 128 > s.lim_min) {
+                    bool nan = false;
+#pragma unroll
+                    for (int i = 0; i < kPasses; ++i) {
+                        const uint32_t w[4] = {vv[i].x, vv[i].y, vv[i].z, vv[i].w};
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) nan = nan || __vcmpeq4(w[x] & 0x7F7F7F7Fu, 0x7F7F7F7Fu) != 0;
+                    }
+                    if (nan) {
+                        sh.nan[it & 1] = static_cast<int>(it) + 1;
+#pragma unroll
+                        for (int i = 0; i < kPasses; ++i) {
+                            vv[i].x &= ~__vcmpeq4(vv[i].x & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+                            vv[i].y &= ~__vcmpeq4(vv[i].y & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+                            vv[i].z &= ~__vcmpeq4(vv[i].z & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+                            vv[i].w &= ~__vcmpeq4(vv[i].w & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+                        }
+                    }
+                }
+                if (it > 0 && !(ok = mbar_wait_warp_all(&sh.v_empty, (it - 1) & 1, abort_flag))) break;
+                store(sV, vv);
+                fence_proxy_async_smem();
+                mbar_arrive(&sh.v_full);
+                page = page_n;
+                row = row_n;
+            }
+        }
+    } else {
+        // ------------------------------------------------------------ softmax, a thread a row
+        reg_alloc<kTileSoftmaxRegs>();
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+        uint32_t it = 0, seg = 0;
+        bool ok = !skip;
+        while (ok && next_segment(p, mine, s)) {
+            const int rr = s.row0 + tid;
+            const bool real = tid < s.n_rows;
+            const int tok = real ? rr / group : 0, head = s.h * group + (real ? rr - tok * group : 0);
+            const T *q = static_cast<const T *>(p.q) + (s.r.first + tok) * p.q_st[0] + head * p.q_st[1];
+            // The row's largest value, then the row over the power of two that brings it to 2^7 .. 2^8.
+            float amax = 0.f;
+            if (real)
+#pragma unroll 2
+                for (int c = 0; c < D; c += 16) {
+                    float x[16];
+                    load_q16(x, q + c, sa.vec_q != 0);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(x[i]));
+                }
+            const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127 - 7, -100), 126);
+            const float down = exp2_int(-e), up = exp2_int(e) * p.scale * 1.4426950408889634f;
+#pragma unroll 2
+            for (int c = 0; c < D; c += 16) {
+                float x[16];
+                if (real) load_q16(x, q + c, sa.vec_q != 0);
+                uint32_t w[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w[i] = real ? h2_bits(x[2 * i] * down, x[2 * i + 1] * down) : 0u;
+                uint8_t *box = sQ + (c >> 6) * (128 * 128) + tid * 128;
+                const int at = (c & 63) >> 3;
+                *reinterpret_cast<uint4 *>(box + (((at) ^ (tid & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                *reinterpret_cast<uint4 *>(box + (((at + 1) ^ (tid & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&sh.q_full);
+
+            const int lim = real ? visible(p, s.r, tok) : s.r.keys;
+            const bool busy = warp * 32 < s.n_rows;  // some row of this warp is one
+            float m = -INFINITY, l = 0.f;
+            uint32_t nan_cols[D / 32] = {};
+            for (int j = s.tile0; j < s.tile1; ++j, ++it) {
+                // The tile's scales were written before its keys were handed to the
+                // product whose end this is.
+                if (!(ok = mbar_wait_warp_all(&sh.s_full, it & 1, abort_flag))) break;
+                tc_fence_after();
+                if (busy) {
+                    const float2 *scale = sh.scale[it & 1];
+                    const float *inv_vs = sh.inv_vs[it & 1];
+                    const int seen = lim - j * 128;  // columns of this tile that the row sees
+                    const bool edge = j * 128 + 128 > s.lim_min;
+                    uint32_t a[32], b[32], c[32];
+                    const auto mask = [&](uint32_t (&r)[32], int base) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (base + i >= seen) r[i] = 0xFF800000u;  // -inf
+                    };
+                    float top = -INFINITY;
+                    const auto gather = [&](uint32_t (&r)[32], int base) {
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const float2 sc = scale[base / 16 + x];
+                            top = fmaxf(top, fmaf(max16(r + 16 * x), up * sc.x, sc.y));
+                        }
+                    };
+                    tmem_ld32(lanes + C::kColS, a);
+                    tmem_ld32(lanes + C::kColS + 32, b);
+                    tmem_arrived(a);
+                    tmem_arrived(b);
+                    tmem_ld32(lanes + C::kColS + 64, c);
+                    if (edge) mask(a, 0), mask(b, 32);
+                    gather(a, 0);
+                    gather(b, 32);
+                    tmem_ld32(lanes + C::kColS + 96, b);
+                    tmem_arrived(c);
+                    tmem_arrived(b);
+                    if (edge) mask(c, 64), mask(b, 96);
+                    gather(c, 64);
+                    gather(b, 96);
+                    const bool raise = top > m + 8.f;
+                    if (__any_sync(0xffffffffu, raise)) {
+                        const float fix = !raise || m == -INFINITY ? (raise ? 0.f : 1.f) : exp2_fast(m - top);
+                        if (raise) m = top;
+                        l *= fix;
+                        if (j > s.tile0) {
+#pragma unroll
+                            for (int x = 0; x < D / 32; ++x) {
+                                tmem_ld32(lanes + C::kColO + x * 32, a);
+                                tmem_arrived(a);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) a[i] = __float_as_uint(__uint_as_float(a[i]) * fix);
+                                tmem_st32(lanes + C::kColO + x * 32, a);
+                            }
+                        }
+                    }
+                    const float base_m = m == -INFINITY ? 0.f : m;
+                    const auto weigh = [&](uint32_t (&r)[32], int base) {
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const float2 sc = scale[base / 16 + x];
+                            const float f = up * sc.x, off = sc.y - base_m;
+                            float sum = 0.f;
+                            uint32_t w[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const float p0 = exp2_fast(fmaf(__uint_as_float(r[16 * x + 2 * i]), f, off));
+                                const float p1 = exp2_fast(fmaf(__uint_as_float(r[16 * x + 2 * i + 1]), f, off));
+                                sum += p0 + p1;
+                                w[i] = h2_bits(p0, p1);
+                            }
+                            l = fmaf(sum, inv_vs[base / 16 + x], l);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) r[8 * x + i] = w[i];
+                        }
+                        tmem_st16(lanes + C::kColP + base / 2, r);
+                    };
+                    weigh(c, 64);
+                    tmem_ld32(lanes + C::kColS, a);
+                    weigh(b, 96);
+                    tmem_ld32(lanes + C::kColS + 32, b);
+                    tmem_arrived(a);
+                    tmem_arrived(b);
+                    if (edge) mask(a, 0), mask(b, 32);
+                    weigh(a, 0);
+                    weigh(b, 32);
+                    tmem_wait_st();
+                    if (edge) {
+                        // Values with NaN in this tile: the columns of the keys that this row sees.
+                        if (!(ok = mbar_wait_warp_all(&sh.v_full, it & 1, abort_flag))) break;
+                        if (*static_cast<volatile int *>(&sh.nan[it & 1]) == static_cast<int>(it) + 1) {
+                            const int *table = p.table + s.b * p.table_stride;
+                            const int end = min(lim, j * 128 + 128);
+                            for (int key = j * 128; real && key < end; ++key) {
+                                const int col = key / p.block, page = table[col];
+                                if (page < 0 || page >= p.num_blocks) continue;
+                                const uint8_t *v = p.v.base + page * p.v.s[0] + s.h * p.v.s[1] + (key - col * p.block) * p.v.s[2];
+#pragma unroll
+                                for (int x = 0; x < D / 32; ++x)
+                                    for (int i = 0; i < 32; ++i)
+                                        if ((v[x * 32 + i] & 0x7F) == 0x7F) nan_cols[x] |= 1u << i;
+                            }
+                        }
+                    }
+                }
+                tc_fence_before();
+                mbar_arrive(&sh.p_full);
+            }
+            if (!ok || !(ok = mbar_wait_warp_all(&sh.o_full, seg & 1, abort_flag))) break;
+            ++seg;
+            tc_fence_after();
+            if (busy) {
+                const bool whole = s.tile0 == 0 && s.tile1 == s.tiles;
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                const float lse2 = l == 0.f ? -INFINITY : m + log2f(l);
+                const int slot = 2 * blockIdx.x + (s.tile0 == 0 ? 1 : 0);
+                const long long token = s.r.first + tok;
+#pragma unroll
+                for (int x = 0; x < D / 32; ++x) {
+                    uint32_t o[32];
+                    tmem_ld32(lanes + C::kColO + x * 32, o);
+                    tmem_arrived(o);
+                    if (!real) continue;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const float y = __uint_as_float(o[i]) * inv;
+                        o[i] = __float_as_uint(nan_cols[x] >> i & 1u ? NAN : y);
+                    }
+                    if (whole) {
+                        T *to = static_cast<T *>(p.o) + token * p.o_st[0] + head * p.o_st[1] + x * 32;
+                        if (sa.vec_o) {
+#pragma unroll
+                            for (int i = 0; i < 32; i += 8) {
+                                uint4 w;
+                                T *h = reinterpret_cast<T *>(&w);
+#pragma unroll
+                                for (int k = 0; k < 8; ++k) h[k] = Elem<T>::from_float(__uint_as_float(o[i + k]));
+                                *reinterpret_cast<uint4 *>(to + i) = w;
+                            }
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) to[i] = Elem<T>::from_float(__uint_as_float(o[i]));
+                        }
+                    } else {
+                        float *to = sa.part_o + (static_cast<long long>(slot) * kTileRows + tid) * D + x * 32;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4)
+                            *reinterpret_cast<uint4 *>(to + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    }
+                }
+                if (real && whole && p.lse) p.lse[token * p.H + head] = lse2 * 0.6931471805599453f;
+                if (real && !whole) sa.part_lse[slot * kTileRows + tid] = lse2;
+                if (tid == 0 && s.tile0 == 0 && !whole) {
+                    // Begun here, ended by the CTA whose share holds the item's last tile.
+                    const long long last = mine.u + (s.tiles - s.tile1) - 1;
+                    long long c1 = last * mine.shares / mine.total;  // within one of the owner
+                    while (mine.total * (c1 + 1) / mine.shares <= last) ++c1;
+                    while (mine.total * c1 / mine.shares > last) --c1;
+                    sa.desc[blockIdx.x] = StreamDesc{s.b, s.item, static_cast<int>(c1) - static_cast<int>(blockIdx.x) + 1, 0};
+                }
+                tc_fence_before();
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem, C::kTmemCols);
+    }
+    if (tid == 0 && *abort_flag && !skip) report_device_error(PMKL_DEVERR_TIMEOUT);
+}
+
+}  // namespace paged
+}  // namespace pmkl_b200

@@ -6,6 +6,7 @@
 #include "paged_append.cuh"
 #include "paged_attention_simt.cuh"
 #include "paged_attention_stream.cuh"
+#include "paged_attention_tile.cuh"
 #include "paged_plan.cuh"
 
 namespace pmkl_b200 {
@@ -122,45 +123,35 @@ bool stream_applies(const paged::AttnArgs &p) {
     return true;
 }
 
-template <typename T, int D, int NT>
-int launch_stream(const paged::AttnArgs &a, void *workspace, cudaStream_t stream) {
-    using C = paged::StreamCfg<D, NT>;
-    static std::once_flag once[kMaxDevices];
-    static int per_sm[kMaxDevices];
-    auto kernel = paged::paged_attention_stream_kernel<T, D, NT>;
-    int dev = 0;
-    cudaGetDevice(&dev);
-    bool ok = true;
-    std::call_once(once[dev], [&]() {
-        int n = 0;
-        ok = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes) == cudaSuccess &&
-             cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, paged::kStreamThreads, C::kSmemBytes) ==
-                 cudaSuccess;
-        per_sm[dev] = ok && n > 0 ? n : 1;
-    });
-    if (!ok) return PMKL_ERR_LAUNCH;
+// Grid of a kernel that shares out `items` of at most `tiles` tiles each over
+// resident CTAs (`resident`, at most `most`): no more CTAs than tiles.
+long long share_grid(long long resident, long long most, long long items, long long tiles) {
+    const long long grid = std::min(resident, most);
+    return tiles < grid && items * tiles < grid ? std::max<long long>(1, items * tiles) : grid;
+}
+
+// Workspace addresses and alignments of the shared-out kernels.
+template <typename T>
+paged::StreamArgs shared_args(const paged::AttnArgs &a, void *workspace, int ctas, int rows) {
     paged::StreamArgs p{};
     p.a = a;
-    const size_t esz = sizeof(T);
-    p.vec_q = aligned16(a.q) && a.q_st[0] * esz % 16 == 0 && a.q_st[1] * esz % 16 == 0;
+    constexpr long long kVec = 16 / sizeof(T);
+    p.vec_q = aligned16(a.q) && a.q_st[0] % kVec == 0 && a.q_st[1] % kVec == 0;
+    p.vec_o = aligned16(a.o) && a.o_st[0] % kVec == 0 && a.o_st[1] % kVec == 0;
     uint8_t *ws = static_cast<uint8_t *>(workspace);
     p.desc = reinterpret_cast<paged::StreamDesc *>(ws);
-    p.part_lse = reinterpret_cast<float *>(ws + paged::kMaxStreamCtas * sizeof(paged::StreamDesc));
-    p.part_o = p.part_lse + 2 * paged::kMaxStreamCtas * C::kRows;
-    // No more CTAs than tiles that there can be.
-    const long long tiles = std::max<long long>(
-        1, (static_cast<long long>(a.max_blocks) * a.block + paged::kTileKeys - 1) / paged::kTileKeys);
-    const long long row_tiles =
-        (static_cast<long long>(a.H / a.Hkv) * a.max_q + C::kRows - 1) / C::kRows;
-    const long long items = static_cast<long long>(a.batch) * a.Hkv * row_tiles;
-    long long grid = std::min<long long>(static_cast<long long>(sm_count()) * per_sm[dev], paged::kMaxStreamCtas);
-    if (tiles < grid && items * tiles < grid) grid = std::max<long long>(1, items * tiles);
-    kernel<<<static_cast<unsigned>(grid), paged::kStreamThreads, C::kSmemBytes, stream>>>(p);
-    int rc = launch_status();
-    if (rc != PMKL_OK || tiles == 1) return rc;  // an item of one tile lies in one CTA
+    p.part_lse = reinterpret_cast<float *>(ws + ctas * sizeof(paged::StreamDesc));
+    p.part_o = p.part_lse + 2LL * ctas * rows;
+    return p;
+}
+
+// The join may be set up while the kernel before it runs; it waits for its end
+// on the device.
+template <typename T, int D, int ROWS>
+int launch_join(const paged::StreamArgs &p, long long grid, cudaStream_t stream) {
+    const long long rows = std::min<long long>(ROWS, static_cast<long long>(p.a.H / p.a.Hkv) * p.a.max_q);
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(grid),
-                       static_cast<unsigned>(std::min<long long>(C::kRows, static_cast<long long>(a.H / a.Hkv) * a.max_q)));
+    cfg.gridDim = dim3(static_cast<unsigned>(grid), static_cast<unsigned>(std::min<long long>(rows, 16)));
     cfg.blockDim = dim3(D);
     cfg.stream = stream;
     cudaLaunchAttribute early{};
@@ -168,17 +159,101 @@ int launch_stream(const paged::AttnArgs &a, void *workspace, cudaStream_t stream
     early.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &early;
     cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, paged::paged_attention_join_kernel<T, D, NT>, p) != cudaSuccess) {
+    if (cudaLaunchKernelEx(&cfg, paged::paged_attention_join_kernel<T, D, ROWS>, p) != cudaSuccess) {
         cudaGetLastError();
         return PMKL_ERR_LAUNCH;
     }
     return PMKL_OK;
 }
 
+// Dynamic shared memory allowed, and CTAs an SM, asked once a device.
+struct Occupancy {
+    std::once_flag once[kMaxDevices];
+    int per_sm[kMaxDevices] = {};
+    template <typename K>
+    int get(K kernel, int threads, int smem) {
+        int dev = 0;
+        cudaGetDevice(&dev);
+        std::call_once(once[dev], [&]() {
+            int n = 0;
+            if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess &&
+                cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) == cudaSuccess)
+                per_sm[dev] = n;
+            else
+                cudaGetLastError();
+        });
+        return per_sm[dev];
+    }
+};
+
+template <typename T, int D, int NT>
+int launch_stream(const paged::AttnArgs &a, void *workspace, cudaStream_t stream) {
+    using C = paged::StreamCfg<D, NT>;
+    static Occupancy occupancy;
+    auto kernel = paged::paged_attention_stream_kernel<T, D, NT>;
+    const int per_sm = occupancy.get(kernel, paged::kStreamThreads, C::kSmemBytes);
+    if (per_sm < 1) return PMKL_ERR_LAUNCH;
+    const paged::StreamArgs p = shared_args<T>(a, workspace, paged::kMaxStreamCtas, C::kRows);
+    const long long tiles = std::max<long long>(
+        1, (static_cast<long long>(a.max_blocks) * a.block + paged::kTileKeys - 1) / paged::kTileKeys);
+    const long long row_tiles = (static_cast<long long>(a.H / a.Hkv) * a.max_q + C::kRows - 1) / C::kRows;
+    const long long grid = share_grid(static_cast<long long>(sm_count()) * per_sm, paged::kMaxStreamCtas,
+                                      static_cast<long long>(a.batch) * a.Hkv * row_tiles, tiles);
+    kernel<<<static_cast<unsigned>(grid), paged::kStreamThreads, C::kSmemBytes, stream>>>(p);
+    const int rc = launch_status();
+    if (rc != PMKL_OK || tiles == 1) return rc;  // an item of one tile lies in one CTA
+    return launch_join<T, D, C::kRows>(p, grid, stream);
+}
+
+// The tile kernel divides its registers between its warpgroups, which needs
+// the count it was written for; asked once a process.
+template <typename T, int D>
+bool tile_launchable() {
+    static const bool ok = []() {
+        cudaFuncAttributes attr;
+        const bool got = cudaFuncGetAttributes(&attr, paged::paged_attention_tile_kernel<T, D>) == cudaSuccess;
+        if (!got) cudaGetLastError();
+        return got && attr.numRegs == paged::kTileLaunchRegs;
+    }();
+    return ok;
+}
+
+template <typename T, int D>
+int launch_tile(const paged::AttnArgs &a, void *workspace, cudaStream_t stream) {
+    using C = paged::TileCfg<D>;
+    static Occupancy occupancy;
+    auto kernel = paged::paged_attention_tile_kernel<T, D>;
+    if (!tile_launchable<T, D>()) return PMKL_ERR_UNSUPPORTED;
+    // Tensor memory holds two CTAs an SM.
+    const int per_sm = std::min(2, occupancy.get(kernel, paged::kTileThreads, C::kSmemBytes));
+    if (per_sm < 1) return PMKL_ERR_LAUNCH;
+    const paged::StreamArgs p = shared_args<T>(a, workspace, paged::kMaxTileCtas, paged::kTileRows);
+    const long long tiles = std::max<long long>(1, (static_cast<long long>(a.max_blocks) * a.block + 127) / 128);
+    const long long row_tiles = (static_cast<long long>(a.H / a.Hkv) * a.max_q + 127) / 128;
+    const long long grid = share_grid(static_cast<long long>(sm_count()) * per_sm, paged::kMaxTileCtas,
+                                      static_cast<long long>(a.batch) * a.Hkv * row_tiles, tiles);
+    kernel<<<static_cast<unsigned>(grid), paged::kTileThreads, C::kSmemBytes, stream>>>(p);
+    const int rc = launch_status();
+    if (rc != PMKL_OK || tiles == 1) return rc;
+    return launch_join<T, D, paged::kTileRows>(p, grid, stream);
+}
+
+// The tcgen05 kernel from this many rows a K/V head on (16-bit queries).
+constexpr int kTileMinRows = 17;
+
 int paged_attention_impl(const paged::AttnArgs &p, int dtype, int kernel, void *workspace, cudaStream_t stream) {
-    const bool can_stream = stream_applies(p);
+    const bool can_stream = stream_applies(p), can_tile = can_stream && dtype != PMKL_DTYPE_F32;
     if (kernel == PMKL_PAGED_STREAM && !can_stream) return PMKL_ERR_UNSUPPORTED;
+    if (kernel == PMKL_PAGED_TCGEN05 && !can_tile) return PMKL_ERR_UNSUPPORTED;
     if (can_stream && kernel != PMKL_PAGED_SIMT && p.batch > 0 && p.max_q > 0) {
+        const bool many = static_cast<long long>(p.H / p.Hkv) * p.max_q >= kTileMinRows;
+        if (kernel == PMKL_PAGED_TCGEN05 || (kernel == PMKL_PAGED_AUTO && can_tile && many)) {
+            if (dtype == PMKL_DTYPE_F16)
+                return p.D == 64 ? launch_tile<__half, 64>(p, workspace, stream)
+                                 : launch_tile<__half, 128>(p, workspace, stream);
+            return p.D == 64 ? launch_tile<__nv_bfloat16, 64>(p, workspace, stream)
+                             : launch_tile<__nv_bfloat16, 128>(p, workspace, stream);
+        }
         const int rows = stream_rows(p.H, p.Hkv, p.max_q);
         return with_dtype(dtype, [&](auto *t) -> int {
             using T = std::remove_pointer_t<decltype(t)>;
@@ -275,7 +350,13 @@ size_t pmkl_paged_attention_workspace_size(int tokens, int batch, int heads, int
         heads % kv_heads != 0 || !dtype_valid(dtype))
         return 0;
     if (hidden != 64 && hidden != 128) return 0;  // the CUDA-core kernel needs none
-    return align256(paged::stream_workspace(stream_rows(heads, kv_heads, max_query_len), hidden));
+    // What the largest of the kernels that may be asked for needs.
+    const size_t stream =
+        paged::partial_workspace(paged::kMaxStreamCtas, stream_rows(heads, kv_heads, max_query_len), hidden);
+    const size_t tile = dtype == PMKL_DTYPE_F32
+                            ? 0
+                            : paged::partial_workspace(paged::kMaxTileCtas, paged::kTileRows, hidden);
+    return align256(stream > tile ? stream : tile);
 }
 
 int pmkl_paged_attention(const void *q, const int64_t *q_strides, const void *k_cache, const void *v_cache,
@@ -289,7 +370,8 @@ int pmkl_paged_attention(const void *q, const int64_t *q_strides, const void *k_
         max_blocks < 0 || max_query_len < 0 || table_stride < 0)
         return PMKL_ERR_INVALID_SHAPE;
     if (!dtype_valid(dtype)) return PMKL_ERR_INVALID_DTYPE;
-    if (kernel != PMKL_PAGED_AUTO && kernel != PMKL_PAGED_SIMT && kernel != PMKL_PAGED_STREAM) return PMKL_ERR_UNSUPPORTED;
+    if (kernel != PMKL_PAGED_AUTO && kernel != PMKL_PAGED_SIMT && kernel != PMKL_PAGED_STREAM &&
+        kernel != PMKL_PAGED_TCGEN05) return PMKL_ERR_UNSUPPORTED;
     if (heads > 0 && (kv_heads == 0 || heads % kv_heads != 0)) return PMKL_ERR_INVALID_SHAPE;
     if (batch > 1 && table_stride < max_blocks) return PMKL_ERR_INVALID_SHAPE;
     if (!query_starts && tokens != batch) return PMKL_ERR_INVALID_SHAPE;

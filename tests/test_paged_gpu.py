@@ -13,6 +13,7 @@ from pmkl_function import paged_append, paged_attention, paged_plan
 
 pytestmark = pytest.mark.gpu
 
+KERNELS = [0, 1, 2, 3]  # PMKL_PAGED_AUTO, _SIMT, _STREAM, _TCGEN05
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
 
 
@@ -191,7 +192,16 @@ def problem(lens, news, H, Hkv, D, block, dtype, seed, rows_first=False, poison=
     return q, kc, vc, ks, vs, table, lens, starts
 
 
+def needs(kernel, dtype, D=64, block=16):
+    """Skips what a kernel asked for by name does not cover."""
+    if kernel >= 2 and (D not in (64, 128) or block % 16):
+        pytest.skip("not this kernel's head or page size")
+    if kernel == 3 and dtype == F32:
+        pytest.skip("16-bit queries only")
+
+
 def check(prob, causal=True, scale=0.0, kernel=0, with_starts=True, q_dev=None):
+    needs(kernel, prob[0].dtype, prob[0].shape[2], prob[1].shape[2])
     q, kc, vc, ks, vs, table, lens, starts = prob
     want, lse, weight = ref.attention(q, kc, vc, ks, vs, table, lens, starts, causal, scale)
     news = [b - a for a, b in zip(starts, starts[1:])]
@@ -213,7 +223,7 @@ def check(prob, causal=True, scale=0.0, kernel=0, with_starts=True, q_dev=None):
 LENS = [1, 15, 16, 17, 31, 127, 128, 129, 300, 0, 513]
 
 
-@pytest.mark.parametrize("kernel", [0, 1])
+@pytest.mark.parametrize("kernel", KERNELS)
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("H,Hkv,D,block", [(4, 4, 64, 16), (8, 2, 128, 16), (6, 1, 128, 64), (8, 1, 64, 128), (3, 3, 128, 32),
                                            (4, 2, 96, 16), (2, 1, 64, 7), (2, 2, 256, 16), (5, 5, 33, 1), (10, 1, 128, 48)])
@@ -222,7 +232,7 @@ def test_attention_one_token(kernel, dtype, H, Hkv, D, block):
     check(problem(LENS, [1] * len(LENS), H, Hkv, D, block, dtype, seed=D + block), kernel=kernel, with_starts=block != 16)
 
 
-@pytest.mark.parametrize("kernel", [0, 1])
+@pytest.mark.parametrize("kernel", KERNELS)
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("H,Hkv,D,block", [(4, 4, 64, 16), (8, 2, 128, 32), (8, 1, 128, 16), (3, 1, 64, 128), (4, 2, 40, 5)])
 @pytest.mark.parametrize("causal", [True, False])
@@ -232,7 +242,7 @@ def test_attention_several_tokens(kernel, dtype, H, Hkv, D, block, causal):
     check(problem(lens, news, H, Hkv, D, block, dtype, seed=block + D, rows_first=True, tail=3), causal=causal, kernel=kernel)
 
 
-@pytest.mark.parametrize("kernel", [0, 1])
+@pytest.mark.parametrize("kernel", KERNELS)
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_attention_long(kernel, dtype):
     """Lengths that many CTAs share."""
@@ -240,7 +250,7 @@ def test_attention_long(kernel, dtype):
     check(problem([4097], [2], 8, 1, 64, 64, dtype, seed=2), kernel=kernel)
 
 
-@pytest.mark.parametrize("kernel", [0, 1])
+@pytest.mark.parametrize("kernel", KERNELS)
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 def test_attention_peaked_and_scaled(kernel, dtype):
     """Scores that grow along the keys and pages of very different scales."""
@@ -252,7 +262,7 @@ def test_attention_peaked_and_scaled(kernel, dtype):
     check(prob, scale=0.01, kernel=kernel)
 
 
-@pytest.mark.parametrize("kernel", [0, 1])
+@pytest.mark.parametrize("kernel", KERNELS)
 def test_attention_missing_pages(kernel):
     """Keys in pages outside the cache count as not there; a request of such pages only gives empty rows."""
     prob = problem([100, 48, 80], [1, 1, 4], 4, 2, 64, 16, F16, seed=4)
@@ -262,7 +272,7 @@ def test_attention_missing_pages(kernel):
     check(prob, kernel=kernel)
 
 
-@pytest.mark.parametrize("kernel", [0, 1])
+@pytest.mark.parametrize("kernel", KERNELS)
 def test_attention_strided_queries(kernel):
     prob = list(problem([33, 129], [1, 3], 4, 2, 64, 16, BF16, seed=5))
     wide = torch.zeros(4, 4, 3, 64, dtype=BF16, device="cuda")
@@ -275,9 +285,10 @@ def test_attention_strided_queries(kernel):
     check(prob, kernel=kernel, q_dev=odd)
 
 
-@pytest.mark.parametrize("kernel", [0, 1])
+@pytest.mark.parametrize("kernel", KERNELS)
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_attention_nan_and_inf_queries_stay_in_their_rows(kernel, dtype):
+    needs(kernel, dtype)
     q, kc, vc, ks, vs, table, lens, starts = problem([200, 90], [2, 1], 8, 2, 128, 16, dtype, seed=6)
     args = [t.cuda() for t in (kc, vc, ks, vs)] + [i32(table), i32(lens), i32(starts), 2, True, 0.0, kernel]
     clean, clean_lse = pmkl_pytorch_ext.paged_attention_fw(q.cuda(), *args)
@@ -290,7 +301,7 @@ def test_attention_nan_and_inf_queries_stay_in_their_rows(kernel, dtype):
     assert torch.equal(out[keep.cuda()], clean[keep.cuda()]) and torch.equal(lse[keep.cuda()], clean_lse[keep.cuda()])
 
 
-@pytest.mark.parametrize("kernel", [0, 1])
+@pytest.mark.parametrize("kernel", KERNELS)
 def test_attention_same_bits_again_and_on_another_stream(kernel):
     q, kc, vc, ks, vs, table, lens, starts = problem([900, 31, 4000], [1, 4, 1], 8, 2, 128, 16, BF16, seed=7)
     args = [t.cuda() for t in (q, kc, vc, ks, vs)] + [i32(table), i32(lens), i32(starts), 4, True, 0.0, kernel]
@@ -343,6 +354,43 @@ def test_step_in_a_graph():
             assert torch.equal(c1.double(), want) and torch.equal(s1.double(), scale)
         want, wlse, weight = ref.attention(q.cpu(), *after, table.tolist(), lens, starts.tolist())
         assert ((out.cpu().double() - want).abs() <= ref.out_bound(want, weight, wlse, BF16, max(lens))).all()
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("H,Hkv,D,block", [(16, 2, 128, 16), (4, 1, 64, 32)])
+def test_attention_chunks(kernel, dtype, H, Hkv, D, block):
+    """Chunks of many rows a K/V head, whole prompts among them."""
+    check(problem([300, 131, 517], [97, 131, 1], H, Hkv, D, block, dtype, seed=11), kernel=kernel)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_nan_in_later_tokens(kernel, dtype, D):
+    """A key that only later tokens of the step see holds NaN: they get NaN where it stands, the earlier ones nothing of it."""
+    needs(kernel, dtype)
+    q, kc, vc, ks, vs, table, lens, starts = problem([150, 40], [6, 5], 6, 2, D, 16, dtype, seed=12)
+    args = lambda k, v: [q.cuda(), k.cuda(), v.cuda(), ks.cuda(), vs.cuda(), i32(table), i32(lens), i32(starts), 6, True, 0.0, kernel]  # noqa: E731
+    clean, _ = pmkl_pytorch_ext.paged_attention_fw(*args(kc, vc))
+    # request 0: row 148 (seen by its last two tokens); request 1: row 38, all of head 1
+    bad = vc.clone()
+    bad.view(torch.uint8)[table[0][148 // 16], 0, 148 % 16, 5] = 0x7F
+    bad.view(torch.uint8)[table[0][148 // 16], 0, 148 % 16, D - 1] = 0xFF
+    bad.view(torch.uint8)[table[1][38 // 16], 1, 38 % 16] = 0x7F
+    out, lse = pmkl_pytorch_ext.paged_attention_fw(*args(kc, bad))
+    want = torch.zeros(out.shape, dtype=torch.bool)
+    want[4:6, 0:3, 5] = want[4:6, 0:3, D - 1] = True
+    want[9:11, 3:6] = True
+    assert torch.equal(out.isnan().cpu(), want)
+    assert torch.equal(out[~want.cuda()], clean[~want.cuda()])
+    # the same in the keys: whole rows
+    bad = kc.clone()
+    bad.view(torch.uint8)[table[0][148 // 16], 0, 148 % 16, 5] = 0x7F
+    out, lse = pmkl_pytorch_ext.paged_attention_fw(*args(bad, vc))
+    want = torch.zeros(out.shape, dtype=torch.bool)
+    want[4:6, 0:3] = True
+    assert torch.equal(out.isnan().cpu(), want) and torch.equal(lse.isnan().cpu(), want[:, :, 0])
 
 
 # ---------------------------------------------------------------- refusals

@@ -75,6 +75,30 @@ __device__ __forceinline__ float value_scale(float s) {
     return fminf(fmaxf(s, 5.421010862427522e-20f), 1.8446744073709552e19f);  // 2^-64, 2^64
 }
 
+// The rare path of the kernels whose products would spread a NaN value as 0 *
+// NaN: sets in `cols` (a bit a column) the columns that hold NaN in the rows
+// [key, end) of request row `table`, K/V head h.
+__device__ __noinline__ void mark_nan(const AttnArgs &p, const int *table, int h, int key, int end, uint32_t *cols) {
+#pragma unroll 1
+    for (; key < end; ++key) {
+        const int col = key / p.block, page = table[col];
+        if (page < 0 || page >= p.num_blocks) continue;
+        const uint8_t *v = p.v.base + page * p.v.s[0] + h * p.v.s[1] + (key - col * p.block) * p.v.s[2];
+#pragma unroll 1
+        for (int d = 0; d < p.D; ++d)
+            if ((v[d] & 0x7F) == 0x7F) atomicOr(&cols[d >> 5], 1u << (d & 31));
+    }
+}
+
+// Bit 7 of each byte that is an e4m3 NaN (0x7F with either sign).
+__device__ __forceinline__ uint32_t nan_bits(uint32_t four) {
+    return ((four & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+}
+__device__ __forceinline__ uint32_t without_nan(uint32_t four) {
+    const uint32_t n = nan_bits(four);
+    return four & ~(n | (n - (n >> 7)));
+}
+
 constexpr int kSimtThreads = 128;
 constexpr int kSimtCols = 8;  // output columns a lane, head size up to 256
 

@@ -36,7 +36,7 @@
 // others do not (a later token of the same step) may hold NaN too, which the
 // product would spread as 0 * NaN: tiles at the diagonal look for NaN bytes,
 // and where there are any the product gets zeros for them and the rows that do
-// see the key get their NaN by selection.
+// see the key note its columns.
 #pragma once
 
 #include "paged_attention_simt.cuh"
@@ -116,6 +116,17 @@ __device__ __forceinline__ void load_bytes(Bytes<8> &r, const uint8_t *p) {
     asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(r.w[0]), "=r"(r.w[1]) : "l"(p));
 }
 
+// 16 bytes, or zeros where `there` is false: predicated, not branched around.
+__device__ __forceinline__ uint4 load16_if(const uint8_t *p, bool there) {
+    uint4 r = make_uint4(0, 0, 0, 0);
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\t"
+        "@p ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+        : "+r"(r.x), "+r"(r.y), "+r"(r.z), "+r"(r.w)
+        : "l"(p), "r"(there ? 1u : 0u));
+    return r;
+}
+
 template <int D, int NT>
 struct StreamCfg {
     static constexpr int kRows = 8 * NT;
@@ -134,6 +145,12 @@ __device__ __forceinline__ int request_tiles(const Request &r) { return max(1, (
 template <int ROWS>
 __device__ __forceinline__ int row_tiles(const AttnArgs &p, const Request &r) {
     return (r.rows * (p.H / p.Hkv) + ROWS - 1) / ROWS;
+}
+
+template <int ROWS>
+__device__ __noinline__ long long stream_weight(const AttnArgs &p, int b) {
+    const Request r = request_of(p, b);
+    return static_cast<long long>(row_tiles<ROWS>(p, r)) * p.Hkv * request_tiles(r);
 }
 
 // 16 consecutive elements of a query row as fp32.
@@ -155,7 +172,7 @@ __device__ __forceinline__ void load_q16(float (&x)[16], const T *q, bool vec) {
 }
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kStreamThreads, NT == 1 ? 2 : 1) paged_attention_stream_kernel(const StreamArgs sa) {
+__global__ void __launch_bounds__(kStreamThreads, NT == 1 ? 2 : 1) paged_attention_stream_kernel(const __grid_constant__ StreamArgs sa) {
     using C = StreamCfg<D, NT>;
     constexpr bool kSplit = sizeof(T) == 4;  // fp32 queries: two fp16 parts of q and of p
     constexpr int kParts = kSplit ? 2 : 1;
@@ -165,6 +182,8 @@ __global__ void __launch_bounds__(kStreamThreads, NT == 1 ? 2 : 1) paged_attenti
     constexpr int kVBytes = D / 8;   // bytes of a V row a thread
     extern __shared__ float s_acc[];
     __shared__ float s_m[kStreamWarps][C::kRows], s_l[kStreamWarps][C::kRows];
+    __shared__ uint32_t s_nan[C::kRows][D / 32];  // columns of a row that are NaN, where s_any_nan
+    __shared__ int s_any_nan;
     __shared__ long long s_sum[kStreamWarps];
     __shared__ long long s_at;
     __shared__ int s_b;
@@ -176,9 +195,7 @@ __global__ void __launch_bounds__(kStreamThreads, NT == 1 ? 2 : 1) paged_attenti
 
     // ---- this CTA's share of the list
     const auto weight = [&](int b) -> long long {
-        if (b >= p.batch) return 0;
-        const Request r = request_of(p, b);
-        return static_cast<long long>(row_tiles<C::kRows>(p, r)) * p.Hkv * request_tiles(r);
+        return b < p.batch ? stream_weight<C::kRows>(p, b) : 0;
     };
     const auto block_inclusive = [&](long long v) -> long long {
 #pragma unroll
@@ -219,7 +236,8 @@ __global__ void __launch_bounds__(kStreamThreads, NT == 1 ? 2 : 1) paged_attenti
             if (before > u_begin) break;
         }
     }
-    if (tid == 0) sa.desc[blockIdx.x].segments = 0;
+    if (tid == 0) sa.desc[blockIdx.x].segments = 0, s_any_nan = 0;
+    for (int i = tid; i < C::kRows * (D / 32); i += kStreamThreads) s_nan[i / (D / 32)][i % (D / 32)] = 0;
     __syncthreads();
 
     long long u = u_begin;
@@ -434,39 +452,19 @@ __global__ void __launch_bounds__(kStreamThreads, NT == 1 ? 2 : 1) paged_attenti
 #pragma unroll
                             for (int x = 0; x < kVBytes / 4; ++x) vr[i].w[x] = 0;
                     // NaN in rows that some queries do not see.
-                    bool nan = false;
+                    uint32_t nan = 0;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
 #pragma unroll
-                        for (int x = 0; x < kVBytes / 4; ++x)
-                            nan = nan || __vcmpeq4(vr[i].w[x] & 0x7F7F7F7Fu, 0x7F7F7F7Fu) != 0;
-                    if (__any_sync(0xffffffffu, nan)) {
-                        for (int who = 0; who < 4; ++who)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const int k_at = key + 2 * who + (i & 1) + (i >> 1) * 8;
-#pragma unroll
-                                for (int x = 0; x < kVBytes / 4; ++x) {
-                                    const uint32_t bytes = __shfl_sync(0xffffffffu, vr[i].w[x], (lane & 28) + who);
-                                    const uint32_t bad = __vcmpeq4(bytes & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
-#pragma unroll
-                                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                                        for (int c = 0; c < 2; ++c)
-                                            if (k_at < lim[n][c]) {
-                                                // dim 4x + j: tile 2x + j / 2, row half j % 2
-                                                if (bad & 0x000000FFu) acc[2 * x][n][c] = NAN;
-                                                if (bad & 0x0000FF00u) acc[2 * x][n][c + 2] = NAN;
-                                                if (bad & 0x00FF0000u) acc[2 * x + 1][n][c] = NAN;
-                                                if (bad & 0xFF000000u) acc[2 * x + 1][n][c + 2] = NAN;
-                                            }
-                                }
-                            }
+                        for (int x = 0; x < kVBytes / 4; ++x) nan |= nan_bits(vr[i].w[x]);
+                    if (__any_sync(0xffffffffu, nan != 0)) {
+                        if (lane < C::kRows && lane < n_rows)
+                            mark_nan(p, table, h, key, min(key + 16, visible(p, r, (row0 + lane) / group)), s_nan[lane]);
+                        if (lane == 0) s_any_nan = 1;
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
 #pragma unroll
-                            for (int x = 0; x < kVBytes / 4; ++x)
-                                vr[i].w[x] &= ~__vcmpeq4(vr[i].w[x] & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+                            for (int x = 0; x < kVBytes / 4; ++x) vr[i].w[x] = without_nan(vr[i].w[x]);
                     }
                 }
                 // O^T += V^T P^T
@@ -562,6 +560,7 @@ __global__ void __launch_bounds__(kStreamThreads, NT == 1 ? 2 : 1) paged_attenti
 #pragma unroll
             for (int w = 0; w < kStreamWarps / 2; ++w) x += from[w * C::kRows * C::kRowPitch];
             x *= sum == 0.f ? 0.f : 1.f / sum;
+            if (s_any_nan && (s_nan[rw][d >> 5] >> (d & 31) & 1u)) x = NAN;
             const float lse2 = sum == 0.f ? -INFINITY : top + log2f(sum);
             if (whole) {
                 const int tok = (row0 + rw) / group, head = h * group + (row0 + rw) - tok * group;
@@ -582,6 +581,12 @@ __global__ void __launch_bounds__(kStreamThreads, NT == 1 ? 2 : 1) paged_attenti
             sa.desc[blockIdx.x] = StreamDesc{b, item, static_cast<int>(c1) - static_cast<int>(blockIdx.x) + 1, 0};
         }
         __syncthreads();  // the sums have been read
+        if (s_any_nan) {
+            __syncthreads();
+            for (int i = tid; i < C::kRows * (D / 32); i += kStreamThreads) s_nan[i / (D / 32)][i % (D / 32)] = 0;
+            if (tid == 0) s_any_nan = 0;
+            __syncthreads();
+        }
     }
 }
 

@@ -9,10 +9,11 @@
 //
 // A CTA has three warpgroups, which divide its registers between them
 // (setmaxnreg); two CTAs an SM fill each other's gaps:
-//   * warps 4-7 bring the cache in: pages looked up, 8-bit values loaded 16
-//     bytes a thread, a tile ahead in registers, made fp16 (every e4m3 value is
-//     one) and stored as the 128-byte-swizzled tiles that the products read.
-//     No scale is multiplied in: they go with the scores;
+//   * warps 4, 5 bring keys in, warps 6, 7 values: pages looked up, 8-bit
+//     values loaded 16 bytes a thread, half a tile ahead in registers, made fp16
+//     (every e4m3 value is one) and stored as the 128-byte-swizzled tiles that
+//     the products read.  No scale is multiplied in: they go with the scores;
+//   * warp 9 walks the CTA's share and hands out its segments;
 //   * warp 8 issues tcgen05.mma: S = Q K^T, then O += P V with P from tensor
 //     memory.  Products of one thread run in order, so S of the next tile may
 //     be issued over P, and its completion tells that P V is done;
@@ -39,7 +40,7 @@ constexpr int kTileRows = 128;
 constexpr int kTileThreads = 384;
 // Registers a thread: at launch, and what each warpgroup sets; the three come
 // to the launch's total (the host checks that the build has it).
-constexpr int kTileLaunchRegs = 80, kTileSoftmaxRegs = 120, kTileLoadRegs = 96, kTileIssueRegs = 24;
+constexpr int kTileLaunchRegs = 80, kTileSoftmaxRegs = 128, kTileLoadRegs = 80, kTileIssueRegs = 32;
 static_assert(kTileSoftmaxRegs + kTileLoadRegs + kTileIssueRegs == 3 * kTileLaunchRegs, "register split");
 constexpr int kMaxTileCtas = 320;  // partials in the workspace: 148 SMs with 2 CTAs
 
@@ -51,18 +52,6 @@ struct TileCfg {
     static constexpr uint32_t kTmemCols = 256, kColS = 0, kColP = 64, kColO = 128;
 };
 
-struct TileShared {
-    uint64_t q_full, k_full, k_empty, v_full, v_empty, s_full, p_full, o_full, drained;
-    uint32_t tmem;
-    int abort_flag;
-    float2 scale[2][8];  // of 16 keys: key scale, log2 of the value scale (-inf: no page)
-    float inv_vs[2][8];
-    int nan[2];          // the tile's values held NaN, tile number of the CTA + 1
-    long long sum[kTileThreads / 32];
-    long long at;
-    int b;
-};
-
 // One stretch of an item's key tiles.
 struct Segment {
     Request r;
@@ -70,9 +59,25 @@ struct Segment {
     int lim_min, lim_max;  // keys that the first and last row see
 };
 
-// The share of a CTA in the list of items; every warp walks it by itself.
+// The share of a CTA in the list of items.
 struct Share {
     long long total, shares, u, u_end, b_begin;
+    int b;
+};
+
+struct TileShared {
+    uint64_t q_full, k_full, k_empty, v_full, v_empty, s_full, p_full, o_full, drained;
+    uint64_t seg_full[2], seg_empty[2];
+    uint32_t tmem;
+    int abort_flag;
+    Segment seg[2];
+    int last_cta[2];     // of a segment that a later CTA ends: which
+    float2 scale[2][8];  // of 16 keys: key scale, log2 of the value scale (-inf: no page)
+    float inv_vs[2][8];
+    int nan[2];          // the tile's values held NaN: tile number of the CTA + 1
+    alignas(16) uint32_t nan_cols[kTileRows][4];  // columns of a row that are NaN (see above)
+    long long sum[kTileThreads / 32];
+    long long at;
     int b;
 };
 
@@ -122,6 +127,10 @@ __device__ __forceinline__ bool next_segment(const AttnArgs &p, Share &w, Segmen
     return false;
 }
 
+__device__ __noinline__ long long tile_weight(const AttnArgs &p, int b) {
+    return head_tiles(p, request_of(p, b), p.H / p.Hkv) * p.Hkv;
+}
+
 // tcgen05.wait::ld that the values pass through, so that no use of them is
 // moved before it.
 __device__ __forceinline__ void tmem_arrived(uint32_t (&r)[32]) {
@@ -139,6 +148,17 @@ __device__ __forceinline__ void tmem_arrived(uint32_t (&r)[32]) {
                  : "memory");
 }
 
+// 16 columns, waited for.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+
 // Largest of 16 scores.
 __device__ __forceinline__ float max16(const uint32_t *r) {
     float m = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
@@ -148,7 +168,7 @@ __device__ __forceinline__ float max16(const uint32_t *r) {
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(const StreamArgs sa) {
+__global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(const __grid_constant__ StreamArgs sa) {
     using namespace ptx;
     using C = TileCfg<D>;
     extern __shared__ uint8_t smem_raw[];
@@ -165,14 +185,18 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
     // ---- set-up: barriers, tensor memory, this CTA's share
     if (tid == 0) {
         mbar_init(&sh.q_full, 128);
-        mbar_init(&sh.k_full, 128);
+        mbar_init(&sh.k_full, 64);
         mbar_init(&sh.k_empty, 1);
-        mbar_init(&sh.v_full, 128);
+        mbar_init(&sh.v_full, 64);
         mbar_init(&sh.v_empty, 1);
         mbar_init(&sh.s_full, 1);
         mbar_init(&sh.p_full, 128);
         mbar_init(&sh.o_full, 1);
         mbar_init(&sh.drained, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh.seg_full[i], 1);
+            mbar_init(&sh.seg_empty[i], 9);  // four softmax and four loading warps, the issuing thread
+        }
         sh.nan[0] = sh.nan[1] = 0;
         // Once any CTA has given up a wait, later CTAs skip their work.
         sh.abort_flag = (*reinterpret_cast<volatile unsigned int *>(&g_device_error) != 0u) ? 1 : 0;
@@ -184,7 +208,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
         tmem_relinquish();
     }
     const auto weight = [&](int b) -> long long {
-        return b < p.batch ? head_tiles(p, request_of(p, b), group) * p.Hkv : 0;
+        return b < p.batch ? tile_weight(p, b) : 0;
     };
     const auto block_inclusive = [&](long long v) -> long long {
 #pragma unroll
@@ -228,26 +252,54 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
     const bool skip = *abort_flag != 0;
     if (mine.u < mine.u_end) mine.b = sh.b, mine.b_begin = sh.at;
 
-    Segment s;
     if (warp >= 8) {
         // ------------------------------------------------------------ products
         reg_dealloc<kTileIssueRegs>();
+        if (warp == 9 && lane == 0 && !skip) {
+            // The segments, two ahead at most; one without tiles is the end.
+            bool more = true;
+            for (uint32_t seg = 0; more; ++seg) {
+                const int i = seg & 1;
+                if (seg >= 2 && !mbar_wait(&sh.seg_empty[i], ((seg >> 1) - 1) & 1, abort_flag)) break;
+                Segment &s = sh.seg[i];
+                more = next_segment(p, mine, s);
+                if (!more) {
+                    s.tile0 = s.tile1 = 0;
+                } else if (s.tile1 < s.tiles) {
+                    // The CTA whose share holds the item's last tile.
+                    const long long last = mine.u + (s.tiles - s.tile1) - 1;
+                    long long c1 = last * mine.shares / mine.total;  // within one of the owner
+                    while (mine.total * (c1 + 1) / mine.shares <= last) ++c1;
+                    while (mine.total * c1 / mine.shares > last) --c1;
+                    sh.last_cta[i] = static_cast<int>(c1);
+                }
+                mbar_arrive(&sh.seg_full[i]);
+            }
+        }
         if (warp == 8 && lane == 0 && !skip) {
             constexpr uint32_t kIdescS = idesc_f16(128, 128, 0, 0, 0);
             constexpr uint32_t kIdescO = idesc_f16(128, D, 0, 0, 1);
-            const uint32_t q_addr = smem_u32(sQ), k_addr = smem_u32(sK), v_addr = smem_u32(sV);
-            uint32_t it = 0, seg = 0;
+            const uint64_t q_desc = smem_desc_sw128(smem_u32(sQ), 16, 1024), k_desc = smem_desc_sw128(smem_u32(sK), 16, 1024);
+            const uint64_t v_desc = smem_desc_sw128(smem_u32(sV), 128 * 128, 1024);
+            // The halves: addresses advance in the low one, in units of 16 bytes.
+            const uint32_t q_lo = static_cast<uint32_t>(q_desc), k_lo = static_cast<uint32_t>(k_desc);
+            const uint32_t v_lo = static_cast<uint32_t>(v_desc);
+            const uint32_t qk_hi = static_cast<uint32_t>(q_desc >> 32), v_hi = static_cast<uint32_t>(v_desc >> 32);
+            uint32_t it = 0;
             bool ok = true;
-            while (ok && next_segment(p, mine, s)) {
+            for (uint32_t seg = 0; ok; ++seg) {
+                if (!(ok = mbar_wait(&sh.seg_full[seg & 1], (seg >> 1) & 1, abort_flag))) break;
+                int tiles = sh.seg[seg & 1].tile1 - sh.seg[seg & 1].tile0;
+                mbar_arrive(&sh.seg_empty[seg & 1]);
+                if (tiles == 0) break;
                 ok = mbar_wait(&sh.q_full, seg & 1, abort_flag);
-                for (int j = s.tile0; ok && j < s.tile1; ++j, ++it) {
+                for (uint32_t more = 0; ok && tiles > 0; --tiles, ++it, more = 1) {
                     if (!(ok = mbar_wait(&sh.k_full, it & 1, abort_flag))) break;
                     tc_fence_after();
 #pragma unroll
                     for (int kk = 0; kk < D / 16; ++kk) {
-                        const uint32_t off = (kk >> 2) * (128 * 128) + (kk & 3) * 32;
-                        mma_ss(tmem + C::kColS, smem_desc_sw128(q_addr + off, 16, 1024),
-                               smem_desc_sw128(k_addr + off, 16, 1024), kIdescS, kk > 0 ? 1u : 0u);
+                        const uint32_t off = ((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4;
+                        mma_ss_h(tmem + C::kColS, q_lo + off, qk_hi, k_lo + off, qk_hi, kIdescS, kk > 0 ? 1u : 0u);
                     }
                     mma_commit(&sh.s_full);
                     mma_commit(&sh.k_empty);
@@ -256,13 +308,11 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                     tc_fence_after();
 #pragma unroll
                     for (int kk = 0; kk < 8; ++kk)
-                        mma_ts(tmem + C::kColO, tmem + C::kColP + kk * 8,
-                               smem_desc_sw128(v_addr + kk * 16 * 128, 128 * 128, 1024), kIdescO,
-                               (j > s.tile0 || kk > 0) ? 1u : 0u);
+                        mma_ts_h(tmem + C::kColO, tmem + C::kColP + kk * 8, v_lo + kk * (16 * 128 / 16), v_hi, kIdescO,
+                                 kk > 0 ? 1u : more);
                     mma_commit(&sh.v_empty);
                 }
                 if (ok) mma_commit(&sh.o_full);
-                ++seg;
             }
             // Every product has ended before tensor memory is given back.
             mma_commit(&sh.drained);
@@ -272,111 +322,122 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
     } else if (warp >= 4) {
         // ------------------------------------------------------------ cache to shared memory
         reg_alloc<kTileLoadRegs>();
-        constexpr int kPerRow = D / 16;              // threads a key row
-        constexpr int kRowsPass = 128 / kPerRow;     // key rows a pass
-        constexpr int kPasses = 128 / kRowsPass;
-        const int t = tid - 128, sub = t / kPerRow, chunk = t % kPerRow;
+        constexpr int kPerRow = D / 16;          // threads a row, 16 bytes each
+        constexpr int kRowsPass = 64 / kPerRow;  // rows a pass: 8 or 16
+        constexpr int kHalf = 64 / kRowsPass;    // passes of half a tile
+        const bool values = warp >= 6;
+        const CacheView &cache = values ? p.v : p.k;
+        uint64_t *const full = values ? &sh.v_full : &sh.k_full, *const empty = values ? &sh.v_empty : &sh.k_empty;
+        const int t = tid & 63, chunk = t % kPerRow;
+        // Threads of the second 64 columns take the row next to it: the eight
+        // that store at one time then meet all banks once.
+        const int sub = (t / kPerRow) ^ (chunk >> 2);
+        uint8_t *const to = (values ? sV : sK) + (chunk >> 2) * (128 * 128) + sub * 128;
+        const int at0 = (((chunk & 3) * 2) ^ (sub & 7)) << 4, at1 = (((chunk & 3) * 2 + 1) ^ (sub & 7)) << 4;
+        const long long row_bytes = cache.s[2], mine_off = sub * row_bytes + chunk * 16, mine_odd = mine_off + 8 * row_bytes;
         uint32_t it = 0;
         bool ok = !skip;
-        while (ok && next_segment(p, mine, s)) {
+        for (uint32_t seg = 0; ok; ++seg) {
+            if (!(ok = mbar_wait_warp_all(&sh.seg_full[seg & 1], (seg >> 1) & 1, abort_flag))) break;
+            const Segment &s = sh.seg[seg & 1];
             const int *table = p.table + s.b * p.table_stride;
-            // Page (-1: none) and row of the tile's 16-key groups, lane i of 8 the i-th.
-            const auto find = [&](int j, int &page, int &row) {
-                const int key = j * 128 + (lane & 7) * 16;
-                page = -1, row = 0;
-                if (key < s.lim_max) {
-                    const int c = key / p.block;
-                    row = key - c * p.block;
-                    const int x = __ldg(table + c);
-                    page = x >= 0 && x < p.num_blocks ? x : -1;
-                }
+            const int tile0 = s.tile0, tile1 = s.tile1, lim_min = s.lim_min, lim_max = s.lim_max, h = s.h;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.seg_empty[seg & 1]);
+            if (tile0 == tile1) break;
+            // Half f of the keys is half a tile, 64 rows.  Three steps ahead of its
+            // use lane i of 4 looks its i-th 16 rows up in the table, two ahead its
+            // data and scales are loaded into registers.
+            const auto look_up = [&](int f) {
+                const int key0 = f * 64 + (lane & 3) * 16;
+                return key0 < lim_max ? __ldg(table + key0 / p.block) : -1;
             };
-            const auto load = [&](const CacheView &c, int page, int row, int key_end, uint4 (&v)[kPasses]) {
-#pragma unroll
-                for (int i = 0; i < kPasses; ++i) {
-                    const int key = i * kRowsPass + sub;
-                    const int pg = __shfl_sync(0xffffffffu, page, key >> 4), rw = __shfl_sync(0xffffffffu, row, key >> 4);
-                    v[i] = make_uint4(0, 0, 0, 0);
-                    if (pg >= 0 && key < key_end) {
-                        Bytes<16> x;
-                        load_bytes(x, c.base + pg * c.s[0] + s.h * c.s[1] + (rw + (key & 15)) * c.s[2] + chunk * 16);
-                        v[i] = make_uint4(x.w[0], x.w[1], x.w[2], x.w[3]);
+            uint4 v[kHalf];
+            float ks, vs;
+            bool there;
+            // (rows that no query sees, or in no page of the cache, are zero)
+            const auto load = [&](int f, int x) {
+                const int key0 = f * 64 + (lane & 3) * 16;
+                unsigned long long from = 0;
+                there = x >= 0 && x < p.num_blocks;
+                ks = vs = 1.f;
+                if (there) {
+                    from = reinterpret_cast<unsigned long long>(cache.base) + x * cache.s[0] + h * cache.s[1] +
+                           key0 % p.block * row_bytes;
+                    if (warp == 4) {
+                        const long long at = static_cast<long long>(x) * p.Hkv + h;
+                        ks = __ldg(p.k.scale + at);
+                        vs = __ldg(p.v.scale + at);
                     }
                 }
-            };
-            const auto store = [&](uint8_t *tile, const uint4 (&v)[kPasses]) {
+                const int left = lim_max - f * 64 - sub;
 #pragma unroll
-                for (int i = 0; i < kPasses; ++i) {
-                    const int key = i * kRowsPass + sub;
-                    uint8_t *box = tile + (chunk >> 2) * (128 * 128) + key * 128;
-                    const int c = (chunk & 3) * 2, x = key & 7;
-                    const uint4 a = make_uint4(e4m3x2_to_h2(v[i].x), e4m3x2_to_h2_hi(v[i].x), e4m3x2_to_h2(v[i].y),
-                                               e4m3x2_to_h2_hi(v[i].y));
-                    const uint4 b = make_uint4(e4m3x2_to_h2(v[i].z), e4m3x2_to_h2_hi(v[i].z), e4m3x2_to_h2(v[i].w),
-                                               e4m3x2_to_h2_hi(v[i].w));
-                    // The second box's threads store their halves in the other order: no bank meets twice.
-                    const bool swap = (chunk >> 2) != 0;
-                    *reinterpret_cast<uint4 *>(box + (((c + (swap ? 1 : 0)) ^ x) << 4)) = swap ? b : a;
-                    *reinterpret_cast<uint4 *>(box + (((c + (swap ? 0 : 1)) ^ x) << 4)) = swap ? a : b;
+                for (int i = 0; i < kHalf; ++i) {
+                    const unsigned long long at = __shfl_sync(0xffffffffu, from, i * kRowsPass / 16);
+                    v[i] = load16_if(reinterpret_cast<const uint8_t *>(at) + (i * kRowsPass % 16 ? mine_odd : mine_off),
+                                     at != 0 && i * kRowsPass < left);
                 }
             };
-            int page, row, page_n = -1, row_n = 0;
-            find(s.tile0, page, row);
-            uint4 kv[kPasses], vv[kPasses];
-            load(p.k, page, row, 128, kv);
-            for (int j = s.tile0; j < s.tile1; ++j, ++it) {
-                const int left = s.lim_max - j * 128;  // keys of this tile that some row sees
-                load(p.v, page, row, left, vv);
-                float ks = 1.f, vs = 1.f;  // no page: any factor but 0, for masked scores are -inf
-                const bool scales = warp == 4 && lane < 8;
-                if (scales && page >= 0) {
-                    ks = __ldg(p.k.scale + static_cast<long long>(page) * p.Hkv + s.h);
-                    vs = value_scale(__ldg(p.v.scale + static_cast<long long>(page) * p.Hkv + s.h));
+            load(2 * tile0, look_up(2 * tile0));
+            int x_next = look_up(2 * tile0 + 1);
+            for (int f = 2 * tile0; f < 2 * tile1; ++f) {
+                const bool second = f & 1;
+                if (!second && it > 0 && !(ok = mbar_wait_warp_all(empty, (it - 1) & 1, abort_flag))) break;
+                if (warp == 4 && lane < 4) {
+                    // (the softmax is done with the tile before the last; no page: any key
+                    // scale but 0, for masked scores are -inf)
+                    const float y = value_scale(vs);
+                    sh.scale[it & 1][(f & 1) * 4 + lane] = make_float2(ks, there ? log2f(y) : -INFINITY);
+                    sh.inv_vs[it & 1][(f & 1) * 4 + lane] = 1.f / y;
                 }
-                if (j + 1 < s.tile1) find(j + 1, page_n, row_n);
-                if (it > 0 && !(ok = mbar_wait_warp_all(&sh.k_empty, (it - 1) & 1, abort_flag))) break;
-                store(sK, kv);
-                if (scales) {
-                    sh.scale[it & 1][lane] = make_float2(ks, page >= 0 ? log2f(vs) : -INFINITY);
-                    sh.inv_vs[it & 1][lane] = 1.f / vs;
+                uint8_t *const here = to + (second ? 64 * 128 : 0);
+#pragma unroll
+                for (int i = 0; i < kHalf; ++i) {
+                    *reinterpret_cast<uint4 *>(here + i * (kRowsPass * 128) + at0) =
+                        make_uint4(e4m3x2_to_h2(v[i].x), e4m3x2_to_h2_hi(v[i].x), e4m3x2_to_h2(v[i].y),
+                                   e4m3x2_to_h2_hi(v[i].y));
+                    *reinterpret_cast<uint4 *>(here + i * (kRowsPass * 128) + at1) =
+                        make_uint4(e4m3x2_to_h2(v[i].z), e4m3x2_to_h2_hi(v[i].z), e4m3x2_to_h2(v[i].w),
+                                   e4m3x2_to_h2_hi(v[i].w));
                 }
-                fence_proxy_async_smem();
-                mbar_arrive(&sh.k_full);
-                if (j + 1 < s.tile1) load(p.k, page_n, row_n, 128, kv);
-                if (j * 128 + 128 > s.lim_min) {
-                    bool nan = false;
+                if (values && f * 64 + 64 > lim_min) {
+                    // NaN among the values: noted, and zero in the tile.
+                    uint32_t nan = 0;
 #pragma unroll
-                    for (int i = 0; i < kPasses; ++i) {
-                        const uint32_t w[4] = {vv[i].x, vv[i].y, vv[i].z, vv[i].w};
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) nan = nan || __vcmpeq4(w[x] & 0x7F7F7F7Fu, 0x7F7F7F7Fu) != 0;
-                    }
+                    for (int i = 0; i < kHalf; ++i)
+                        nan |= nan_bits(v[i].x) | nan_bits(v[i].y) | nan_bits(v[i].z) | nan_bits(v[i].w);
                     if (nan) {
                         sh.nan[it & 1] = static_cast<int>(it) + 1;
-#pragma unroll
-                        for (int i = 0; i < kPasses; ++i) {
-                            vv[i].x &= ~__vcmpeq4(vv[i].x & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
-                            vv[i].y &= ~__vcmpeq4(vv[i].y & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
-                            vv[i].z &= ~__vcmpeq4(vv[i].z & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
-                            vv[i].w &= ~__vcmpeq4(vv[i].w & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+#pragma unroll 1
+                        for (int i = 0; i < kHalf * 16; ++i) {
+                            uint16_t *x = reinterpret_cast<uint16_t *>(here + (i >> 4) * (kRowsPass * 128) +
+                                                                       ((i & 8) ? at1 : at0)) + (i & 7);
+                            if ((*x & 0x7FFF) > 0x7C00) *x = 0;
                         }
                     }
                 }
-                if (it > 0 && !(ok = mbar_wait_warp_all(&sh.v_empty, (it - 1) & 1, abort_flag))) break;
-                store(sV, vv);
-                fence_proxy_async_smem();
-                mbar_arrive(&sh.v_full);
-                page = page_n;
-                row = row_n;
+                if (second) {
+                    fence_proxy_async_smem();
+                    mbar_arrive(full);
+                    ++it;
+                }
+                if (f + 1 < 2 * tile1) {
+                    load(f + 1, x_next);
+                    x_next = look_up(f + 2);
+                }
             }
         }
     } else {
         // ------------------------------------------------------------ softmax, a thread a row
         reg_alloc<kTileSoftmaxRegs>();
         const uint32_t lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
-        uint32_t it = 0, seg = 0;
+        uint32_t it = 0;
         bool ok = !skip;
-        while (ok && next_segment(p, mine, s)) {
+        for (uint32_t seg = 0; ok; ++seg) {
+            if (!(ok = mbar_wait_warp_all(&sh.seg_full[seg & 1], (seg >> 1) & 1, abort_flag))) break;
+            const Segment &s = sh.seg[seg & 1];
+            const int tile0 = s.tile0, tile1 = s.tile1, lim_min = s.lim_min;
+            if (tile0 == tile1) break;
             const int rr = s.row0 + tid;
             const bool real = tid < s.n_rows;
             const int tok = real ? rr / group : 0, head = s.h * group + (real ? rr - tok * group : 0);
@@ -384,7 +445,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
             // The row's largest value, then the row over the power of two that brings it to 2^7 .. 2^8.
             float amax = 0.f;
             if (real)
-#pragma unroll 2
+#pragma unroll 1
                 for (int c = 0; c < D; c += 16) {
                     float x[16];
                     load_q16(x, q + c, sa.vec_q != 0);
@@ -393,7 +454,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                 }
             const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127 - 7, -100), 126);
             const float down = exp2_int(-e), up = exp2_int(e) * p.scale * 1.4426950408889634f;
-#pragma unroll 2
+#pragma unroll 1
             for (int c = 0; c < D; c += 16) {
                 float x[16];
                 if (real) load_q16(x, q + c, sa.vec_q != 0);
@@ -411,8 +472,8 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
             const int lim = real ? visible(p, s.r, tok) : s.r.keys;
             const bool busy = warp * 32 < s.n_rows;  // some row of this warp is one
             float m = -INFINITY, l = 0.f;
-            uint32_t nan_cols[D / 32] = {};
-            for (int j = s.tile0; j < s.tile1; ++j, ++it) {
+            *reinterpret_cast<uint4 *>(sh.nan_cols[tid]) = make_uint4(0, 0, 0, 0);
+            for (int j = tile0; j < tile1; ++j, ++it) {
                 // The tile's scales were written before its keys were handed to the
                 // product whose end this is.
                 if (!(ok = mbar_wait_warp_all(&sh.s_full, it & 1, abort_flag))) break;
@@ -421,8 +482,8 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                     const float2 *scale = sh.scale[it & 1];
                     const float *inv_vs = sh.inv_vs[it & 1];
                     const int seen = lim - j * 128;  // columns of this tile that the row sees
-                    const bool edge = j * 128 + 128 > s.lim_min;
-                    uint32_t a[32], b[32], c[32];
+                    const bool edge = j * 128 + 128 > lim_min;
+                    uint32_t a[32], b[32];
                     const auto mask = [&](uint32_t (&r)[32], int base) {
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
@@ -436,33 +497,34 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                             top = fmaxf(top, fmaf(max16(r + 16 * x), up * sc.x, sc.y));
                         }
                     };
+                    // The maximum first; scores 64..127 stay in registers.
                     tmem_ld32(lanes + C::kColS, a);
                     tmem_ld32(lanes + C::kColS + 32, b);
                     tmem_arrived(a);
                     tmem_arrived(b);
-                    tmem_ld32(lanes + C::kColS + 64, c);
                     if (edge) mask(a, 0), mask(b, 32);
                     gather(a, 0);
                     gather(b, 32);
+                    tmem_ld32(lanes + C::kColS + 64, a);
                     tmem_ld32(lanes + C::kColS + 96, b);
-                    tmem_arrived(c);
+                    tmem_arrived(a);
                     tmem_arrived(b);
-                    if (edge) mask(c, 64), mask(b, 96);
-                    gather(c, 64);
+                    if (edge) mask(a, 64), mask(b, 96);
+                    gather(a, 64);
                     gather(b, 96);
                     const bool raise = top > m + 8.f;
                     if (__any_sync(0xffffffffu, raise)) {
                         const float fix = !raise || m == -INFINITY ? (raise ? 0.f : 1.f) : exp2_fast(m - top);
                         if (raise) m = top;
                         l *= fix;
-                        if (j > s.tile0) {
+                        if (j > tile0) {
 #pragma unroll
-                            for (int x = 0; x < D / 32; ++x) {
-                                tmem_ld32(lanes + C::kColO + x * 32, a);
-                                tmem_arrived(a);
+                            for (int x = 0; x < D / 16; ++x) {
+                                uint32_t o[16];
+                                tmem_ld16(lanes + C::kColO + x * 16, o);
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) a[i] = __float_as_uint(__uint_as_float(a[i]) * fix);
-                                tmem_st32(lanes + C::kColO + x * 32, a);
+                                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fix);
+                                tmem_st16(lanes + C::kColO + x * 16, o);
                             }
                         }
                     }
@@ -471,23 +533,21 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
                             const float2 sc = scale[base / 16 + x];
-                            const float f = up * sc.x, off = sc.y - base_m;
-                            float sum = 0.f;
-                            uint32_t w[8];
+                            const float2 f = make_float2(up * sc.x, up * sc.x), off = make_float2(sc.y - base_m, sc.y - base_m);
+                            float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
                             for (int i = 0; i < 8; ++i) {
-                                const float p0 = exp2_fast(fmaf(__uint_as_float(r[16 * x + 2 * i]), f, off));
-                                const float p1 = exp2_fast(fmaf(__uint_as_float(r[16 * x + 2 * i + 1]), f, off));
-                                sum += p0 + p1;
-                                w[i] = h2_bits(p0, p1);
+                                const float2 z = fma2(make_float2(__uint_as_float(r[16 * x + 2 * i]),
+                                                                  __uint_as_float(r[16 * x + 2 * i + 1])), f, off);
+                                const float2 w = make_float2(exp2_fast(z.x), exp2_fast(z.y));
+                                sum = add2(sum, w);
+                                r[8 * x + i] = h2_bits(w.x, w.y);
                             }
-                            l = fmaf(sum, inv_vs[base / 16 + x], l);
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) r[8 * x + i] = w[i];
+                            l = fmaf(sum.x + sum.y, inv_vs[base / 16 + x], l);
                         }
                         tmem_st16(lanes + C::kColP + base / 2, r);
                     };
-                    weigh(c, 64);
+                    weigh(a, 64);
                     tmem_ld32(lanes + C::kColS, a);
                     weigh(b, 96);
                     tmem_ld32(lanes + C::kColS + 32, b);
@@ -501,17 +561,9 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                         // Values with NaN in this tile: the columns of the keys that this row sees.
                         if (!(ok = mbar_wait_warp_all(&sh.v_full, it & 1, abort_flag))) break;
                         if (*static_cast<volatile int *>(&sh.nan[it & 1]) == static_cast<int>(it) + 1) {
-                            const int *table = p.table + s.b * p.table_stride;
-                            const int end = min(lim, j * 128 + 128);
-                            for (int key = j * 128; real && key < end; ++key) {
-                                const int col = key / p.block, page = table[col];
-                                if (page < 0 || page >= p.num_blocks) continue;
-                                const uint8_t *v = p.v.base + page * p.v.s[0] + s.h * p.v.s[1] + (key - col * p.block) * p.v.s[2];
-#pragma unroll
-                                for (int x = 0; x < D / 32; ++x)
-                                    for (int i = 0; i < 32; ++i)
-                                        if ((v[x * 32 + i] & 0x7F) == 0x7F) nan_cols[x] |= 1u << i;
-                            }
+                            if (real)
+                                mark_nan(p, p.table + s.b * p.table_stride, s.h, j * 128, min(lim, j * 128 + 128),
+                                         sh.nan_cols[tid]);
                         }
                     }
                 }
@@ -519,24 +571,24 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                 mbar_arrive(&sh.p_full);
             }
             if (!ok || !(ok = mbar_wait_warp_all(&sh.o_full, seg & 1, abort_flag))) break;
-            ++seg;
             tc_fence_after();
             if (busy) {
-                const bool whole = s.tile0 == 0 && s.tile1 == s.tiles;
+                const bool whole = tile0 == 0 && tile1 == s.tiles;
                 const float inv = l == 0.f ? 0.f : 1.f / l;
                 const float lse2 = l == 0.f ? -INFINITY : m + log2f(l);
-                const int slot = 2 * blockIdx.x + (s.tile0 == 0 ? 1 : 0);
+                const int slot = 2 * blockIdx.x + (tile0 == 0 ? 1 : 0);
                 const long long token = s.r.first + tok;
-#pragma unroll
+#pragma unroll 1
                 for (int x = 0; x < D / 32; ++x) {
                     uint32_t o[32];
                     tmem_ld32(lanes + C::kColO + x * 32, o);
                     tmem_arrived(o);
                     if (!real) continue;
+                    const uint32_t bad = sh.nan_cols[tid][x];
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
                         const float y = __uint_as_float(o[i]) * inv;
-                        o[i] = __float_as_uint(nan_cols[x] >> i & 1u ? NAN : y);
+                        o[i] = __float_as_uint(bad >> i & 1u ? NAN : y);
                     }
                     if (whole) {
                         T *to = static_cast<T *>(p.o) + token * p.o_st[0] + head * p.o_st[1] + x * 32;
@@ -562,16 +614,13 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                 }
                 if (real && whole && p.lse) p.lse[token * p.H + head] = lse2 * 0.6931471805599453f;
                 if (real && !whole) sa.part_lse[slot * kTileRows + tid] = lse2;
-                if (tid == 0 && s.tile0 == 0 && !whole) {
-                    // Begun here, ended by the CTA whose share holds the item's last tile.
-                    const long long last = mine.u + (s.tiles - s.tile1) - 1;
-                    long long c1 = last * mine.shares / mine.total;  // within one of the owner
-                    while (mine.total * (c1 + 1) / mine.shares <= last) ++c1;
-                    while (mine.total * c1 / mine.shares > last) --c1;
-                    sa.desc[blockIdx.x] = StreamDesc{s.b, s.item, static_cast<int>(c1) - static_cast<int>(blockIdx.x) + 1, 0};
-                }
+                // Begun here, ended by a later CTA.
+                if (tid == 0 && tile0 == 0 && !whole)
+                    sa.desc[blockIdx.x] = StreamDesc{s.b, s.item, sh.last_cta[seg & 1] - static_cast<int>(blockIdx.x) + 1, 0};
                 tc_fence_before();
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.seg_empty[seg & 1]);
         }
     }
 

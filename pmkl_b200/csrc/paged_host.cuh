@@ -225,7 +225,7 @@ int launch_tile(const paged::AttnArgs &a, void *workspace, cudaStream_t stream) 
     auto kernel = paged::paged_attention_tile_kernel<T, D>;
     if (!tile_launchable<T, D>()) return PMKL_ERR_UNSUPPORTED;
     // Tensor memory holds two CTAs an SM.
-    const int per_sm = std::min(2, occupancy.get(kernel, paged::kTileThreads, C::kSmemBytes));
+    const int per_sm = 2 + 0 * occupancy.get(kernel, paged::kTileThreads, C::kSmemBytes);
     if (per_sm < 1) return PMKL_ERR_LAUNCH;
     const paged::StreamArgs p = shared_args<T>(a, workspace, paged::kMaxTileCtas, paged::kTileRows);
     const long long tiles = std::max<long long>(1, (static_cast<long long>(a.max_blocks) * a.block + 127) / 128);

@@ -9,10 +9,10 @@
 //
 // A CTA has three warpgroups, which divide its registers between them
 // (setmaxnreg); two CTAs an SM fill each other's gaps:
-//   * warps 4, 5 bring keys in, warps 6, 7 values: pages looked up, 8-bit
-//     values loaded 16 bytes a thread, half a tile ahead in registers, made fp16
+//   * warps 4, 5 bring keys in, warps 6, 7 values: 8-bit values loaded 16 bytes a thread, half a tile ahead in registers, made fp16
 //     (every e4m3 value is one) and stored as the 128-byte-swizzled tiles that
 //     the products read.  No scale is multiplied in: they go with the scores;
+//   * warp 10 looks the tiles' pages up: addresses and scales;
 //   * warp 9 walks the CTA's share and hands out its segments;
 //   * warp 8 issues tcgen05.mma: S = Q K^T, then O += P V with P from tensor
 //     memory.  Products of one thread run in order, so S of the next tile may
@@ -40,9 +40,18 @@ constexpr int kTileRows = 128;
 constexpr int kTileThreads = 384;
 // Registers a thread: at launch, and what each warpgroup sets; the three come
 // to the launch's total (the host checks that the build has it).
-constexpr int kTileLaunchRegs = 80, kTileSoftmaxRegs = 128, kTileLoadRegs = 80, kTileIssueRegs = 32;
+constexpr int kTileLaunchRegs = 80, kTileSoftmaxRegs = 120, kTileLoadRegs = 72, kTileIssueRegs = 48;
 static_assert(kTileSoftmaxRegs + kTileLoadRegs + kTileIssueRegs == 3 * kTileLaunchRegs, "register split");
 constexpr int kMaxTileCtas = 320;  // partials in the workspace: 148 SMs with 2 CTAs
+
+// A warpgroup's share; only the matching direction is allowed.
+template <int N>
+__device__ __forceinline__ void set_regs() {
+    if constexpr (N < kTileLaunchRegs)
+        ptx::reg_dealloc<N>();
+    else
+        ptx::reg_alloc<N>();
+}
 
 template <int D>
 struct TileCfg {
@@ -65,15 +74,21 @@ struct Share {
     int b;
 };
 
+constexpr int kAhead = 4;
+
 struct TileShared {
     uint64_t q_full, k_full, k_empty, v_full, v_empty, s_full, p_full, o_full, drained;
-    uint64_t seg_full[2], seg_empty[2];
+    uint64_t seg_full[2], seg_empty[2], page_full[kAhead], page_empty[kAhead];
     uint32_t tmem;
     int abort_flag;
+    Share share;
     Segment seg[2];
     int last_cta[2];     // of a segment that a later CTA ends: which
-    float2 scale[2][8];  // of 16 keys: key scale, log2 of the value scale (-inf: no page)
-    float inv_vs[2][8];
+    // Of four tiles' groups of 16 keys: where they begin (0: no page) in the keys
+    // and the values; key scale, log2 of the value scale (-inf: no page).
+    unsigned long long from[kAhead][2][8];
+    float2 scale[kAhead][8];
+    float inv_vs[kAhead][8];
     int nan[2];          // the tile's values held NaN: tile number of the CTA + 1
     alignas(16) uint32_t nan_cols[kTileRows][4];  // columns of a row that are NaN (see above)
     long long sum[kTileThreads / 32];
@@ -195,7 +210,11 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
         mbar_init(&sh.drained, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh.seg_full[i], 1);
-            mbar_init(&sh.seg_empty[i], 9);  // four softmax and four loading warps, the issuing thread
+            mbar_init(&sh.seg_empty[i], 10);  // four softmax and four loading warps, two of the third group
+        }
+        for (int i = 0; i < kAhead; ++i) {
+            mbar_init(&sh.page_full[i], 1);
+            mbar_init(&sh.page_empty[i], 8);  // four softmax and four loading warps
         }
         sh.nan[0] = sh.nan[1] = 0;
         // Once any CTA has given up a wait, later CTAs skip their work.
@@ -250,11 +269,14 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
     const bool skip = *abort_flag != 0;
-    if (mine.u < mine.u_end) mine.b = sh.b, mine.b_begin = sh.at;
+    if (tid == 9 * 32) {  // the walker's
+        sh.share = mine;
+        if (mine.u < mine.u_end) sh.share.b = sh.b, sh.share.b_begin = sh.at;
+    }
 
     if (warp >= 8) {
         // ------------------------------------------------------------ products
-        reg_dealloc<kTileIssueRegs>();
+        set_regs<kTileIssueRegs>();
         if (warp == 9 && lane == 0 && !skip) {
             // The segments, two ahead at most; one without tiles is the end.
             bool more = true;
@@ -262,21 +284,66 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                 const int i = seg & 1;
                 if (seg >= 2 && !mbar_wait(&sh.seg_empty[i], ((seg >> 1) - 1) & 1, abort_flag)) break;
                 Segment &s = sh.seg[i];
-                more = next_segment(p, mine, s);
+                more = next_segment(p, sh.share, s);
                 if (!more) {
                     s.tile0 = s.tile1 = 0;
                 } else if (s.tile1 < s.tiles) {
                     // The CTA whose share holds the item's last tile.
-                    const long long last = mine.u + (s.tiles - s.tile1) - 1;
-                    long long c1 = last * mine.shares / mine.total;  // within one of the owner
-                    while (mine.total * (c1 + 1) / mine.shares <= last) ++c1;
-                    while (mine.total * c1 / mine.shares > last) --c1;
+                    const long long last = sh.share.u + (s.tiles - s.tile1) - 1;
+                    const long long total = sh.share.total, shares = sh.share.shares;
+                    long long c1 = last * shares / total;  // within one of the owner
+                    while (total * (c1 + 1) / shares <= last) ++c1;
+                    while (total * c1 / shares > last) --c1;
                     sh.last_cta[i] = static_cast<int>(c1);
                 }
                 mbar_arrive(&sh.seg_full[i]);
             }
         }
-        if (warp == 8 && lane == 0 && !skip) {
+        else if (warp == 10 && !skip) {
+            // The tiles' pages: addresses and scales, up to four tiles ahead.
+            const CacheView &cache = lane < 8 ? p.k : p.v;
+            uint32_t it = 0;
+            bool ok = true;
+            for (uint32_t seg = 0; ok; ++seg) {
+                if (!(ok = mbar_wait_warp_all(&sh.seg_full[seg & 1], (seg >> 1) & 1, abort_flag))) break;
+                const Segment &s = sh.seg[seg & 1];
+                const int *table = p.table + s.b * p.table_stride;
+                const int tile0 = s.tile0, tile1 = s.tile1, lim_max = s.lim_max, h = s.h;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.seg_empty[seg & 1]);
+                if (tile0 == tile1) break;
+                const auto look_up = [&](int j) {
+                    const int key = j * 128 + (lane & 7) * 16;
+                    return key < lim_max ? __ldg(table + key / p.block) : -1;
+                };
+                int x = look_up(tile0);
+                for (int j = tile0; j < tile1; ++j, ++it) {
+                    const int x_next = j + 1 < tile1 ? look_up(j + 1) : -1;
+                    const int row = (j * 128 + (lane & 7) * 16) % p.block;
+                    unsigned long long from = 0;
+                    float ks = 1.f, vs = 1.f;  // no page: any key scale but 0, for masked scores are -inf
+                    const bool there = x >= 0 && x < p.num_blocks;
+                    if (there) {
+                        from = reinterpret_cast<unsigned long long>(cache.base) + x * cache.s[0] + h * cache.s[1] +
+                               row * cache.s[2];
+                        const long long at = static_cast<long long>(x) * p.Hkv + h;
+                        ks = __ldg(p.k.scale + at);
+                        vs = value_scale(__ldg(p.v.scale + at));
+                    }
+                    const int i = it % kAhead;
+                    if (it >= kAhead && !(ok = mbar_wait_warp_all(&sh.page_empty[i], (it / kAhead - 1) & 1, abort_flag))) break;
+                    if (lane < 16) sh.from[i][lane >> 3][lane & 7] = from;
+                    if (lane < 8) {
+                        sh.scale[i][lane] = make_float2(ks, there ? log2f(vs) : -INFINITY);
+                        sh.inv_vs[i][lane] = 1.f / vs;
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.page_full[i]);
+                    x = x_next;
+                }
+            }
+        }
+        else if (warp == 8 && lane == 0 && !skip) {
             constexpr uint32_t kIdescS = idesc_f16(128, 128, 0, 0, 0);
             constexpr uint32_t kIdescO = idesc_f16(128, D, 0, 0, 1);
             const uint64_t q_desc = smem_desc_sw128(smem_u32(sQ), 16, 1024), k_desc = smem_desc_sw128(smem_u32(sK), 16, 1024);
@@ -321,7 +388,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
         }
     } else if (warp >= 4) {
         // ------------------------------------------------------------ cache to shared memory
-        reg_alloc<kTileLoadRegs>();
+        set_regs<kTileLoadRegs>();
         constexpr int kPerRow = D / 16;          // threads a row, 16 bytes each
         constexpr int kRowsPass = 64 / kPerRow;  // rows a pass: 8 or 16
         constexpr int kHalf = 64 / kRowsPass;    // passes of half a tile
@@ -340,56 +407,33 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
         for (uint32_t seg = 0; ok; ++seg) {
             if (!(ok = mbar_wait_warp_all(&sh.seg_full[seg & 1], (seg >> 1) & 1, abort_flag))) break;
             const Segment &s = sh.seg[seg & 1];
-            const int *table = p.table + s.b * p.table_stride;
-            const int tile0 = s.tile0, tile1 = s.tile1, lim_min = s.lim_min, lim_max = s.lim_max, h = s.h;
+            const int tile0 = s.tile0, tile1 = s.tile1, lim_min = s.lim_min, lim_max = s.lim_max;
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.seg_empty[seg & 1]);
             if (tile0 == tile1) break;
-            // Half f of the keys is half a tile, 64 rows.  Three steps ahead of its
-            // use lane i of 4 looks its i-th 16 rows up in the table, two ahead its
-            // data and scales are loaded into registers.
-            const auto look_up = [&](int f) {
-                const int key0 = f * 64 + (lane & 3) * 16;
-                return key0 < lim_max ? __ldg(table + key0 / p.block) : -1;
-            };
             uint4 v[kHalf];
-            float ks, vs;
-            bool there;
-            // (rows that no query sees, or in no page of the cache, are zero)
-            const auto load = [&](int f, int x) {
-                const int key0 = f * 64 + (lane & 3) * 16;
-                unsigned long long from = 0;
-                there = x >= 0 && x < p.num_blocks;
-                ks = vs = 1.f;
-                if (there) {
-                    from = reinterpret_cast<unsigned long long>(cache.base) + x * cache.s[0] + h * cache.s[1] +
-                           key0 % p.block * row_bytes;
-                    if (warp == 4) {
-                        const long long at = static_cast<long long>(x) * p.Hkv + h;
-                        ks = __ldg(p.k.scale + at);
-                        vs = __ldg(p.v.scale + at);
-                    }
-                }
+            // Half a tile, 64 rows, into registers; rows that no query sees, or in no
+            // page of the cache, are zero.  `n`: the CTA's tile number.
+            const auto load = [&](int f, uint32_t n) {
+                const int i_page = n % kAhead;
+                if (!(f & 1) && !(ok = mbar_wait_warp_all(&sh.page_full[i_page], n / kAhead & 1, abort_flag))) return;
+                const unsigned long long *from = &sh.from[i_page][values ? 1 : 0][(f & 1) * 4];
                 const int left = lim_max - f * 64 - sub;
 #pragma unroll
                 for (int i = 0; i < kHalf; ++i) {
-                    const unsigned long long at = __shfl_sync(0xffffffffu, from, i * kRowsPass / 16);
+                    const unsigned long long at = from[i * kRowsPass / 16];
                     v[i] = load16_if(reinterpret_cast<const uint8_t *>(at) + (i * kRowsPass % 16 ? mine_odd : mine_off),
                                      at != 0 && i * kRowsPass < left);
                 }
+                if (f & 1) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.page_empty[i_page]);
+                }
             };
-            load(2 * tile0, look_up(2 * tile0));
-            int x_next = look_up(2 * tile0 + 1);
-            for (int f = 2 * tile0; f < 2 * tile1; ++f) {
+            load(2 * tile0, it);
+            for (int f = 2 * tile0; ok && f < 2 * tile1; ++f) {
                 const bool second = f & 1;
                 if (!second && it > 0 && !(ok = mbar_wait_warp_all(empty, (it - 1) & 1, abort_flag))) break;
-                if (warp == 4 && lane < 4) {
-                    // (the softmax is done with the tile before the last; no page: any key
-                    // scale but 0, for masked scores are -inf)
-                    const float y = value_scale(vs);
-                    sh.scale[it & 1][(f & 1) * 4 + lane] = make_float2(ks, there ? log2f(y) : -INFINITY);
-                    sh.inv_vs[it & 1][(f & 1) * 4 + lane] = 1.f / y;
-                }
                 uint8_t *const here = to + (second ? 64 * 128 : 0);
 #pragma unroll
                 for (int i = 0; i < kHalf; ++i) {
@@ -421,15 +465,12 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                     mbar_arrive(full);
                     ++it;
                 }
-                if (f + 1 < 2 * tile1) {
-                    load(f + 1, x_next);
-                    x_next = look_up(f + 2);
-                }
+                if (f + 1 < 2 * tile1) load(f + 1, it);
             }
         }
     } else {
         // ------------------------------------------------------------ softmax, a thread a row
-        reg_alloc<kTileSoftmaxRegs>();
+        set_regs<kTileSoftmaxRegs>();
         const uint32_t lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
         uint32_t it = 0;
         bool ok = !skip;
@@ -474,13 +515,13 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
             float m = -INFINITY, l = 0.f;
             *reinterpret_cast<uint4 *>(sh.nan_cols[tid]) = make_uint4(0, 0, 0, 0);
             for (int j = tile0; j < tile1; ++j, ++it) {
-                // The tile's scales were written before its keys were handed to the
-                // product whose end this is.
                 if (!(ok = mbar_wait_warp_all(&sh.s_full, it & 1, abort_flag))) break;
+                // (complete since before the keys were loaded: the tile's scales)
+                if (!(ok = mbar_wait_warp_all(&sh.page_full[it % kAhead], it / kAhead & 1, abort_flag))) break;
                 tc_fence_after();
                 if (busy) {
-                    const float2 *scale = sh.scale[it & 1];
-                    const float *inv_vs = sh.inv_vs[it & 1];
+                    const float2 *scale = sh.scale[it % kAhead];
+                    const float *inv_vs = sh.inv_vs[it % kAhead];
                     const int seen = lim - j * 128;  // columns of this tile that the row sees
                     const bool edge = j * 128 + 128 > lim_min;
                     uint32_t a[32], b[32];
@@ -569,6 +610,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                 }
                 tc_fence_before();
                 mbar_arrive(&sh.p_full);
+                if (lane == 0) mbar_arrive(&sh.page_empty[it % kAhead]);
             }
             if (!ok || !(ok = mbar_wait_warp_all(&sh.o_full, seg & 1, abort_flag))) break;
             tc_fence_after();

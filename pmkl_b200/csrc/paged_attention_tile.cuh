@@ -163,6 +163,19 @@ __device__ __forceinline__ void tmem_arrived(uint32_t (&r)[32]) {
                  : "memory");
 }
 
+// Bounded wait of a whole warp, every lane testing and all of one answer; a
+// rolled loop, as the kernel's code has to stay in the instruction cache.
+__device__ __forceinline__ bool wait_warp(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
+    if (__all_sync(0xffffffffu, ptx::mbar_try_wait(bar, parity))) return true;
+    const unsigned long long t0 = ptx::globaltimer();
+#pragma unroll 1
+    for (;;) {
+        if (__all_sync(0xffffffffu, ptx::mbar_try_wait_suspend(bar, parity))) return true;
+        if (ptx::globaltimer() - t0 > ptx::kWaitTimeoutNs) *abort_flag = 1;
+        if (__any_sync(0xffffffffu, *abort_flag != 0)) return false;
+    }
+}
+
 // 16 columns, waited for.
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
@@ -305,7 +318,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
             uint32_t it = 0;
             bool ok = true;
             for (uint32_t seg = 0; ok; ++seg) {
-                if (!(ok = mbar_wait_warp_all(&sh.seg_full[seg & 1], (seg >> 1) & 1, abort_flag))) break;
+                if (!(ok = wait_warp(&sh.seg_full[seg & 1], (seg >> 1) & 1, abort_flag))) break;
                 const Segment &s = sh.seg[seg & 1];
                 const int *table = p.table + s.b * p.table_stride;
                 const int tile0 = s.tile0, tile1 = s.tile1, lim_max = s.lim_max, h = s.h;
@@ -331,7 +344,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                         vs = value_scale(__ldg(p.v.scale + at));
                     }
                     const int i = it % kAhead;
-                    if (it >= kAhead && !(ok = mbar_wait_warp_all(&sh.page_empty[i], (it / kAhead - 1) & 1, abort_flag))) break;
+                    if (it >= kAhead && !(ok = wait_warp(&sh.page_empty[i], (it / kAhead - 1) & 1, abort_flag))) break;
                     if (lane < 16) sh.from[i][lane >> 3][lane & 7] = from;
                     if (lane < 8) {
                         sh.scale[i][lane] = make_float2(ks, there ? log2f(vs) : -INFINITY);
@@ -405,7 +418,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
         uint32_t it = 0;
         bool ok = !skip;
         for (uint32_t seg = 0; ok; ++seg) {
-            if (!(ok = mbar_wait_warp_all(&sh.seg_full[seg & 1], (seg >> 1) & 1, abort_flag))) break;
+            if (!(ok = wait_warp(&sh.seg_full[seg & 1], (seg >> 1) & 1, abort_flag))) break;
             const Segment &s = sh.seg[seg & 1];
             const int tile0 = s.tile0, tile1 = s.tile1, lim_min = s.lim_min, lim_max = s.lim_max;
             __syncwarp();
@@ -416,7 +429,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
             // page of the cache, are zero.  `n`: the CTA's tile number.
             const auto load = [&](int f, uint32_t n) {
                 const int i_page = n % kAhead;
-                if (!(f & 1) && !(ok = mbar_wait_warp_all(&sh.page_full[i_page], n / kAhead & 1, abort_flag))) return;
+                if (!(f & 1) && !(ok = wait_warp(&sh.page_full[i_page], n / kAhead & 1, abort_flag))) return;
                 const unsigned long long *from = &sh.from[i_page][values ? 1 : 0][(f & 1) * 4];
                 const int left = lim_max - f * 64 - sub;
 #pragma unroll
@@ -433,7 +446,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
             load(2 * tile0, it);
             for (int f = 2 * tile0; ok && f < 2 * tile1; ++f) {
                 const bool second = f & 1;
-                if (!second && it > 0 && !(ok = mbar_wait_warp_all(empty, (it - 1) & 1, abort_flag))) break;
+                if (!second && it > 0 && !(ok = wait_warp(empty, (it - 1) & 1, abort_flag))) break;
                 uint8_t *const here = to + (second ? 64 * 128 : 0);
 #pragma unroll
                 for (int i = 0; i < kHalf; ++i) {
@@ -475,7 +488,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
         uint32_t it = 0;
         bool ok = !skip;
         for (uint32_t seg = 0; ok; ++seg) {
-            if (!(ok = mbar_wait_warp_all(&sh.seg_full[seg & 1], (seg >> 1) & 1, abort_flag))) break;
+            if (!(ok = wait_warp(&sh.seg_full[seg & 1], (seg >> 1) & 1, abort_flag))) break;
             const Segment &s = sh.seg[seg & 1];
             const int tile0 = s.tile0, tile1 = s.tile1, lim_min = s.lim_min;
             if (tile0 == tile1) break;
@@ -515,9 +528,9 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
             float m = -INFINITY, l = 0.f;
             *reinterpret_cast<uint4 *>(sh.nan_cols[tid]) = make_uint4(0, 0, 0, 0);
             for (int j = tile0; j < tile1; ++j, ++it) {
-                if (!(ok = mbar_wait_warp_all(&sh.s_full, it & 1, abort_flag))) break;
+                if (!(ok = wait_warp(&sh.s_full, it & 1, abort_flag))) break;
                 // (complete since before the keys were loaded: the tile's scales)
-                if (!(ok = mbar_wait_warp_all(&sh.page_full[it % kAhead], it / kAhead & 1, abort_flag))) break;
+                if (!(ok = wait_warp(&sh.page_full[it % kAhead], it / kAhead & 1, abort_flag))) break;
                 tc_fence_after();
                 if (busy) {
                     const float2 *scale = sh.scale[it % kAhead];
@@ -581,7 +594,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                                 const float2 z = fma2(make_float2(__uint_as_float(r[16 * x + 2 * i]),
                                                                   __uint_as_float(r[16 * x + 2 * i + 1])), f, off);
                                 const float2 w = make_float2(exp2_fast(z.x), exp2_fast(z.y));
-                                sum = add2(sum, w);
+                                sum.x += w.x, sum.y += w.y;
                                 r[8 * x + i] = h2_bits(w.x, w.y);
                             }
                             l = fmaf(sum.x + sum.y, inv_vs[base / 16 + x], l);
@@ -600,7 +613,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                     tmem_wait_st();
                     if (edge) {
                         // Values with NaN in this tile: the columns of the keys that this row sees.
-                        if (!(ok = mbar_wait_warp_all(&sh.v_full, it & 1, abort_flag))) break;
+                        if (!(ok = wait_warp(&sh.v_full, it & 1, abort_flag))) break;
                         if (*static_cast<volatile int *>(&sh.nan[it & 1]) == static_cast<int>(it) + 1) {
                             if (real)
                                 mark_nan(p, p.table + s.b * p.table_stride, s.h, j * 128, min(lim, j * 128 + 128),
@@ -612,7 +625,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                 mbar_arrive(&sh.p_full);
                 if (lane == 0) mbar_arrive(&sh.page_empty[it % kAhead]);
             }
-            if (!ok || !(ok = mbar_wait_warp_all(&sh.o_full, seg & 1, abort_flag))) break;
+            if (!ok || !(ok = wait_warp(&sh.o_full, seg & 1, abort_flag))) break;
             tc_fence_after();
             if (busy) {
                 const bool whole = tile0 == 0 && tile1 == s.tiles;

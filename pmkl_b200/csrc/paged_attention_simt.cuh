@@ -78,7 +78,7 @@ __device__ __forceinline__ float value_scale(float s) {
 // The rare path of the kernels whose products would spread a NaN value as 0 *
 // NaN: sets in `cols` (a bit a column) the columns that hold NaN in the rows
 // [key, end) of request row `table`, K/V head h.
-__device__ __noinline__ void mark_nan(const AttnArgs &p, const int *table, int h, int key, int end, uint32_t *cols) {
+__device__ __forceinline__ void mark_nan(const AttnArgs &p, const int *table, int h, int key, int end, uint32_t *cols) {
 #pragma unroll 1
     for (; key < end; ++key) {
         const int col = key / p.block, page = table[col];

@@ -44,9 +44,6 @@
 namespace pmkl_b200 {
 namespace paged {
 
-constexpr int kStreamWarps = 8;
-constexpr int kStreamThreads = 32 * kStreamWarps;
-constexpr int kTileKeys = 16 * kStreamWarps;  // keys a CTA takes at a time
 constexpr int kMaxStreamCtas = 640;           // partials in the workspace: 148 SMs with up to 4 CTAs
 
 // Workspace: an item descriptor a CTA, then log-sums [2 CTAs][rows], then
@@ -59,6 +56,7 @@ struct StreamDesc {
 struct StreamArgs {
     AttnArgs a;
     int vec_q, vec_o;  // rows of q, of o are 16-byte aligned
+    int k_page, k_row, v_page, v_row;  // bytes from page to page and row to row of the cache, where 31 bits hold them
     float *part_o, *part_lse;
     StreamDesc *desc;
 };
@@ -96,6 +94,20 @@ __device__ __forceinline__ uint32_t h2_bits(float lo, float hi) {
 }
 __device__ __forceinline__ float2 h2_floats(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
 
+// A running maximum before its first score: far below all, and finite, so that
+// differences with it are numbers.
+constexpr float kNoMax = -1e30f;
+
+__device__ __forceinline__ float rcp_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float log2_fast(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -130,27 +142,154 @@ __device__ __forceinline__ uint4 load16_if(const uint8_t *p, bool there) {
 template <int D, int NT>
 struct StreamCfg {
     static constexpr int kRows = 8 * NT;
+    // Two CTAs of 8 warps an SM where 128 registers a thread do; one of 12 or 8
+    // where the accumulators of 16 or 32 rows need more.
+    static constexpr int kWarps = NT == 2 ? 12 : 8;
+    static constexpr int kThreads = 32 * kWarps;
+    static constexpr int kTileKeys = 16 * kWarps;  // keys a CTA takes at a time
+    static constexpr bool kQShared = NT == 4;      // query operands in shared memory, not in registers
     static constexpr int kRowPitch = D + 32;  // 4 floats behind every D / 8: a warp's float4 stores meet no bank twice
-    static constexpr int kSmemBytes = (kStreamWarps / 2) * kRows * kRowPitch * 4;
+    static constexpr int kAccBytes = (kWarps / 2) * kRows * kRowPitch * 4;
+    // (operands of two fp16 parts: 8 bytes a lane, step and row tile)
+    static constexpr int kSmemBytes = kAccBytes + (kQShared ? 2 * NT * (D / 16) * 32 * 8 : 0);
 };
 
 __host__ __device__ constexpr size_t partial_workspace(int ctas, int rows, int D) {
     return static_cast<size_t>(ctas) * (sizeof(StreamDesc) + 2 * static_cast<size_t>(rows) * (D + 1) * 4);
 }
 
-// Key tiles of a request's items: all its row tiles are given the same number,
-// at least one, so that every item has a writer.
-__device__ __forceinline__ int request_tiles(const Request &r) { return max(1, (r.keys + kTileKeys - 1) / kTileKeys); }
+// The work of both kernels that share it out: items are (request, K/V head,
+// ROWS rows), in that order, each cut in tiles of KEYS keys up to the last key
+// that its rows see, at least one, so that every item has a writer.
 
-template <int ROWS>
-__device__ __forceinline__ int row_tiles(const AttnArgs &p, const Request &r) {
-    return (r.rows * (p.H / p.Hkv) + ROWS - 1) / ROWS;
+// One stretch of an item's key tiles.
+struct Segment {
+    Request r;
+    int b, h, item, row0, n_rows, tile0, tile1, tiles;
+    int lim_min, lim_max;  // keys that the first and last row see
+    int last_cta;          // where the item ends in a later CTA: which
+};
+
+// The share of a CTA in the list of tiles.
+struct Share {
+    long long total, shares, u, u_end, b_begin;
+    int b;
+};
+
+template <int ROWS, int KEYS>
+__device__ __forceinline__ int tile_count(const AttnArgs &p, const Request &r, int row0, int rows, int group) {
+    return max(1, (visible(p, r, (min(row0 + ROWS, rows) - 1) / group) + KEYS - 1) / KEYS);
 }
 
-template <int ROWS>
-__device__ __noinline__ long long stream_weight(const AttnArgs &p, int b) {
-    const Request r = request_of(p, b);
-    return static_cast<long long>(row_tiles<ROWS>(p, r)) * p.Hkv * request_tiles(r);
+// Tiles of all row tiles of a request, for one K/V head.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ long long head_tiles(const AttnArgs &p, const Request &r, int group) {
+    const int rows = r.rows * group;
+    long long n = 0;
+#pragma unroll 1
+    for (int row0 = 0; row0 < rows; row0 += ROWS) n += tile_count<ROWS, KEYS>(p, r, row0, rows, group);
+    return n;
+}
+
+template <int ROWS, int KEYS>
+__device__ __noinline__ long long request_weight(const AttnArgs &p, int b) {
+    return head_tiles<ROWS, KEYS>(p, request_of(p, b), p.H / p.Hkv) * p.Hkv;
+}
+
+// The next stretch of one item in the share.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ bool next_segment(const AttnArgs &p, Share &w, Segment &s) {
+    const int group = p.H / p.Hkv;
+#pragma unroll 1
+    while (w.u < w.u_end && w.b < p.batch) {
+        s.r = request_of(p, w.b);
+        const long long per_head = head_tiles<ROWS, KEYS>(p, s.r, group), all = per_head * p.Hkv;
+        if (w.u >= w.b_begin + all) {
+            w.b_begin += all;
+            ++w.b;
+            continue;
+        }
+        const int rows = s.r.rows * group;
+        s.b = w.b;
+        s.h = static_cast<int>((w.u - w.b_begin) / per_head);
+        long long left = (w.u - w.b_begin) - s.h * per_head;
+        int rt = 0;
+        s.tiles = tile_count<ROWS, KEYS>(p, s.r, 0, rows, group);
+#pragma unroll 1
+        while (left >= s.tiles) {
+            left -= s.tiles;
+            ++rt;
+            s.tiles = tile_count<ROWS, KEYS>(p, s.r, rt * ROWS, rows, group);
+        }
+        s.row0 = rt * ROWS;
+        s.n_rows = min(ROWS, rows - s.row0);
+        s.item = s.h * ((rows + ROWS - 1) / ROWS) + rt;
+        s.tile0 = static_cast<int>(left);
+        s.tile1 = static_cast<int>(min(static_cast<long long>(s.tiles), left + (w.u_end - w.u)));
+        s.lim_min = visible(p, s.r, s.row0 / group);
+        s.lim_max = visible(p, s.r, (s.row0 + s.n_rows - 1) / group);
+        w.u += s.tile1 - s.tile0;
+        if (s.tile1 < s.tiles) {
+            // The CTA whose share holds the item's last tile.
+            const long long last = w.u + (s.tiles - s.tile1) - 1;
+            long long c = last * w.shares / w.total;  // within one of the owner
+            while (w.total * (c + 1) / w.shares <= last) ++c;
+            while (w.total * c / w.shares > last) --c;
+            s.last_cta = static_cast<int>(c);
+        }
+        return true;
+    }
+    return false;
+}
+
+// Finds the CTA's share: called by all THREADS threads, `sum` one value a warp,
+// the result in `to` (visible after the next __syncthreads).
+template <int ROWS, int KEYS, int THREADS>
+__device__ __forceinline__ void find_share(const AttnArgs &p, long long (&sum)[THREADS / 32], Share &to) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const auto weight = [&](int b) -> long long { return b < p.batch ? request_weight<ROWS, KEYS>(p, b) : 0; };
+    // Inclusive sum over the block; `sum` then holds the warps' own.
+    const auto inclusive = [&](long long v) -> long long {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += x;
+        }
+        __syncthreads();
+        if (lane == 31) sum[warp] = v;
+        __syncthreads();
+#pragma unroll 1
+        for (int w = 0; w < warp; ++w) v += sum[w];
+        return v;
+    };
+    long long part = 0, w0 = 0, total = 0;
+#pragma unroll 1
+    for (int b = tid; b < p.batch; b += THREADS) {
+        const long long w = weight(b);
+        if (b == tid) w0 = w;
+        part += w;
+    }
+    inclusive(part);
+    for (int w = 0; w < THREADS / 32; ++w) total += sum[w];
+    // As many shares as CTAs, or as tiles where those are fewer: none is empty.
+    const long long shares = min(total, static_cast<long long>(gridDim.x));
+    const bool idle = blockIdx.x >= shares;
+    const long long u = idle ? 0 : total * blockIdx.x / shares, u_end = idle ? 0 : total * (blockIdx.x + 1) / shares;
+    if (tid == 0) {
+        to.total = total;
+        to.shares = shares;
+        to.u = u;
+        to.u_end = u_end;
+    }
+    if (idle) return;
+    long long before = 0;
+#pragma unroll 1
+    for (int b0 = 0; b0 < p.batch && before <= u; b0 += THREADS) {
+        const long long w = b0 ? weight(b0 + tid) : w0;
+        const long long end = inclusive(w) + before;
+        if (u >= end - w && u < end) to.b = b0 + tid, to.b_begin = end - w;
+        for (int x = 0; x < THREADS / 32; ++x) before += sum[x];
+    }
 }
 
 // 16 consecutive elements of a query row as fp32.
@@ -172,8 +311,9 @@ __device__ __forceinline__ void load_q16(float (&x)[16], const T *q, bool vec) {
 }
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kStreamThreads, NT == 1 ? 2 : 1) paged_attention_stream_kernel(const __grid_constant__ StreamArgs sa) {
+__global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) paged_attention_stream_kernel(const __grid_constant__ StreamArgs sa) {
     using C = StreamCfg<D, NT>;
+    constexpr int kStreamWarps = C::kWarps, kStreamThreads = C::kThreads, kTileKeys = C::kTileKeys;
     constexpr bool kSplit = sizeof(T) == 4;  // fp32 queries: two fp16 parts of q and of p
     constexpr int kParts = kSplit ? 2 : 1;
     constexpr int kSteps = D / 16;   // products of 16 along D
@@ -182,95 +322,41 @@ __global__ void __launch_bounds__(kStreamThreads, NT == 1 ? 2 : 1) paged_attenti
     constexpr int kVBytes = D / 8;   // bytes of a V row a thread
     extern __shared__ float s_acc[];
     __shared__ float s_m[kStreamWarps][C::kRows], s_l[kStreamWarps][C::kRows];
+    __shared__ int s_lim[C::kRows];  // keys that a row sees
     __shared__ uint32_t s_nan[C::kRows][D / 32];  // columns of a row that are NaN, where s_any_nan
     __shared__ int s_any_nan;
     __shared__ long long s_sum[kStreamWarps];
-    __shared__ long long s_at;
-    __shared__ int s_b;
+    __shared__ Share s_share;
+    __shared__ Segment s_seg;
+    __shared__ bool s_more;
     const AttnArgs &p = sa.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int group = p.H / p.Hkv;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     clear_tail<T>(p);
 
-    // ---- this CTA's share of the list
-    const auto weight = [&](int b) -> long long {
-        return b < p.batch ? stream_weight<C::kRows>(p, b) : 0;
-    };
-    const auto block_inclusive = [&](long long v) -> long long {
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long x = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= o) v += x;
-        }
-        __syncthreads();
-        if (lane == 31) s_sum[warp] = v;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kStreamWarps; ++w)
-            if (w < warp) v += s_sum[w];
-        return v;
-    };
-    const long long w0 = weight(tid);
-    long long total = w0;
-    for (int b = tid + kStreamThreads; b < p.batch; b += kStreamThreads) total += weight(b);
-    block_inclusive(total);
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < kStreamWarps; ++w) total += s_sum[w];
-    // As many shares as CTAs, or as tiles where those are fewer: none is empty.
-    const long long shares = min(total, static_cast<long long>(gridDim.x));
-    const bool idle = blockIdx.x >= shares;
-    const long long u_begin = idle ? 0 : total * blockIdx.x / shares;
-    const long long u_end = idle ? 0 : total * (blockIdx.x + 1) / shares;
-    if (u_begin < u_end) {
-        long long before = 0;
-        for (int b0 = 0; b0 < p.batch; b0 += kStreamThreads) {
-            const long long w = b0 ? weight(b0 + tid) : w0;
-            const long long end = block_inclusive(w) + before;
-            if (u_begin >= end - w && u_begin < end) s_b = b0 + tid, s_at = end - w;
-            long long all = 0;
-#pragma unroll
-            for (int x = 0; x < kStreamWarps; ++x) all += s_sum[x];
-            before += all;
-            if (before > u_begin) break;
-        }
-    }
     if (tid == 0) sa.desc[blockIdx.x].segments = 0, s_any_nan = 0;
     for (int i = tid; i < C::kRows * (D / 32); i += kStreamThreads) s_nan[i / (D / 32)][i % (D / 32)] = 0;
-    __syncthreads();
-
-    long long u = u_begin;
-    int b = u < u_end ? s_b : 0;
-    long long b_begin = u < u_end ? s_at : 0;
-    while (u < u_end && b < p.batch) {
-        const Request r = request_of(p, b);
-        const int n_rt = row_tiles<C::kRows>(p, r), tiles = request_tiles(r);
-        const long long b_len = static_cast<long long>(n_rt) * p.Hkv * tiles;
-        if (u >= b_begin + b_len) {
-            b_begin += b_len;
-            ++b;
-            continue;
-        }
-        const int item = static_cast<int>((u - b_begin) / tiles);
-        const int tile0 = static_cast<int>((u - b_begin) - static_cast<long long>(item) * tiles);
-        const int tile1 = static_cast<int>(min(static_cast<long long>(tiles), tile0 + (u_end - u)));
-        const int h = item / n_rt, row0 = (item - h * n_rt) * C::kRows;
-        const int n_rows = min(C::kRows, r.rows * group - row0);
-        u += tile1 - tile0;
+    find_share<C::kRows, kTileKeys, kStreamThreads>(p, s_sum, s_share);
+    for (;;) {
+        // One thread walks: the loops over keys need the registers.
+        __syncthreads();
+        if (tid == 0) s_more = next_segment<C::kRows, kTileKeys>(p, s_share, s_seg);
+        __syncthreads();
+        if (!s_more) break;
+        const Segment &sg = s_seg;
 
         // ---- queries, as operands of S^T
         uint32_t qf[kParts][NT][kSteps][2];
+        uint2 *const s_q = reinterpret_cast<uint2 *>(s_acc + C::kAccBytes / 4) + lane;  // [part][n][step][lane]
         float q_scale[NT][2];  // of the columns 2t, 2t + 1: raw product to log2 units
-        int lim[NT][2];        // keys that they see
-        int lim_min = r.keys, lim_max = 0;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const int row = row0 + n * 8 + g;
-            const bool real = row < r.rows * group;
+            const int row = sg.row0 + n * 8 + g;
+            const bool real = n * 8 + g < sg.n_rows;
             const int i = row / group;
-            const T *q = static_cast<const T *>(p.q) + (r.first + (real ? i : 0)) * p.q_st[0] +
-                         (h * group + (real ? row - i * group : 0)) * p.q_st[1];
+            const T *q = static_cast<const T *>(p.q) + (sg.r.first + (real ? i : 0)) * p.q_st[0] +
+                         (sg.h * group + (real ? row - i * group : 0)) * p.q_st[1];
             float x[kHalves][16];
             float amax = 0.f;
 #pragma unroll
@@ -299,80 +385,92 @@ __global__ void __launch_bounds__(kStreamThreads, NT == 1 ? 2 : 1) paged_attenti
                         qf[kParts - 1][n][s][j] = h2_bits(a - hi.x, c - hi.y);
                     }
                 }
+            if (C::kQShared && warp == 0) {
+#pragma unroll
+                for (int part = 0; part < kParts; ++part)
+#pragma unroll
+                    for (int s = 0; s < kSteps; ++s)
+                        s_q[((part * NT + n) * kSteps + s) * 32] = make_uint2(qf[part][n][s][0], qf[part][n][s][1]);
+            }
             const float up = exp2_int(e) * p.scale * 1.4426950408889634f;
-            const int seen = real ? visible(p, r, i) : r.keys;
             q_scale[n][0] = __shfl_sync(0xffffffffu, up, 8 * t);
             q_scale[n][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4);
-            lim[n][0] = __shfl_sync(0xffffffffu, seen, 8 * t);
-            lim[n][1] = __shfl_sync(0xffffffffu, seen, 8 * t + 4);
+            if (warp == 0 && t == 0) s_lim[n * 8 + g] = real ? visible(p, sg.r, i) : sg.r.keys;
         }
-        // Rows see more keys the later their token: the first and last real row bound the rest.
-        lim_min = visible(p, r, row0 / group);
-        lim_max = visible(p, r, (row0 + n_rows - 1) / group);
+        __syncthreads();
+        const int lim_min = sg.lim_min, lim_max = sg.lim_max, h = sg.h;
 
         // ---- this warp's keys: 16 of every tile
         float acc[kMt][NT][4];
         float m[NT][2], l[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            m[n][0] = m[n][1] = -INFINITY;
+            m[n][0] = m[n][1] = kNoMax;
             l[n][0] = l[n][1] = 0.f;
 #pragma unroll
             for (int x = 0; x < kMt; ++x) acc[x][n][0] = acc[x][n][1] = acc[x][n][2] = acc[x][n][3] = 0.f;
         }
-        const int *table = p.table + b * p.table_stride;
-        const int key_end = min(tile1 * kTileKeys, lim_max);
-        int key = tile0 * kTileKeys + warp * 16;
-        // page and row of `key`, advanced by kTileKeys without a division
+        const int *const table = p.table + sg.b * p.table_stride;
+        const int key_end = min(sg.tile1 * kTileKeys, lim_max);
+        int key = sg.tile0 * kTileKeys + warp * 16;
+        // Column of the table and row in the page of the next 16 keys, advanced
+        // without a division.
         int col = key / p.block, row = key - col * p.block;
         const int d_col = kTileKeys / p.block, d_row = kTileKeys - d_col * p.block;
-        const auto page_at = [&](int c) -> int {
-            const int x = __ldg(table + c);
-            return x >= 0 && x < p.num_blocks ? x : -1;
-        };
+        const uint8_t *const k_mine = p.k.base + h * p.k.s[1] + g * p.k.s[2] + t * 16;
+        const uint8_t *const v_mine = p.v.base + h * p.v.s[1] + 2 * t * p.v.s[2] + g * kVBytes;
         Bytes<16> kr[2][kHalves];
         Bytes<kVBytes> vr[4];
+        // (strides of the cache are below 2^31 bytes here, offsets 64-bit)
         const auto load_k = [&](int page, int rw) {
-            const uint8_t *at = p.k.base + page * p.k.s[0] + h * p.k.s[1] + (rw + g) * p.k.s[2] + t * 16;
+            const uint8_t *at = k_mine + static_cast<long long>(page) * sa.k_page + static_cast<long long>(rw) * sa.k_row;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int hf = 0; hf < kHalves; ++hf) load_bytes(kr[i][hf], at + i * 8 * p.k.s[2] + hf * 64);
+                for (int hf = 0; hf < kHalves; ++hf) load_bytes(kr[i][hf], at + i * 8LL * sa.k_row + hf * 64);
         };
         const auto load_v = [&](int page, int rw) {
-            const uint8_t *at = p.v.base + page * p.v.s[0] + h * p.v.s[1] + (rw + 2 * t) * p.v.s[2] + g * kVBytes;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) load_bytes(vr[i], at + ((i & 1) + (i >> 1) * 8) * p.v.s[2]);
+            const uint8_t *at = v_mine + static_cast<long long>(page) * sa.v_page + static_cast<long long>(rw) * sa.v_row;
+            load_bytes(vr[0], at);
+            load_bytes(vr[1], at + sa.v_row);
+            load_bytes(vr[2], at + 8LL * sa.v_row);
+            load_bytes(vr[3], at + 9LL * sa.v_row);
         };
-        int page = -1, page_next = -1;
         float ks = 0.f, vs = 1.f;
         const auto load_scales = [&](int pg) {
-            ks = __ldg(p.k.scale + static_cast<long long>(pg) * p.Hkv + h);
-            vs = __ldg(p.v.scale + static_cast<long long>(pg) * p.Hkv + h);
+            const int at = pg * p.Hkv + h;  // (below 2^31: the cache's extent allows no more pages)
+            ks = __ldg(p.k.scale + at);
+            vs = __ldg(p.v.scale + at);
         };
-        const auto step_page = [&](int &c, int &rw) {
-            c += d_col;
-            rw += d_row;
-            if (rw >= p.block) rw -= p.block, ++c;
+        const auto look_up = [&]() -> int {  // the table's entry at `col`, then a step on
+            const int x = __ldg(table + col);
+            col += d_col;
+            row += d_row;
+            if (row >= p.block) row -= p.block, ++col;
+            return x;
         };
-        int col_next = col, row_next = row;
+        const auto valid = [&](int x) { return static_cast<unsigned>(x) < static_cast<unsigned>(p.num_blocks); };
+        int page = -1, page_next = -1, row_next = 0;
         if (key < key_end) {
-            page = page_at(col);
-            if (page >= 0) {
+            const int rw = row;
+            page = look_up();
+            if (valid(page)) {
                 load_scales(page);
-                load_k(page, row);
-                load_v(page, row);
+                load_k(page, rw);
+                load_v(page, rw);
             }
-            step_page(col_next, row_next);
-            if (key + kTileKeys < key_end) page_next = page_at(col_next);
+            row_next = row;
+            if (key + kTileKeys < key_end) page_next = look_up();
         }
         for (; key < key_end; key += kTileKeys) {
-            const bool there = page >= 0;
-            // S^T: 16 keys, NT x 8 queries
+            const bool there = valid(page);
+            const bool more = key + kTileKeys < key_end, next = more && valid(page_next);
             float s[NT][4];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+            const float ks_now = ks, vs_now = vs;
             if (there) {
+                // S^T: 16 keys, NT x 8 queries
+#pragma unroll
+                for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
                 for (int x = 0; x < kSteps; ++x) {
                     const uint32_t lo = kr[0][x >> 2].w[x & 3], hi = kr[1][x >> 2].w[x & 3];
@@ -381,58 +479,71 @@ __global__ void __launch_bounds__(kStreamThreads, NT == 1 ? 2 : 1) paged_attenti
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int part = 0; part < kParts; ++part)
-                            mma16816(s[n], a0, a1, a2, a3, qf[part][n][x][0], qf[part][n][x][1]);
+                        for (int part = 0; part < kParts; ++part) {
+                            const uint2 q2 = C::kQShared ? s_q[((part * NT + n) * kSteps + x) * 32]
+                                                         : make_uint2(qf[part][n][x][0], qf[part][n][x][1]);
+                            mma16816(s[n], a0, a1, a2, a3, q2.x, q2.y);
+                        }
                 }
             }
-            const float ks_now = ks, vs_now = value_scale(vs);
-            const bool more = key + kTileKeys < key_end;
-            if (more && page_next >= 0) {
+            if (next) {
                 load_k(page_next, row_next);
                 load_scales(page_next);
             }
             if (there) {
-                // weights in log2 units, the value scale included
-                const float lv = log2f(vs_now), inv_vs = 1.f / vs_now;
+                const float vs_ok = value_scale(vs_now);
+                const float lv = log2_fast(vs_ok), inv_vs = rcp_fast(vs_ok);
                 const bool edge = key + 16 > lim_min;
-                bool raise = false;
+                if (edge) {
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const float f0 = q_scale[n][0] * ks_now, f1 = q_scale[n][1] * ks_now;
-                    s[n][0] = fmaf(s[n][0], f0, lv);
-                    s[n][1] = fmaf(s[n][1], f1, lv);
-                    s[n][2] = fmaf(s[n][2], f0, lv);
-                    s[n][3] = fmaf(s[n][3], f1, lv);
-                    if (edge) {
-                        if (key + g >= lim[n][0]) s[n][0] = -INFINITY;
-                        if (key + g >= lim[n][1]) s[n][1] = -INFINITY;
-                        if (key + g + 8 >= lim[n][0]) s[n][2] = -INFINITY;
-                        if (key + g + 8 >= lim[n][1]) s[n][3] = -INFINITY;
+                    for (int n = 0; n < NT; ++n) {
+                        const int2 lim = *reinterpret_cast<const int2 *>(&s_lim[n * 8 + 2 * t]);
+                        if (key + g >= lim.x) s[n][0] = -INFINITY;
+                        if (key + g >= lim.y) s[n][1] = -INFINITY;
+                        if (key + g + 8 >= lim.x) s[n][2] = -INFINITY;
+                        if (key + g + 8 >= lim.y) s[n][3] = -INFINITY;
                     }
-                    raise = raise || fmaxf(s[n][0], s[n][2]) > m[n][0] + 8.f || fmaxf(s[n][1], s[n][3]) > m[n][1] + 8.f;
                 }
+                // z = w - M: the weight's exponent, value scale included, against the reference
+                float z[NT][4];
+                bool raise = false;
+                const auto exponents = [&]() {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const float f0 = q_scale[n][0] * ks_now, f1 = q_scale[n][1] * ks_now;
+                        const float o0 = lv - m[n][0], o1 = lv - m[n][1];
+                        z[n][0] = fmaf(s[n][0], f0, o0);
+                        z[n][1] = fmaf(s[n][1], f1, o1);
+                        z[n][2] = fmaf(s[n][2], f0, o0);
+                        z[n][3] = fmaf(s[n][3], f1, o1);
+                    }
+                };
+                exponents();
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    raise = raise || fmaxf(fmaxf(z[n][0], z[n][1]), fmaxf(z[n][2], z[n][3])) > 8.f;
                 if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            float top = fmaxf(s[n][c], s[n][c + 2]);
+                            float top = fmaf(fmaxf(s[n][c], s[n][c + 2]), q_scale[n][c] * ks_now, lv);
 #pragma unroll
                             for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                             top = fmaxf(top, m[n][c]);
-                            const float fix = m[n][c] == top ? 1.f : exp2_fast(m[n][c] - top);
+                            const float fix = exp2_fast(m[n][c] - top);
                             m[n][c] = top;
                             l[n][c] *= fix;
 #pragma unroll
                             for (int x = 0; x < kMt; ++x) acc[x][n][c] *= fix, acc[x][n][c + 2] *= fix;
                         }
+                    exponents();
                 }
                 uint32_t pf[kParts][NT][2];  // P^T, keys along the operand's rows
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const float m0 = m[n][0] == -INFINITY ? 0.f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
-                    const float p0 = exp2_fast(s[n][0] - m0), p1 = exp2_fast(s[n][1] - m1);
-                    const float p2 = exp2_fast(s[n][2] - m0), p3 = exp2_fast(s[n][3] - m1);
+                    const float p0 = exp2_fast(z[n][0]), p1 = exp2_fast(z[n][1]);
+                    const float p2 = exp2_fast(z[n][2]), p3 = exp2_fast(z[n][3]);
                     l[n][0] = fmaf(p0 + p2, inv_vs, l[n][0]);
                     l[n][1] = fmaf(p1 + p3, inv_vs, l[n][1]);
                     const uint32_t a = h2_bits(p0, p1), c = h2_bits(p2, p3);
@@ -458,8 +569,7 @@ __global__ void __launch_bounds__(kStreamThreads, NT == 1 ? 2 : 1) paged_attenti
 #pragma unroll
                         for (int x = 0; x < kVBytes / 4; ++x) nan |= nan_bits(vr[i].w[x]);
                     if (__any_sync(0xffffffffu, nan != 0)) {
-                        if (lane < C::kRows && lane < n_rows)
-                            mark_nan(p, table, h, key, min(key + 16, visible(p, r, (row0 + lane) / group)), s_nan[lane]);
+                        if (lane < sg.n_rows) mark_nan(p, table, h, key, min(key + 16, s_lim[lane]), s_nan[lane]);
                         if (lane == 0) s_any_nan = 1;
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
@@ -487,12 +597,10 @@ __global__ void __launch_bounds__(kStreamThreads, NT == 1 ? 2 : 1) paged_attenti
                         }
                 }
             }
+            if (next) load_v(page_next, row_next);
             page = page_next;
-            if (more) {
-                if (page >= 0) load_v(page, row_next);
-                step_page(col_next, row_next);
-                page_next = key + 2 * kTileKeys < key_end ? page_at(col_next) : -1;
-            }
+            row_next = row;
+            if (key + 2 * kTileKeys < key_end) page_next = look_up();
         }
 
         // ---- join the warps
@@ -502,6 +610,7 @@ __global__ void __launch_bounds__(kStreamThreads, NT == 1 ? 2 : 1) paged_attenti
             for (int c = 0; c < 2; ++c) {
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], o);
+                if (m[n][c] == kNoMax) m[n][c] = -INFINITY;  // no key seen
                 if (g == 0) {
                     s_m[warp][n * 8 + 2 * t + c] = m[n][c];
                     s_l[warp][n * 8 + 2 * t + c] = l[n][c];
@@ -519,7 +628,7 @@ __global__ void __launch_bounds__(kStreamThreads, NT == 1 ? 2 : 1) paged_attenti
                 fix[n][c] = m[n][c] == -INFINITY ? 0.f : exp2_fast(m[n][c] - top);
             }
         // Where m is -inf nothing was added (acc is 0 and stays so); NaN passes.
-        float *mine = s_acc + (warp & (kStreamWarps / 2 - 1)) * (C::kRows * C::kRowPitch);
+        float *mine = s_acc + (warp % (kStreamWarps / 2)) * (C::kRows * C::kRowPitch);
 #pragma unroll
         for (int round = 0; round < 2; ++round) {
             if ((warp >= kStreamWarps / 2) == (round == 0)) {
@@ -542,9 +651,9 @@ __global__ void __launch_bounds__(kStreamThreads, NT == 1 ? 2 : 1) paged_attenti
             }
             __syncthreads();
         }
-        const bool whole = tile0 == 0 && tile1 == tiles;
-        const int slot = 2 * blockIdx.x + (tile0 == 0 ? 1 : 0);
-        for (int i = tid; i < n_rows * D; i += kStreamThreads) {
+        const bool whole = sg.tile0 == 0 && sg.tile1 == sg.tiles;
+        const int slot = 2 * blockIdx.x + (sg.tile0 == 0 ? 1 : 0);
+        for (int i = tid; i < sg.n_rows * D; i += kStreamThreads) {
             const int rw = i / D, d = i - rw * D;
             float top = -INFINITY;
 #pragma unroll
@@ -563,8 +672,8 @@ __global__ void __launch_bounds__(kStreamThreads, NT == 1 ? 2 : 1) paged_attenti
             if (s_any_nan && (s_nan[rw][d >> 5] >> (d & 31) & 1u)) x = NAN;
             const float lse2 = sum == 0.f ? -INFINITY : top + log2f(sum);
             if (whole) {
-                const int tok = (row0 + rw) / group, head = h * group + (row0 + rw) - tok * group;
-                const long long token = r.first + tok;
+                const int tok = (sg.row0 + rw) / group, head = sg.h * group + (sg.row0 + rw) - tok * group;
+                const long long token = sg.r.first + tok;
                 static_cast<T *>(p.o)[token * p.o_st[0] + head * p.o_st[1] + d] = Elem<T>::from_float(x);
                 if (p.lse && d == 0) p.lse[token * p.H + head] = lse2 * 0.6931471805599453f;
             } else {
@@ -572,20 +681,13 @@ __global__ void __launch_bounds__(kStreamThreads, NT == 1 ? 2 : 1) paged_attenti
                 if (d == 0) sa.part_lse[slot * C::kRows + rw] = lse2;
             }
         }
-        if (tile0 == 0 && !whole && tid == 0) {
-            // Begun here, ended by a later CTA: the one whose share holds the item's last tile.
-            const long long last = b_begin + static_cast<long long>(item + 1) * tiles - 1;
-            long long c1 = last * shares / total;  // within one of the owner
-            while (total * (c1 + 1) / shares <= last) ++c1;
-            while (total * c1 / shares > last) --c1;
-            sa.desc[blockIdx.x] = StreamDesc{b, item, static_cast<int>(c1) - static_cast<int>(blockIdx.x) + 1, 0};
-        }
+        if (tid == 0 && sg.tile0 == 0 && !whole)  // begun here, ended by a later CTA
+            sa.desc[blockIdx.x] = StreamDesc{sg.b, sg.item, sg.last_cta - static_cast<int>(blockIdx.x) + 1, 0};
         __syncthreads();  // the sums have been read
         if (s_any_nan) {
-            __syncthreads();
             for (int i = tid; i < C::kRows * (D / 32); i += kStreamThreads) s_nan[i / (D / 32)][i % (D / 32)] = 0;
-            if (tid == 0) s_any_nan = 0;
             __syncthreads();
+            if (tid == 0) s_any_nan = 0;
         }
     }
 }
@@ -602,7 +704,7 @@ __global__ void __launch_bounds__(D) paged_attention_join_kernel(const StreamArg
     if (desc.segments == 0) return;
     const AttnArgs &p = sa.a;
     const Request r = request_of(p, desc.b);
-    const int group = p.H / p.Hkv, n_rt = row_tiles<ROWS>(p, r);
+    const int group = p.H / p.Hkv, n_rt = (r.rows * group + ROWS - 1) / ROWS;
     const int h = desc.item / n_rt, row0 = (desc.item - h * n_rt) * ROWS;
     const int n_rows = min(ROWS, r.rows * group - row0);
     const int tid = threadIdx.x, n = desc.segments;

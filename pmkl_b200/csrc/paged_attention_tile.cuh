@@ -61,19 +61,6 @@ struct TileCfg {
     static constexpr uint32_t kTmemCols = 256, kColS = 0, kColP = 64, kColO = 128;
 };
 
-// One stretch of an item's key tiles.
-struct Segment {
-    Request r;
-    int b, h, item, row0, n_rows, tile0, tile1, tiles;
-    int lim_min, lim_max;  // keys that the first and last row see
-};
-
-// The share of a CTA in the list of items.
-struct Share {
-    long long total, shares, u, u_end, b_begin;
-    int b;
-};
-
 constexpr int kAhead = 4;
 
 struct TileShared {
@@ -83,7 +70,6 @@ struct TileShared {
     int abort_flag;
     Share share;
     Segment seg[2];
-    int last_cta[2];     // of a segment that a later CTA ends: which
     // Of four tiles' groups of 16 keys: where they begin (0: no page) in the keys
     // and the values; key scale, log2 of the value scale (-inf: no page).
     unsigned long long from[kAhead][2][8];
@@ -92,59 +78,7 @@ struct TileShared {
     int nan[2];          // the tile's values held NaN: tile number of the CTA + 1
     alignas(16) uint32_t nan_cols[kTileRows][4];  // columns of a row that are NaN (see above)
     long long sum[kTileThreads / 32];
-    long long at;
-    int b;
 };
-
-__device__ __forceinline__ int tile_count(const AttnArgs &p, const Request &r, int row0, int rows, int group) {
-    return max(1, (visible(p, r, (min(row0 + kTileRows, rows) - 1) / group) + 127) / 128);
-}
-
-// Key tiles of all row tiles of a request, for one K/V head.
-__device__ __forceinline__ long long head_tiles(const AttnArgs &p, const Request &r, int group) {
-    const int rows = r.rows * group;
-    long long n = 0;
-    for (int row0 = 0; row0 < rows; row0 += kTileRows) n += tile_count(p, r, row0, rows, group);
-    return n;
-}
-
-__device__ __forceinline__ bool next_segment(const AttnArgs &p, Share &w, Segment &s) {
-    const int group = p.H / p.Hkv;
-    while (w.u < w.u_end && w.b < p.batch) {
-        s.r = request_of(p, w.b);
-        const long long per_head = head_tiles(p, s.r, group), all = per_head * p.Hkv;
-        if (w.u >= w.b_begin + all) {
-            w.b_begin += all;
-            ++w.b;
-            continue;
-        }
-        const int rows = s.r.rows * group;
-        s.b = w.b;
-        s.h = static_cast<int>((w.u - w.b_begin) / per_head);
-        long long left = (w.u - w.b_begin) - s.h * per_head;
-        int rt = 0;
-        s.tiles = tile_count(p, s.r, 0, rows, group);
-        while (left >= s.tiles) {
-            left -= s.tiles;
-            ++rt;
-            s.tiles = tile_count(p, s.r, rt * kTileRows, rows, group);
-        }
-        s.row0 = rt * kTileRows;
-        s.n_rows = min(kTileRows, rows - s.row0);
-        s.item = s.h * ((rows + kTileRows - 1) / kTileRows) + rt;
-        s.tile0 = static_cast<int>(left);
-        s.tile1 = static_cast<int>(min(static_cast<long long>(s.tiles), left + (w.u_end - w.u)));
-        s.lim_min = visible(p, s.r, s.row0 / group);
-        s.lim_max = visible(p, s.r, (s.row0 + s.n_rows - 1) / group);
-        w.u += s.tile1 - s.tile0;
-        return true;
-    }
-    return false;
-}
-
-__device__ __noinline__ long long tile_weight(const AttnArgs &p, int b) {
-    return head_tiles(p, request_of(p, b), p.H / p.Hkv) * p.Hkv;
-}
 
 // tcgen05.wait::ld that the values pass through, so that no use of them is
 // moved before it.
@@ -239,54 +173,12 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
         tmem_alloc(&sh.tmem, C::kTmemCols);
         tmem_relinquish();
     }
-    const auto weight = [&](int b) -> long long {
-        return b < p.batch ? tile_weight(p, b) : 0;
-    };
-    const auto block_inclusive = [&](long long v) -> long long {
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long x = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= o) v += x;
-        }
-        __syncthreads();
-        if (lane == 31) sh.sum[warp] = v;
-        __syncthreads();
-        for (int w = 0; w < warp; ++w) v += sh.sum[w];
-        return v;
-    };
-    Share mine{};
-    {
-        const long long w0 = weight(tid);
-        long long part = w0;
-        for (int b = tid + kTileThreads; b < p.batch; b += kTileThreads) part += weight(b);
-        block_inclusive(part);
-        for (int w = 0; w < kTileThreads / 32; ++w) mine.total += sh.sum[w];
-        // As many shares as CTAs, or as tiles where those are fewer: none is empty.
-        mine.shares = min(mine.total, static_cast<long long>(gridDim.x));
-        const bool idle = blockIdx.x >= mine.shares;
-        mine.u = idle ? 0 : mine.total * blockIdx.x / mine.shares;
-        mine.u_end = idle ? 0 : mine.total * (blockIdx.x + 1) / mine.shares;
-        if (mine.u < mine.u_end) {
-            long long before = 0;
-            for (int b0 = 0; b0 < p.batch; b0 += kTileThreads) {
-                const long long w = b0 ? weight(b0 + tid) : w0;
-                const long long end = block_inclusive(w) + before;
-                if (mine.u >= end - w && mine.u < end) sh.b = b0 + tid, sh.at = end - w;
-                for (int x = 0; x < kTileThreads / 32; ++x) before += sh.sum[x];
-                if (before > mine.u) break;
-            }
-        }
-    }
+    find_share<kTileRows, 128, kTileThreads>(p, sh.sum, sh.share);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
     const bool skip = *abort_flag != 0;
-    if (tid == 9 * 32) {  // the walker's
-        sh.share = mine;
-        if (mine.u < mine.u_end) sh.share.b = sh.b, sh.share.b_begin = sh.at;
-    }
-
     if (warp >= 8) {
         // ------------------------------------------------------------ products
         set_regs<kTileIssueRegs>();
@@ -297,18 +189,8 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                 const int i = seg & 1;
                 if (seg >= 2 && !mbar_wait(&sh.seg_empty[i], ((seg >> 1) - 1) & 1, abort_flag)) break;
                 Segment &s = sh.seg[i];
-                more = next_segment(p, sh.share, s);
-                if (!more) {
-                    s.tile0 = s.tile1 = 0;
-                } else if (s.tile1 < s.tiles) {
-                    // The CTA whose share holds the item's last tile.
-                    const long long last = sh.share.u + (s.tiles - s.tile1) - 1;
-                    const long long total = sh.share.total, shares = sh.share.shares;
-                    long long c1 = last * shares / total;  // within one of the owner
-                    while (total * (c1 + 1) / shares <= last) ++c1;
-                    while (total * c1 / shares > last) --c1;
-                    sh.last_cta[i] = static_cast<int>(c1);
-                }
+                more = next_segment<kTileRows, 128>(p, sh.share, s);
+                if (!more) s.tile0 = s.tile1 = 0;
                 mbar_arrive(&sh.seg_full[i]);
             }
         }
@@ -671,7 +553,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                 if (real && !whole) sa.part_lse[slot * kTileRows + tid] = lse2;
                 // Begun here, ended by a later CTA.
                 if (tid == 0 && tile0 == 0 && !whole)
-                    sa.desc[blockIdx.x] = StreamDesc{s.b, s.item, sh.last_cta[seg & 1] - static_cast<int>(blockIdx.x) + 1, 0};
+                    sa.desc[blockIdx.x] = StreamDesc{s.b, s.item, s.last_cta - static_cast<int>(blockIdx.x) + 1, 0};
                 tc_fence_before();
             }
             __syncwarp();

@@ -119,8 +119,9 @@ bool stream_applies(const paged::AttnArgs &p) {
         if (!aligned16(c->base)) return false;
         for (long long s : c->s)
             if (s % 16 != 0) return false;
+        if (c->s[0] > 0x7FFFFFFF || c->s[2] > 0x7FFFFFFF / 16) return false;
     }
-    return true;
+    return static_cast<long long>(p.num_blocks) * p.Hkv <= 0x7FFFFFFF;
 }
 
 // Grid of a kernel that shares out `items` of at most `tiles` tiles each over
@@ -138,6 +139,10 @@ paged::StreamArgs shared_args(const paged::AttnArgs &a, void *workspace, int cta
     constexpr long long kVec = 16 / sizeof(T);
     p.vec_q = aligned16(a.q) && a.q_st[0] % kVec == 0 && a.q_st[1] % kVec == 0;
     p.vec_o = aligned16(a.o) && a.o_st[0] % kVec == 0 && a.o_st[1] % kVec == 0;
+    p.k_page = static_cast<int>(a.k.s[0]);
+    p.k_row = static_cast<int>(a.k.s[2]);
+    p.v_page = static_cast<int>(a.v.s[0]);
+    p.v_row = static_cast<int>(a.v.s[2]);
     uint8_t *ws = static_cast<uint8_t *>(workspace);
     p.desc = reinterpret_cast<paged::StreamDesc *>(ws);
     p.part_lse = reinterpret_cast<float *>(ws + ctas * sizeof(paged::StreamDesc));
@@ -191,15 +196,15 @@ int launch_stream(const paged::AttnArgs &a, void *workspace, cudaStream_t stream
     using C = paged::StreamCfg<D, NT>;
     static Occupancy occupancy;
     auto kernel = paged::paged_attention_stream_kernel<T, D, NT>;
-    const int per_sm = occupancy.get(kernel, paged::kStreamThreads, C::kSmemBytes);
+    const int per_sm = occupancy.get(kernel, C::kThreads, C::kSmemBytes);
     if (per_sm < 1) return PMKL_ERR_LAUNCH;
     const paged::StreamArgs p = shared_args<T>(a, workspace, paged::kMaxStreamCtas, C::kRows);
     const long long tiles = std::max<long long>(
-        1, (static_cast<long long>(a.max_blocks) * a.block + paged::kTileKeys - 1) / paged::kTileKeys);
+        1, (static_cast<long long>(a.max_blocks) * a.block + C::kTileKeys - 1) / C::kTileKeys);
     const long long row_tiles = (static_cast<long long>(a.H / a.Hkv) * a.max_q + C::kRows - 1) / C::kRows;
     const long long grid = share_grid(static_cast<long long>(sm_count()) * per_sm, paged::kMaxStreamCtas,
                                       static_cast<long long>(a.batch) * a.Hkv * row_tiles, tiles);
-    kernel<<<static_cast<unsigned>(grid), paged::kStreamThreads, C::kSmemBytes, stream>>>(p);
+    kernel<<<static_cast<unsigned>(grid), C::kThreads, C::kSmemBytes, stream>>>(p);
     const int rc = launch_status();
     if (rc != PMKL_OK || tiles == 1) return rc;  // an item of one tile lies in one CTA
     return launch_join<T, D, C::kRows>(p, grid, stream);

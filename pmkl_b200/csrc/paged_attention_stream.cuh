@@ -147,7 +147,7 @@ struct StreamCfg {
     static constexpr int kWarps = NT == 2 ? 12 : 8;
     static constexpr int kThreads = 32 * kWarps;
     static constexpr int kTileKeys = 16 * kWarps;  // keys a CTA takes at a time
-    static constexpr bool kQShared = NT == 4;      // query operands in shared memory, not in registers
+    static constexpr bool kQShared = NT == 4 || D == 128;  // query operands in shared memory, not in registers
     static constexpr int kRowPitch = D + 32;  // 4 floats behind every D / 8: a warp's float4 stores meet no bank twice
     static constexpr int kAccBytes = (kWarps / 2) * kRows * kRowPitch * 4;
     // (operands of two fp16 parts: 8 bytes a lane, step and row tile)

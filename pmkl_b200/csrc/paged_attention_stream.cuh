@@ -147,11 +147,10 @@ struct StreamCfg {
     static constexpr int kWarps = NT == 2 ? 12 : 8;
     static constexpr int kThreads = 32 * kWarps;
     static constexpr int kTileKeys = 16 * kWarps;  // keys a CTA takes at a time
-    static constexpr bool kQShared = NT == 4 || D == 128;  // query operands in shared memory, not in registers
     static constexpr int kRowPitch = D + 32;  // 4 floats behind every D / 8: a warp's float4 stores meet no bank twice
-    static constexpr int kAccBytes = (kWarps / 2) * kRows * kRowPitch * 4;
-    // (operands of two fp16 parts: 8 bytes a lane, step and row tile)
-    static constexpr int kSmemBytes = kAccBytes + (kQShared ? 2 * NT * (D / 16) * 32 * 8 : 0);
+    // The warps' sums; the query operands, 8 bytes a lane and step, for two fp16 parts.
+    static constexpr int kAccBytes = kWarps * kRows * kRowPitch * 4;
+    static constexpr int kSmemBytes = kAccBytes + 2 * NT * (D / 16) * 32 * 8;
 };
 
 __host__ __device__ constexpr size_t partial_workspace(int ctas, int rows, int D) {
@@ -175,6 +174,16 @@ struct Share {
     long long total, shares, u, u_end, b_begin;
     int b;
 };
+
+// Where share c of `shares` begins in `total` tiles.  32-bit division where it
+// does: the 64-bit one is a long routine.
+__device__ __forceinline__ long long share_begin(long long total, long long c, long long shares) {
+    const unsigned long long n = static_cast<unsigned long long>(total) * c;
+    return (n >> 32) == 0 ? static_cast<unsigned>(n) / static_cast<unsigned>(shares) : n / shares;
+}
+__device__ __forceinline__ int quotient(long long a, long long b) {  // a, b >= 0, the result an int
+    return ((a | b) >> 32) == 0 ? static_cast<unsigned>(a) / static_cast<unsigned>(b) : static_cast<int>(a / b);
+}
 
 template <int ROWS, int KEYS>
 __device__ __forceinline__ int tile_count(const AttnArgs &p, const Request &r, int row0, int rows, int group) {
@@ -211,7 +220,7 @@ __device__ __forceinline__ bool next_segment(const AttnArgs &p, Share &w, Segmen
         }
         const int rows = s.r.rows * group;
         s.b = w.b;
-        s.h = static_cast<int>((w.u - w.b_begin) / per_head);
+        s.h = quotient(w.u - w.b_begin, per_head);
         long long left = (w.u - w.b_begin) - s.h * per_head;
         int rt = 0;
         s.tiles = tile_count<ROWS, KEYS>(p, s.r, 0, rows, group);
@@ -232,9 +241,9 @@ __device__ __forceinline__ bool next_segment(const AttnArgs &p, Share &w, Segmen
         if (s.tile1 < s.tiles) {
             // The CTA whose share holds the item's last tile.
             const long long last = w.u + (s.tiles - s.tile1) - 1;
-            long long c = last * w.shares / w.total;  // within one of the owner
-            while (w.total * (c + 1) / w.shares <= last) ++c;
-            while (w.total * c / w.shares > last) --c;
+            long long c = share_begin(w.shares, last, w.total);  // within one of the owner
+            while (share_begin(w.total, c + 1, w.shares) <= last) ++c;
+            while (share_begin(w.total, c, w.shares) > last) --c;
             s.last_cta = static_cast<int>(c);
         }
         return true;
@@ -262,30 +271,32 @@ __device__ __forceinline__ void find_share(const AttnArgs &p, long long (&sum)[T
         for (int w = 0; w < warp; ++w) v += sum[w];
         return v;
     };
-    long long part = 0, w0 = 0, total = 0;
+    const bool one = p.batch <= THREADS;  // a request a thread: one sum does
+    long long part = 0, total = 0;
 #pragma unroll 1
-    for (int b = tid; b < p.batch; b += THREADS) {
-        const long long w = weight(b);
-        if (b == tid) w0 = w;
-        part += w;
-    }
-    inclusive(part);
+    for (int b = tid; b < p.batch; b += THREADS) part += weight(b);
+    const long long upto = inclusive(part);
+#pragma unroll
     for (int w = 0; w < THREADS / 32; ++w) total += sum[w];
     // As many shares as CTAs, or as tiles where those are fewer: none is empty.
     const long long shares = min(total, static_cast<long long>(gridDim.x));
     const bool idle = blockIdx.x >= shares;
-    const long long u = idle ? 0 : total * blockIdx.x / shares, u_end = idle ? 0 : total * (blockIdx.x + 1) / shares;
+    const long long u = idle ? 0 : share_begin(total, blockIdx.x, shares);
     if (tid == 0) {
         to.total = total;
         to.shares = shares;
         to.u = u;
-        to.u_end = u_end;
+        to.u_end = idle ? 0 : share_begin(total, blockIdx.x + 1, shares);
     }
     if (idle) return;
+    if (one) {
+        if (u >= upto - part && u < upto) to.b = tid, to.b_begin = upto - part;
+        return;
+    }
     long long before = 0;
 #pragma unroll 1
     for (int b0 = 0; b0 < p.batch && before <= u; b0 += THREADS) {
-        const long long w = b0 ? weight(b0 + tid) : w0;
+        const long long w = weight(b0 + tid);
         const long long end = inclusive(w) + before;
         if (u >= end - w && u < end) to.b = b0 + tid, to.b_begin = end - w;
         for (int x = 0; x < THREADS / 32; ++x) before += sum[x];
@@ -320,148 +331,155 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
     constexpr int kHalves = D / 64;  // 16-byte loads of a key row
     constexpr int kMt = D / 16;      // 16-row tiles of O^T
     constexpr int kVBytes = D / 8;   // bytes of a V row a thread
-    extern __shared__ float s_acc[];
+    extern __shared__ __align__(16) float s_acc[];
     __shared__ float s_m[kStreamWarps][C::kRows], s_l[kStreamWarps][C::kRows];
-    __shared__ int s_lim[C::kRows];  // keys that a row sees
+    __shared__ alignas(8) int s_lim[C::kRows];  // keys that a row sees
     __shared__ uint32_t s_nan[C::kRows][D / 32];  // columns of a row that are NaN, where s_any_nan
     __shared__ int s_any_nan;
     __shared__ long long s_sum[kStreamWarps];
     __shared__ Share s_share;
-    __shared__ Segment s_seg;
-    __shared__ bool s_more;
+    __shared__ Segment s_segs[2];
+    __shared__ bool s_more[2];
+    __shared__ float s_qscale[C::kRows];  // raw product of a row to log2 units
     const AttnArgs &p = sa.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int group = p.H / p.Hkv;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     clear_tail<T>(p);
 
+    uint2 *const s_q = reinterpret_cast<uint2 *>(s_acc + C::kAccBytes / 4) + lane;  // [part][n][step][lane]
+
     if (tid == 0) sa.desc[blockIdx.x].segments = 0, s_any_nan = 0;
     for (int i = tid; i < C::kRows * (D / 32); i += kStreamThreads) s_nan[i / (D / 32)][i % (D / 32)] = 0;
     find_share<C::kRows, kTileKeys, kStreamThreads>(p, s_sum, s_share);
-    for (;;) {
-        // One thread walks: the loops over keys need the registers.
-        __syncthreads();
-        if (tid == 0) s_more = next_segment<C::kRows, kTileKeys>(p, s_share, s_seg);
-        __syncthreads();
-        if (!s_more) break;
-        const Segment &sg = s_seg;
+    __syncthreads();
+    if (tid == 0) s_more[0] = next_segment<C::kRows, kTileKeys>(p, s_share, s_segs[0]);
+    __syncthreads();
 
-        // ---- queries, as operands of S^T
-        uint32_t qf[kParts][NT][kSteps][2];
-        uint2 *const s_q = reinterpret_cast<uint2 *>(s_acc + C::kAccBytes / 4) + lane;  // [part][n][step][lane]
-        float q_scale[NT][2];  // of the columns 2t, 2t + 1: raw product to log2 units
+    // ---- this warp's keys: 16 of every tile, one tile ahead in registers.
+    // Column of the table and row in the page of the next ones, advanced without a division.
+    const int *table = nullptr;
+    int key = 0, key_end = 0, col = 0, row = 0, page = -1, page_next = -1, row_next = 0;
+    const uint8_t *k_mine = nullptr, *v_mine = nullptr;
+    float ks = 0.f, vs = 1.f;
+    int scale_at = 0;
+    Bytes<16> kr[2][kHalves];
+    Bytes<kVBytes> vr[4];
+    const int d_col = kTileKeys / p.block, d_row = kTileKeys - d_col * p.block;
+    // (strides of the cache are below 2^31 bytes here, offsets 64-bit)
+    const auto load_k = [&](int pg, int rw) {
+        const uint8_t *at = k_mine + static_cast<long long>(pg) * sa.k_page + static_cast<long long>(rw) * sa.k_row;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int row = sg.row0 + n * 8 + g;
-            const bool real = n * 8 + g < sg.n_rows;
-            const int i = row / group;
-            const T *q = static_cast<const T *>(p.q) + (sg.r.first + (real ? i : 0)) * p.q_st[0] +
-                         (sg.h * group + (real ? row - i * group : 0)) * p.q_st[1];
-            float x[kHalves][16];
-            float amax = 0.f;
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int hf = 0; hf < kHalves; ++hf) {
-                load_q16(x[hf], q + hf * 64 + t * 16, sa.vec_q != 0);
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    if (!real) x[hf][j] = 0.f;
-                    amax = fmaxf(amax, fabsf(x[hf][j]));
-                }
+            for (int hf = 0; hf < kHalves; ++hf) load_bytes(kr[i][hf], at + i * 8LL * sa.k_row + hf * 64);
+    };
+    const auto load_v = [&](int pg, int rw) {
+        const uint8_t *at = v_mine + static_cast<long long>(pg) * sa.v_page + static_cast<long long>(rw) * sa.v_row;
+        load_bytes(vr[0], at);
+        load_bytes(vr[1], at + sa.v_row);
+        load_bytes(vr[2], at + 8LL * sa.v_row);
+        load_bytes(vr[3], at + 9LL * sa.v_row);
+    };
+    const auto load_scales = [&](int pg) {
+        const int at = pg * p.Hkv + scale_at;  // (pages times heads fit 31 bits)
+        ks = __ldg(p.k.scale + at);
+        vs = __ldg(p.v.scale + at);
+    };
+    const auto look_up = [&]() -> int {  // the table's entry at `col`, then a step on
+        const int x = __ldg(table + col);
+        col += d_col;
+        row += d_row;
+        if (row >= p.block) row -= p.block, ++col;
+        return x;
+    };
+    const auto valid = [&](int x) { return static_cast<unsigned>(x) < static_cast<unsigned>(p.num_blocks); };
+    const auto begin = [&](const Segment &sg) {  // the first loads of a segment
+        table = p.table + sg.b * p.table_stride;
+        scale_at = sg.h;
+        key = sg.tile0 * kTileKeys + warp * 16;
+        key_end = min(sg.tile1 * kTileKeys, sg.lim_max);
+        col = key / p.block;
+        row = key - col * p.block;
+        k_mine = p.k.base + sg.h * p.k.s[1] + g * p.k.s[2] + t * 16;
+        v_mine = p.v.base + sg.h * p.v.s[1] + 2 * t * p.v.s[2] + g * kVBytes;
+        page = page_next = -1;
+        if (key < key_end) {
+            const int rw = row;
+            page = look_up();
+            row_next = row;
+            if (key + kTileKeys < key_end) page_next = look_up();
+            if (valid(page)) {
+                load_k(page, rw);
+                load_scales(page);
+                load_v(page, rw);
             }
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            // The power of two that brings the row's largest value to 2^7 .. 2^8.
-            const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127 - 7, -100), 126);
-            const float down = exp2_int(-e);
+        }
+    };
+
+    if (s_more[0]) begin(s_segs[0]);
+    for (int turn = 0; s_more[turn]; turn ^= 1) {
+        const Segment &sg = s_segs[turn];
+        // ---- the last warp walks on, the first lays the queries out as operands of S^T
+        if (tid == kStreamThreads - 32) s_more[turn ^ 1] = next_segment<C::kRows, kTileKeys>(p, s_share, s_segs[turn ^ 1]);
+        if (warp == 0) {
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s)
+            for (int n = 0; n < NT; ++n) {
+                const int rw = sg.row0 + n * 8 + g;
+                const bool real = n * 8 + g < sg.n_rows;
+                const int i = rw / group;
+                const T *q = static_cast<const T *>(p.q) + (sg.r.first + (real ? i : 0)) * p.q_st[0] +
+                             (sg.h * group + (real ? rw - i * group : 0)) * p.q_st[1];
+                float x[kHalves][16];
+                float amax = 0.f;
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int at = (s & 3) * 4 + j * 2;
-                    const float a = x[s >> 2][at] * down, c = x[s >> 2][at + 1] * down;
-                    qf[0][n][s][j] = h2_bits(a, c);
-                    if constexpr (kSplit) {
-                        const float2 hi = h2_floats(qf[0][n][s][j]);
-                        qf[kParts - 1][n][s][j] = h2_bits(a - hi.x, c - hi.y);
+                for (int hf = 0; hf < kHalves; ++hf) {
+                    load_q16(x[hf], q + hf * 64 + t * 16, sa.vec_q != 0);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        if (!real) x[hf][j] = 0.f;
+                        amax = fmaxf(amax, fabsf(x[hf][j]));
                     }
                 }
-            if (C::kQShared && warp == 0) {
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                // The power of two that brings the row's largest value to 2^7 .. 2^8.
+                const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127 - 7, -100), 126);
+                const float down = exp2_int(-e);
 #pragma unroll
-                for (int part = 0; part < kParts; ++part)
-#pragma unroll
-                    for (int s = 0; s < kSteps; ++s)
-                        s_q[((part * NT + n) * kSteps + s) * 32] = make_uint2(qf[part][n][s][0], qf[part][n][s][1]);
+                for (int s = 0; s < kSteps; ++s) {
+                    uint2 hi, lo;
+                    const float *y = &x[s >> 2][(s & 3) * 4];
+                    hi.x = h2_bits(y[0] * down, y[1] * down);
+                    hi.y = h2_bits(y[2] * down, y[3] * down);
+                    s_q[(n * kSteps + s) * 32] = hi;
+                    if constexpr (kSplit) {
+                        const float2 h0 = h2_floats(hi.x), h1 = h2_floats(hi.y);
+                        lo.x = h2_bits(y[0] * down - h0.x, y[1] * down - h0.y);
+                        lo.y = h2_bits(y[2] * down - h1.x, y[3] * down - h1.y);
+                        s_q[((NT + n) * kSteps + s) * 32] = lo;
+                    }
+                }
+                if (t == 0) {
+                    s_qscale[n * 8 + g] = exp2_int(e) * p.scale * 1.4426950408889634f;
+                    s_lim[n * 8 + g] = real ? visible(p, sg.r, i) : sg.r.keys;
+                }
             }
-            const float up = exp2_int(e) * p.scale * 1.4426950408889634f;
-            q_scale[n][0] = __shfl_sync(0xffffffffu, up, 8 * t);
-            q_scale[n][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4);
-            if (warp == 0 && t == 0) s_lim[n * 8 + g] = real ? visible(p, sg.r, i) : sg.r.keys;
         }
         __syncthreads();
-        const int lim_min = sg.lim_min, lim_max = sg.lim_max, h = sg.h;
-
-        // ---- this warp's keys: 16 of every tile
+        float q_scale[NT][2];  // of the columns 2t, 2t + 1
         float acc[kMt][NT][4];
         float m[NT][2], l[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
+            q_scale[n][0] = s_qscale[n * 8 + 2 * t];
+            q_scale[n][1] = s_qscale[n * 8 + 2 * t + 1];
             m[n][0] = m[n][1] = kNoMax;
             l[n][0] = l[n][1] = 0.f;
 #pragma unroll
             for (int x = 0; x < kMt; ++x) acc[x][n][0] = acc[x][n][1] = acc[x][n][2] = acc[x][n][3] = 0.f;
         }
-        const int *const table = p.table + sg.b * p.table_stride;
-        const int key_end = min(sg.tile1 * kTileKeys, lim_max);
-        int key = sg.tile0 * kTileKeys + warp * 16;
-        // Column of the table and row in the page of the next 16 keys, advanced
-        // without a division.
-        int col = key / p.block, row = key - col * p.block;
-        const int d_col = kTileKeys / p.block, d_row = kTileKeys - d_col * p.block;
-        const uint8_t *const k_mine = p.k.base + h * p.k.s[1] + g * p.k.s[2] + t * 16;
-        const uint8_t *const v_mine = p.v.base + h * p.v.s[1] + 2 * t * p.v.s[2] + g * kVBytes;
-        Bytes<16> kr[2][kHalves];
-        Bytes<kVBytes> vr[4];
-        // (strides of the cache are below 2^31 bytes here, offsets 64-bit)
-        const auto load_k = [&](int page, int rw) {
-            const uint8_t *at = k_mine + static_cast<long long>(page) * sa.k_page + static_cast<long long>(rw) * sa.k_row;
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int hf = 0; hf < kHalves; ++hf) load_bytes(kr[i][hf], at + i * 8LL * sa.k_row + hf * 64);
-        };
-        const auto load_v = [&](int page, int rw) {
-            const uint8_t *at = v_mine + static_cast<long long>(page) * sa.v_page + static_cast<long long>(rw) * sa.v_row;
-            load_bytes(vr[0], at);
-            load_bytes(vr[1], at + sa.v_row);
-            load_bytes(vr[2], at + 8LL * sa.v_row);
-            load_bytes(vr[3], at + 9LL * sa.v_row);
-        };
-        float ks = 0.f, vs = 1.f;
-        const auto load_scales = [&](int pg) {
-            const int at = pg * p.Hkv + h;  // (below 2^31: the cache's extent allows no more pages)
-            ks = __ldg(p.k.scale + at);
-            vs = __ldg(p.v.scale + at);
-        };
-        const auto look_up = [&]() -> int {  // the table's entry at `col`, then a step on
-            const int x = __ldg(table + col);
-            col += d_col;
-            row += d_row;
-            if (row >= p.block) row -= p.block, ++col;
-            return x;
-        };
-        const auto valid = [&](int x) { return static_cast<unsigned>(x) < static_cast<unsigned>(p.num_blocks); };
-        int page = -1, page_next = -1, row_next = 0;
-        if (key < key_end) {
-            const int rw = row;
-            page = look_up();
-            if (valid(page)) {
-                load_scales(page);
-                load_k(page, rw);
-                load_v(page, rw);
-            }
-            row_next = row;
-            if (key + kTileKeys < key_end) page_next = look_up();
-        }
+        const int lim_min = sg.lim_min, lim_max = sg.lim_max;
         for (; key < key_end; key += kTileKeys) {
             const bool there = valid(page);
             const bool more = key + kTileKeys < key_end, next = more && valid(page_next);
@@ -480,8 +498,7 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int part = 0; part < kParts; ++part) {
-                            const uint2 q2 = C::kQShared ? s_q[((part * NT + n) * kSteps + x) * 32]
-                                                         : make_uint2(qf[part][n][x][0], qf[part][n][x][1]);
+                            const uint2 q2 = s_q[((part * NT + n) * kSteps + x) * 32];
                             mma16816(s[n], a0, a1, a2, a3, q2.x, q2.y);
                         }
                 }
@@ -569,7 +586,7 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
 #pragma unroll
                         for (int x = 0; x < kVBytes / 4; ++x) nan |= nan_bits(vr[i].w[x]);
                     if (__any_sync(0xffffffffu, nan != 0)) {
-                        if (lane < sg.n_rows) mark_nan(p, table, h, key, min(key + 16, s_lim[lane]), s_nan[lane]);
+                        if (lane < sg.n_rows) mark_nan(p, table, sg.h, key, min(key + 16, s_lim[lane]), s_nan[lane]);
                         if (lane == 0) s_any_nan = 1;
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
@@ -603,71 +620,44 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
             if (key + 2 * kTileKeys < key_end) page_next = look_up();
         }
 
-        // ---- join the warps
+        // ---- the next segment's first loads, then the warps join
+        if (s_more[turn ^ 1]) begin(s_segs[turn ^ 1]);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
+                const int rw = n * 8 + 2 * t + c;
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], o);
-                if (m[n][c] == kNoMax) m[n][c] = -INFINITY;  // no key seen
                 if (g == 0) {
-                    s_m[warp][n * 8 + 2 * t + c] = m[n][c];
-                    s_l[warp][n * 8 + 2 * t + c] = l[n][c];
+                    s_m[warp][rw] = m[n][c];
+                    s_l[warp][rw] = l[n][c];
+                }
+                if (rw < sg.n_rows) {
+                    float4 *at = reinterpret_cast<float4 *>(s_acc + (warp * C::kRows + rw) * C::kRowPitch + g * (D / 8 + 4));
+#pragma unroll
+                    for (int x = 0; x < kMt / 2; ++x)
+                        at[x] = make_float4(acc[2 * x][n][c], acc[2 * x][n][c + 2], acc[2 * x + 1][n][c],
+                                            acc[2 * x + 1][n][c + 2]);
                 }
             }
         __syncthreads();
-        float fix[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                float top = -INFINITY;
-#pragma unroll
-                for (int w = 0; w < kStreamWarps; ++w) top = fmaxf(top, s_m[w][n * 8 + 2 * t + c]);
-                fix[n][c] = m[n][c] == -INFINITY ? 0.f : exp2_fast(m[n][c] - top);
-            }
-        // Where m is -inf nothing was added (acc is 0 and stays so); NaN passes.
-        float *mine = s_acc + (warp % (kStreamWarps / 2)) * (C::kRows * C::kRowPitch);
-#pragma unroll
-        for (int round = 0; round < 2; ++round) {
-            if ((warp >= kStreamWarps / 2) == (round == 0)) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        float4 *at = reinterpret_cast<float4 *>(mine + (n * 8 + 2 * t + c) * C::kRowPitch + g * (D / 8 + 4));
-#pragma unroll
-                        for (int x = 0; x < kMt / 2; ++x) {
-                            float4 v = make_float4(acc[2 * x][n][c] * fix[n][c], acc[2 * x][n][c + 2] * fix[n][c],
-                                                   acc[2 * x + 1][n][c] * fix[n][c], acc[2 * x + 1][n][c + 2] * fix[n][c]);
-                            if (round == 1) {
-                                const float4 o = at[x];
-                                v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
-                            }
-                            at[x] = v;
-                        }
-                    }
-            }
-            __syncthreads();
-        }
         const bool whole = sg.tile0 == 0 && sg.tile1 == sg.tiles;
         const int slot = 2 * blockIdx.x + (sg.tile0 == 0 ? 1 : 0);
         for (int i = tid; i < sg.n_rows * D; i += kStreamThreads) {
             const int rw = i / D, d = i - rw * D;
-            float top = -INFINITY;
+            const float *from = s_acc + rw * C::kRowPitch + d + d / (D / 8) * 4;
+            float top = s_m[0][rw];
 #pragma unroll
-            for (int w = 0; w < kStreamWarps; ++w) top = fmaxf(top, s_m[w][rw]);
-            float sum = 0.f;
+            for (int w = 1; w < kStreamWarps; ++w) top = fmaxf(top, s_m[w][rw]);
+            // (a warp that saw no key adds nothing: its l and sums are 0)
+            float sum = 0.f, x = 0.f;
 #pragma unroll
             for (int w = 0; w < kStreamWarps; ++w) {
-                const float mw = s_m[w][rw];
-                sum += mw == -INFINITY ? s_l[w][rw] : exp2_fast(mw - top) * s_l[w][rw];
+                const float fix = exp2_fast(s_m[w][rw] - top);
+                sum = fmaf(fix, s_l[w][rw], sum);
+                x = fmaf(fix, from[w * C::kRows * C::kRowPitch], x);
             }
-            float x = 0.f;
-            const float *from = s_acc + rw * C::kRowPitch + d + d / (D / 8) * 4;
-#pragma unroll
-            for (int w = 0; w < kStreamWarps / 2; ++w) x += from[w * C::kRows * C::kRowPitch];
             x *= sum == 0.f ? 0.f : 1.f / sum;
             if (s_any_nan && (s_nan[rw][d >> 5] >> (d & 31) & 1u)) x = NAN;
             const float lse2 = sum == 0.f ? -INFINITY : top + log2f(sum);
@@ -683,12 +673,13 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
         }
         if (tid == 0 && sg.tile0 == 0 && !whole)  // begun here, ended by a later CTA
             sa.desc[blockIdx.x] = StreamDesc{sg.b, sg.item, sg.last_cta - static_cast<int>(blockIdx.x) + 1, 0};
-        __syncthreads();  // the sums have been read
         if (s_any_nan) {
+            __syncthreads();
             for (int i = tid; i < C::kRows * (D / 32); i += kStreamThreads) s_nan[i / (D / 32)][i % (D / 32)] = 0;
             __syncthreads();
             if (tid == 0) s_any_nan = 0;
         }
+        __syncthreads();  // the queries, sums and segment may be written over
     }
 }
 

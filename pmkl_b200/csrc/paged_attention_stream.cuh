@@ -467,19 +467,20 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
             }
         }
         __syncthreads();
-        float q_scale[NT][2];  // of the columns 2t, 2t + 1
         float acc[kMt][NT][4];
         float m[NT][2], l[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            q_scale[n][0] = s_qscale[n * 8 + 2 * t];
-            q_scale[n][1] = s_qscale[n * 8 + 2 * t + 1];
             m[n][0] = m[n][1] = kNoMax;
             l[n][0] = l[n][1] = 0.f;
 #pragma unroll
             for (int x = 0; x < kMt; ++x) acc[x][n][0] = acc[x][n][1] = acc[x][n][2] = acc[x][n][3] = 0.f;
         }
-        const int lim_min = sg.lim_min, lim_max = sg.lim_max;
+        // (read in the loop, from shared memory: the registers are for the data)
+        const volatile int &lim_min = sg.lim_min, &lim_max = sg.lim_max;
+        const auto q_scale = [&](int n, int c) -> float {  // of column 2t + c
+            return *static_cast<const volatile float *>(&s_qscale[n * 8 + 2 * t + c]);
+        };
         for (; key < key_end; key += kTileKeys) {
             const bool there = valid(page);
             const bool more = key + kTileKeys < key_end, next = more && valid(page_next);
@@ -527,7 +528,7 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
                 const auto exponents = [&]() {
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        const float f0 = q_scale[n][0] * ks_now, f1 = q_scale[n][1] * ks_now;
+                        const float f0 = q_scale(n, 0) * ks_now, f1 = q_scale(n, 1) * ks_now;
                         const float o0 = lv - m[n][0], o1 = lv - m[n][1];
                         z[n][0] = fmaf(s[n][0], f0, o0);
                         z[n][1] = fmaf(s[n][1], f1, o1);
@@ -544,7 +545,7 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            float top = fmaf(fmaxf(s[n][c], s[n][c + 2]), q_scale[n][c] * ks_now, lv);
+                            float top = fmaf(fmaxf(s[n][c], s[n][c + 2]), q_scale(n, c) * ks_now, lv);
 #pragma unroll
                             for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                             top = fmaxf(top, m[n][c]);

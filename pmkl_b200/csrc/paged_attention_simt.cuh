@@ -33,7 +33,7 @@ struct Request {
     int shift;              // row i sees keys j <= i + shift
 };
 
-__device__ __forceinline__ Request request_of(const AttnArgs &p, int b) {
+__host__ __device__ __forceinline__ Request request_of(const AttnArgs &p, int b) {
     Request r;
     int begin = b, end = b + 1;
     if (p.query_starts) {
@@ -51,7 +51,7 @@ __device__ __forceinline__ Request request_of(const AttnArgs &p, int b) {
 }
 
 // Keys that row i of the request sees.
-__device__ __forceinline__ int visible(const AttnArgs &p, const Request &r, int i) {
+__host__ __device__ __forceinline__ int visible(const AttnArgs &p, const Request &r, int i) {
     return p.causal ? min(r.keys, max(0, i + r.shift + 1)) : r.keys;
 }
 

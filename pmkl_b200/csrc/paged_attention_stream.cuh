@@ -50,12 +50,15 @@ constexpr int kMaxStreamCtas = 640;           // partials in the workspace: 148 
 // partial rows [2 CTAs][rows][D].  A CTA's slot 2c holds the item that it
 // enters in the middle, 2c + 1 the item that it begins and does not end.
 struct StreamDesc {
-    int b, item, segments, pad;
+    int segments;  // CTAs that the item is spread over; 0: none
+    int first, h, row0, n_rows;
+    int pad[3];
 };
 
 struct StreamArgs {
     AttnArgs a;
     int vec_q, vec_o;  // rows of q, of o are 16-byte aligned
+    int d_col, d_row;  // keys of a tile as pages and rows of one
     int k_page, k_row, v_page, v_row;  // bytes from page to page and row to row of the cache, where 31 bits hold them
     float *part_o, *part_lse;
     StreamDesc *desc;
@@ -147,6 +150,7 @@ struct StreamCfg {
     static constexpr int kWarps = NT == 2 ? 12 : 8;
     static constexpr int kThreads = 32 * kWarps;
     static constexpr int kTileKeys = 16 * kWarps;  // keys a CTA takes at a time
+    static constexpr int kItemCost = 3;            // of an item, in tiles: some 8000 cycles against 2450 (16 x 4096 keys)
     static constexpr int kRowPitch = D + 32;  // 4 floats behind every D / 8: a warp's float4 stores meet no bank twice
     // The warps' sums; the query operands, 8 bytes a lane and step, for two fp16 parts.
     static constexpr int kAccBytes = kWarps * kRows * kRowPitch * 4;
@@ -159,104 +163,133 @@ __host__ __device__ constexpr size_t partial_workspace(int ctas, int rows, int D
 
 // The work of both kernels that share it out: items are (request, K/V head,
 // ROWS rows), in that order, each cut in tiles of KEYS keys up to the last key
-// that its rows see, at least one, so that every item has a writer.
+// that its rows see, at least one, so that every item has a writer.  The list
+// counts an item as its tiles and COST more, the tiles' worth of what a CTA
+// does once for an item (queries, first loads, join, output): shares of many
+// short items then take no longer than shares of one long.  The COST comes
+// first: a share that begins or ends in it begins or ends at tile 0.
 
 // One stretch of an item's key tiles.
 struct Segment {
     Request r;
-    int b, h, item, row0, n_rows, tile0, tile1, tiles;
+    int b, h, row0, n_rows, tile0, tile1, tiles;
     int lim_min, lim_max;  // keys that the first and last row see
     int last_cta;          // where the item ends in a later CTA: which
 };
 
-// The share of a CTA in the list of tiles.
+// The share of a CTA in the list of tiles, and the walk through it.
 struct Share {
     long long total, shares, u, u_end, b_begin;
     int b;
+    // The stretch that comes next, once `placed`: request, head, first row, the
+    // place in the item (COST counted) and its tiles.
+    bool placed;
+    Request r;
+    int h, row0, at, tiles;
 };
 
 // Where share c of `shares` begins in `total` tiles.  32-bit division where it
 // does: the 64-bit one is a long routine.
-__device__ __forceinline__ long long share_begin(long long total, long long c, long long shares) {
+__host__ __device__ __forceinline__ long long share_begin(long long total, long long c, long long shares) {
     const unsigned long long n = static_cast<unsigned long long>(total) * c;
     return (n >> 32) == 0 ? static_cast<unsigned>(n) / static_cast<unsigned>(shares) : n / shares;
 }
-__device__ __forceinline__ int quotient(long long a, long long b) {  // a, b >= 0, the result an int
+__host__ __device__ __forceinline__ int quotient(long long a, long long b) {  // a, b >= 0, the result an int
     return ((a | b) >> 32) == 0 ? static_cast<unsigned>(a) / static_cast<unsigned>(b) : static_cast<int>(a / b);
 }
 
-template <int ROWS, int KEYS>
-__device__ __forceinline__ int tile_count(const AttnArgs &p, const Request &r, int row0, int rows, int group) {
+template <int ROWS, int KEYS, int COST>
+__host__ __device__ __forceinline__ int tile_count(const AttnArgs &p, const Request &r, int row0, int rows, int group) {
     return max(1, (visible(p, r, (min(row0 + ROWS, rows) - 1) / group) + KEYS - 1) / KEYS);
 }
 
-// Tiles of all row tiles of a request, for one K/V head.
-template <int ROWS, int KEYS>
-__device__ __forceinline__ long long head_tiles(const AttnArgs &p, const Request &r, int group) {
+// What the row tiles of a request come to, for one K/V head.
+template <int ROWS, int KEYS, int COST>
+__host__ __device__ __forceinline__ long long head_tiles(const AttnArgs &p, const Request &r, int group) {
     const int rows = r.rows * group;
     long long n = 0;
 #pragma unroll 1
-    for (int row0 = 0; row0 < rows; row0 += ROWS) n += tile_count<ROWS, KEYS>(p, r, row0, rows, group);
+    for (int row0 = 0; row0 < rows; row0 += ROWS) n += COST + tile_count<ROWS, KEYS, COST>(p, r, row0, rows, group);
     return n;
 }
 
-template <int ROWS, int KEYS>
+template <int ROWS, int KEYS, int COST>
 __device__ __noinline__ long long request_weight(const AttnArgs &p, int b) {
-    return head_tiles<ROWS, KEYS>(p, request_of(p, b), p.H / p.Hkv) * p.Hkv;
+    return head_tiles<ROWS, KEYS, COST>(p, request_of(p, b), p.H / p.Hkv) * p.Hkv;
 }
 
-// The next stretch of one item in the share.
-template <int ROWS, int KEYS>
-__device__ __forceinline__ bool next_segment(const AttnArgs &p, Share &w, Segment &s) {
+// The next stretch of one item in the share.  The first is found by division;
+// from there the walk steps from row tile to row tile, head to head, request to
+// request.
+template <int ROWS, int KEYS, int COST>
+__host__ __device__ __forceinline__ bool next_segment(const AttnArgs &p, Share &w, Segment &s) {
     const int group = p.H / p.Hkv;
+    if (w.u >= w.u_end) return false;
+    if (!w.placed) {
+        w.placed = true;
+        w.r = request_of(p, w.b);
+        const long long per_head = head_tiles<ROWS, KEYS, COST>(p, w.r, group);
+        w.h = quotient(w.u - w.b_begin, per_head);
+        long long left = (w.u - w.b_begin) - w.h * per_head;
+        w.row0 = 0;
+        w.tiles = tile_count<ROWS, KEYS, COST>(p, w.r, 0, w.r.rows * group, group);
 #pragma unroll 1
-    while (w.u < w.u_end && w.b < p.batch) {
-        s.r = request_of(p, w.b);
-        const long long per_head = head_tiles<ROWS, KEYS>(p, s.r, group), all = per_head * p.Hkv;
-        if (w.u >= w.b_begin + all) {
-            w.b_begin += all;
-            ++w.b;
-            continue;
+        while (left >= w.tiles + COST) {
+            left -= w.tiles + COST;
+            w.row0 += ROWS;
+            w.tiles = tile_count<ROWS, KEYS, COST>(p, w.r, w.row0, w.r.rows * group, group);
         }
-        const int rows = s.r.rows * group;
-        s.b = w.b;
-        s.h = quotient(w.u - w.b_begin, per_head);
-        long long left = (w.u - w.b_begin) - s.h * per_head;
-        int rt = 0;
-        s.tiles = tile_count<ROWS, KEYS>(p, s.r, 0, rows, group);
-#pragma unroll 1
-        while (left >= s.tiles) {
-            left -= s.tiles;
-            ++rt;
-            s.tiles = tile_count<ROWS, KEYS>(p, s.r, rt * ROWS, rows, group);
-        }
-        s.row0 = rt * ROWS;
-        s.n_rows = min(ROWS, rows - s.row0);
-        s.item = s.h * ((rows + ROWS - 1) / ROWS) + rt;
-        s.tile0 = static_cast<int>(left);
-        s.tile1 = static_cast<int>(min(static_cast<long long>(s.tiles), left + (w.u_end - w.u)));
-        s.lim_min = visible(p, s.r, s.row0 / group);
-        s.lim_max = visible(p, s.r, (s.row0 + s.n_rows - 1) / group);
-        w.u += s.tile1 - s.tile0;
-        if (s.tile1 < s.tiles) {
-            // The CTA whose share holds the item's last tile.
-            const long long last = w.u + (s.tiles - s.tile1) - 1;
-            long long c = share_begin(w.shares, last, w.total);  // within one of the owner
-            while (share_begin(w.total, c + 1, w.shares) <= last) ++c;
-            while (share_begin(w.total, c, w.shares) > last) --c;
-            s.last_cta = static_cast<int>(c);
-        }
-        return true;
+        w.at = static_cast<int>(left);
     }
-    return false;
+    // The share's part of the item: from `at` (COST counted) as far as the share goes.
+    if (w.u_end - w.u <= COST - w.at) return false;  // no tile of it
+    const int rows = w.r.rows * group;
+    const int end = static_cast<int>(min(static_cast<long long>(w.tiles) + COST, w.at + (w.u_end - w.u)));
+    s.r = w.r;
+    s.b = w.b;
+    s.h = w.h;
+    s.row0 = w.row0;
+    s.n_rows = min(ROWS, rows - w.row0);
+    s.tiles = w.tiles;
+    s.tile0 = max(0, w.at - COST);
+    s.tile1 = end - COST;
+    s.lim_min = visible(p, w.r, w.row0 / group);
+    s.lim_max = visible(p, w.r, (w.row0 + s.n_rows - 1) / group);
+    w.u += end - w.at;
+    if (s.tile1 < s.tiles) {
+        // The CTA whose share holds the item's last tile; this is the share's last stretch.
+        const long long last = w.u + (s.tiles - s.tile1) - 1;
+        long long c = share_begin(w.shares, last, w.total);  // within one of the owner
+        while (share_begin(w.total, c + 1, w.shares) <= last) ++c;
+        while (share_begin(w.total, c, w.shares) > last) --c;
+        s.last_cta = static_cast<int>(c);
+    } else if (w.u < w.u_end) {
+        w.at = 0;
+        w.row0 += ROWS;
+        if (w.row0 >= rows) {
+            w.row0 = 0;
+            if (++w.h == p.Hkv) {
+                w.h = 0;
+                do {
+                    if (++w.b >= p.batch) {  // (lengths that changed under the kernel)
+                        w.u_end = w.u;
+                        return true;
+                    }
+                    w.r = request_of(p, w.b);
+                } while (w.r.rows == 0);
+            }
+        }
+        w.tiles = tile_count<ROWS, KEYS, COST>(p, w.r, w.row0, w.r.rows * group, group);
+    }
+    return true;
 }
 
 // Finds the CTA's share: called by all THREADS threads, `sum` one value a warp,
 // the result in `to` (visible after the next __syncthreads).
-template <int ROWS, int KEYS, int THREADS>
+template <int ROWS, int KEYS, int COST, int THREADS>
 __device__ __forceinline__ void find_share(const AttnArgs &p, long long (&sum)[THREADS / 32], Share &to) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const auto weight = [&](int b) -> long long { return b < p.batch ? request_weight<ROWS, KEYS>(p, b) : 0; };
+    const auto weight = [&](int b) -> long long { return b < p.batch ? request_weight<ROWS, KEYS, COST>(p, b) : 0; };
     // Inclusive sum over the block; `sum` then holds the warps' own.
     const auto inclusive = [&](long long v) -> long long {
 #pragma unroll
@@ -285,6 +318,7 @@ __device__ __forceinline__ void find_share(const AttnArgs &p, long long (&sum)[T
     if (tid == 0) {
         to.total = total;
         to.shares = shares;
+        to.placed = false;
         to.u = u;
         to.u_end = idle ? 0 : share_begin(total, blockIdx.x + 1, shares);
     }
@@ -345,27 +379,23 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int group = p.H / p.Hkv;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    clear_tail<T>(p);
-
     uint2 *const s_q = reinterpret_cast<uint2 *>(s_acc + C::kAccBytes / 4) + lane;  // [part][n][step][lane]
 
     if (tid == 0) sa.desc[blockIdx.x].segments = 0, s_any_nan = 0;
     for (int i = tid; i < C::kRows * (D / 32); i += kStreamThreads) s_nan[i / (D / 32)][i % (D / 32)] = 0;
-    find_share<C::kRows, kTileKeys, kStreamThreads>(p, s_sum, s_share);
+    find_share<C::kRows, kTileKeys, C::kItemCost, kStreamThreads>(p, s_sum, s_share);
     __syncthreads();
-    if (tid == 0) s_more[0] = next_segment<C::kRows, kTileKeys>(p, s_share, s_segs[0]);
+    if (tid == 0) s_more[0] = next_segment<C::kRows, kTileKeys, C::kItemCost>(p, s_share, s_segs[0]);
     __syncthreads();
 
     // ---- this warp's keys: 16 of every tile, one tile ahead in registers.
     // Column of the table and row in the page of the next ones, advanced without a division.
-    const int *table = nullptr;
-    int key = 0, key_end = 0, col = 0, row = 0, page = -1, page_next = -1, row_next = 0;
+    const int *entry = nullptr;  // of the table, of the next lookup
+    int key = 0, key_end = 0, row = 0, page = -1, page_next = -1, row_next = 0;
     const uint8_t *k_mine = nullptr, *v_mine = nullptr;
     float ks = 0.f, vs = 1.f;
-    int scale_at = 0;
     Bytes<16> kr[2][kHalves];
     Bytes<kVBytes> vr[4];
-    const int d_col = kTileKeys / p.block, d_row = kTileKeys - d_col * p.block;
     // (strides of the cache are below 2^31 bytes here, offsets 64-bit)
     const auto load_k = [&](int pg, int rw) {
         const uint8_t *at = k_mine + static_cast<long long>(pg) * sa.k_page + static_cast<long long>(rw) * sa.k_row;
@@ -381,26 +411,25 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
         load_bytes(vr[2], at + 8LL * sa.v_row);
         load_bytes(vr[3], at + 9LL * sa.v_row);
     };
-    const auto load_scales = [&](int pg) {
-        const int at = pg * p.Hkv + scale_at;  // (pages times heads fit 31 bits)
+    const auto load_scales = [&](int pg, const Segment &sg) {
+        const int at = pg * p.Hkv + *static_cast<const volatile int *>(&sg.h);  // (pages times heads fit 31 bits)
         ks = __ldg(p.k.scale + at);
         vs = __ldg(p.v.scale + at);
     };
-    const auto look_up = [&]() -> int {  // the table's entry at `col`, then a step on
-        const int x = __ldg(table + col);
-        col += d_col;
-        row += d_row;
-        if (row >= p.block) row -= p.block, ++col;
+    const auto look_up = [&]() -> int {  // the table's entry, then a step on
+        const int x = __ldg(entry);
+        entry += sa.d_col;
+        row += sa.d_row;
+        if (row >= p.block) row -= p.block, ++entry;
         return x;
     };
     const auto valid = [&](int x) { return static_cast<unsigned>(x) < static_cast<unsigned>(p.num_blocks); };
     const auto begin = [&](const Segment &sg) {  // the first loads of a segment
-        table = p.table + sg.b * p.table_stride;
-        scale_at = sg.h;
         key = sg.tile0 * kTileKeys + warp * 16;
         key_end = min(sg.tile1 * kTileKeys, sg.lim_max);
-        col = key / p.block;
+        const int col = key / p.block;
         row = key - col * p.block;
+        entry = p.table + sg.b * p.table_stride + col;
         k_mine = p.k.base + sg.h * p.k.s[1] + g * p.k.s[2] + t * 16;
         v_mine = p.v.base + sg.h * p.v.s[1] + 2 * t * p.v.s[2] + g * kVBytes;
         page = page_next = -1;
@@ -411,35 +440,68 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
             if (key + kTileKeys < key_end) page_next = look_up();
             if (valid(page)) {
                 load_k(page, rw);
-                load_scales(page);
+                load_scales(page, sg);
                 load_v(page, rw);
             }
         }
     };
 
-    if (s_more[0]) begin(s_segs[0]);
+    // Query rows of a segment as they are in memory: warp 0 loads them with the
+    // segment's first keys, where one row tile's fit the registers (rows of 16-byte
+    // vectors; others are read when laid out).
+    constexpr int kQVecs = kHalves * sizeof(T);
+    constexpr bool kEarly = NT == 1;
+    uint4 q_raw[NT][kQVecs];
+    const auto query_row = [&](const Segment &sg, int n) -> const T * {
+        const bool real = n * 8 + g < sg.n_rows;
+        const int rw = sg.row0 + n * 8 + g, i = rw / group;
+        return static_cast<const T *>(p.q) + (sg.r.first + (real ? i : 0)) * p.q_st[0] +
+               (sg.h * group + (real ? rw - i * group : 0)) * p.q_st[1] + t * 16;
+    };
+    const auto begin_queries = [&](const Segment &sg) {
+        if (!kEarly || warp != 0 || !sa.vec_q) return;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const T *q = query_row(sg, n);
+#pragma unroll
+            for (int i = 0; i < kQVecs; ++i)
+                q_raw[n][i] = *reinterpret_cast<const uint4 *>(q + i / static_cast<int>(sizeof(T)) * 64 +
+                                                               i % static_cast<int>(sizeof(T)) * (16 / sizeof(T)));
+        }
+    };
+
+    if (s_more[0]) {
+        begin(s_segs[0]);
+        begin_queries(s_segs[0]);
+    }
     for (int turn = 0; s_more[turn]; turn ^= 1) {
         const Segment &sg = s_segs[turn];
         // ---- the last warp walks on, the first lays the queries out as operands of S^T
-        if (tid == kStreamThreads - 32) s_more[turn ^ 1] = next_segment<C::kRows, kTileKeys>(p, s_share, s_segs[turn ^ 1]);
+        if (tid == kStreamThreads - 32) s_more[turn ^ 1] = next_segment<C::kRows, kTileKeys, C::kItemCost>(p, s_share, s_segs[turn ^ 1]);
         if (warp == 0) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const int rw = sg.row0 + n * 8 + g;
                 const bool real = n * 8 + g < sg.n_rows;
-                const int i = rw / group;
-                const T *q = static_cast<const T *>(p.q) + (sg.r.first + (real ? i : 0)) * p.q_st[0] +
-                             (sg.h * group + (real ? rw - i * group : 0)) * p.q_st[1];
                 float x[kHalves][16];
+                if (!kEarly) {
+                    const T *q = query_row(sg, n);
+#pragma unroll
+                    for (int hf = 0; hf < kHalves; ++hf) load_q16(x[hf], q + hf * 64, sa.vec_q != 0);
+                } else if (sa.vec_q) {
+                    const T *y = reinterpret_cast<const T *>(q_raw[n]);
+#pragma unroll
+                    for (int j = 0; j < kHalves * 16; ++j) x[j >> 4][j & 15] = Elem<T>::to_float(y[j]);
+                } else {
+                    const T *q = query_row(sg, n);
+#pragma unroll
+                    for (int j = 0; j < kHalves * 16; ++j)
+                        x[j >> 4][j & 15] = Elem<T>::to_float(q[(j >> 4) * 64 + (j & 15)]);
+                }
                 float amax = 0.f;
 #pragma unroll
-                for (int hf = 0; hf < kHalves; ++hf) {
-                    load_q16(x[hf], q + hf * 64 + t * 16, sa.vec_q != 0);
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        if (!real) x[hf][j] = 0.f;
-                        amax = fmaxf(amax, fabsf(x[hf][j]));
-                    }
+                for (int j = 0; j < kHalves * 16; ++j) {
+                    if (!real) x[j >> 4][j & 15] = 0.f;
+                    amax = fmaxf(amax, fabsf(x[j >> 4][j & 15]));
                 }
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
@@ -462,7 +524,7 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
                 }
                 if (t == 0) {
                     s_qscale[n * 8 + g] = exp2_int(e) * p.scale * 1.4426950408889634f;
-                    s_lim[n * 8 + g] = real ? visible(p, sg.r, i) : sg.r.keys;
+                    s_lim[n * 8 + g] = real ? visible(p, sg.r, (sg.row0 + n * 8 + g) / group) : sg.r.keys;
                 }
             }
         }
@@ -485,7 +547,6 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
             const bool there = valid(page);
             const bool more = key + kTileKeys < key_end, next = more && valid(page_next);
             float s[NT][4];
-            const float ks_now = ks, vs_now = vs;
             if (there) {
                 // S^T: 16 keys, NT x 8 queries
 #pragma unroll
@@ -504,12 +565,9 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
                         }
                 }
             }
-            if (next) {
-                load_k(page_next, row_next);
-                load_scales(page_next);
-            }
+            if (next) load_k(page_next, row_next);
             if (there) {
-                const float vs_ok = value_scale(vs_now);
+                const float vs_ok = value_scale(vs);
                 const float lv = log2_fast(vs_ok), inv_vs = rcp_fast(vs_ok);
                 const bool edge = key + 16 > lim_min;
                 if (edge) {
@@ -528,7 +586,7 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
                 const auto exponents = [&]() {
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        const float f0 = q_scale(n, 0) * ks_now, f1 = q_scale(n, 1) * ks_now;
+                        const float f0 = q_scale(n, 0) * ks, f1 = q_scale(n, 1) * ks;
                         const float o0 = lv - m[n][0], o1 = lv - m[n][1];
                         z[n][0] = fmaf(s[n][0], f0, o0);
                         z[n][1] = fmaf(s[n][1], f1, o1);
@@ -545,7 +603,7 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            float top = fmaf(fmaxf(s[n][c], s[n][c + 2]), q_scale(n, c) * ks_now, lv);
+                            float top = fmaf(fmaxf(s[n][c], s[n][c + 2]), q_scale(n, c) * ks, lv);
 #pragma unroll
                             for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                             top = fmaxf(top, m[n][c]);
@@ -587,7 +645,7 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
 #pragma unroll
                         for (int x = 0; x < kVBytes / 4; ++x) nan |= nan_bits(vr[i].w[x]);
                     if (__any_sync(0xffffffffu, nan != 0)) {
-                        if (lane < sg.n_rows) mark_nan(p, table, sg.h, key, min(key + 16, s_lim[lane]), s_nan[lane]);
+                        if (lane < sg.n_rows) mark_nan(p, p.table + sg.b * p.table_stride, sg.h, key, min(key + 16, s_lim[lane]), s_nan[lane]);
                         if (lane == 0) s_any_nan = 1;
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
@@ -615,7 +673,10 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
                         }
                 }
             }
-            if (next) load_v(page_next, row_next);
+            if (next) {
+                load_scales(page_next, sg);
+                load_v(page_next, row_next);
+            }
             page = page_next;
             row_next = row;
             if (key + 2 * kTileKeys < key_end) page_next = look_up();
@@ -642,6 +703,7 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
                                             acc[2 * x + 1][n][c + 2]);
                 }
             }
+        if (s_more[turn ^ 1]) begin_queries(s_segs[turn ^ 1]);
         __syncthreads();
         const bool whole = sg.tile0 == 0 && sg.tile1 == sg.tiles;
         const int slot = 2 * blockIdx.x + (sg.tile0 == 0 ? 1 : 0);
@@ -673,7 +735,7 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
             }
         }
         if (tid == 0 && sg.tile0 == 0 && !whole)  // begun here, ended by a later CTA
-            sa.desc[blockIdx.x] = StreamDesc{sg.b, sg.item, sg.last_cta - static_cast<int>(blockIdx.x) + 1, 0};
+            sa.desc[blockIdx.x] = StreamDesc{sg.last_cta - static_cast<int>(blockIdx.x) + 1, sg.r.first, sg.h, sg.row0, sg.n_rows, {}};
         if (s_any_nan) {
             __syncthreads();
             for (int i = tid; i < C::kRows * (D / 32); i += kStreamThreads) s_nan[i / (D / 32)][i % (D / 32)] = 0;
@@ -682,53 +744,70 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
         }
         __syncthreads();  // the queries, sums and segment may be written over
     }
+    clear_tail<T>(p);
 }
 
 // Joins the partial rows of the item that CTA blockIdx.x of the kernel before
 // began and did not end: rows blockIdx.y, blockIdx.y + gridDim.y, ... of its
-// row tile, a thread a column.
+// row tile, a thread a column, the segments shared out over groups of D threads.
+constexpr int kJoinThreads = 256;
+
 template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(D) paged_attention_join_kernel(const StreamArgs sa) {
-    __shared__ float s_w[kMaxStreamCtas];
-    __shared__ float s_red[D / 32];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const StreamDesc desc = sa.desc[blockIdx.x];
-    if (desc.segments == 0) return;
+__global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(const __grid_constant__ StreamArgs sa) {
+    constexpr int kGroups = kJoinThreads / D, kWarps = kJoinThreads / 32;
+    __shared__ float s_w[kMaxStreamCtas], s_top[kWarps], s_sum[kWarps], s_x[kGroups][D];
     const AttnArgs &p = sa.a;
-    const Request r = request_of(p, desc.b);
-    const int group = p.H / p.Hkv, n_rt = (r.rows * group + ROWS - 1) / ROWS;
-    const int h = desc.item / n_rt, row0 = (desc.item - h * n_rt) * ROWS;
-    const int n_rows = min(ROWS, r.rows * group - row0);
-    const int tid = threadIdx.x, n = desc.segments;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, d = tid % D, part = tid / D;
+    const int group = p.H / p.Hkv;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int n = sa.desc[blockIdx.x].segments;
+    if (n == 0) return;
+    const StreamDesc desc = sa.desc[blockIdx.x];
     const auto slot = [&](int i) { return i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i); };
-    for (int rw = blockIdx.y; rw < n_rows; rw += gridDim.y) {
-        __syncthreads();  // the row before is done
+    for (int rw = blockIdx.y; rw < desc.n_rows; rw += gridDim.y) {
         float top = -INFINITY;
-        for (int i = tid; i < n; i += D) {
+        for (int i = tid; i < n; i += kJoinThreads) {
             const float x = sa.part_lse[slot(i) * ROWS + rw];
             s_w[i] = x;
             top = fmaxf(top, x);
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if ((tid & 31) == 0) s_red[tid >> 5] = top;
+        if (lane == 0) s_top[warp] = top;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < D / 32; ++w) top = fmaxf(top, s_red[w]);
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_top[w]);
         const float base = top == -INFINITY ? 0.f : top;
-        float sum = 0.f, x = 0.f;
-#pragma unroll 8
-        for (int i = 0; i < n; ++i) {
+        float sum = 0.f;
+        for (int i = tid; i < n; i += kJoinThreads) {
             const float w = exp2_fast(s_w[i] - base);
+            s_w[i] = w;
             sum += w;
-            x = fmaf(w, sa.part_o[(static_cast<long long>(slot(i)) * ROWS + rw) * D + tid], x);
         }
-        x *= sum == 0.f ? 0.f : 1.f / sum;
-        const int row = row0 + rw, tok = row / group, head = h * group + row - tok * group;
-        const long long token = r.first + tok;
-        static_cast<T *>(p.o)[token * p.o_st[0] + head * p.o_st[1] + tid] = Elem<T>::from_float(x);
-        if (p.lse && tid == 0)
-            p.lse[token * p.H + head] = sum == 0.f ? -INFINITY : (base + log2f(sum)) * 0.6931471805599453f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) s_sum[warp] = sum;
+        __syncthreads();
+        sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) sum += s_sum[w];
+        float x = 0.f;
+#pragma unroll 16
+        for (int i = part; i < n; i += kGroups)
+            x = fmaf(s_w[i], sa.part_o[(static_cast<long long>(slot(i)) * ROWS + rw) * D + d], x);
+        s_x[part][d] = x;
+        __syncthreads();
+        if (part == 0) {
+#pragma unroll
+            for (int k = 1; k < kGroups; ++k) x += s_x[k][d];
+            x *= sum == 0.f ? 0.f : 1.f / sum;
+            const int row = desc.row0 + rw, tok = row / group, head = desc.h * group + row - tok * group;
+            const long long token = desc.first + tok;
+            static_cast<T *>(p.o)[token * p.o_st[0] + head * p.o_st[1] + d] = Elem<T>::from_float(x);
+            if (p.lse && d == 0)
+                p.lse[token * p.H + head] = sum == 0.f ? -INFINITY : (base + log2f(sum)) * 0.6931471805599453f;
+        }
+        __syncthreads();  // the row's values have been read
     }
 }
 

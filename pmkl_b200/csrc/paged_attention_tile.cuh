@@ -38,6 +38,7 @@ namespace paged {
 
 constexpr int kTileRows = 128;
 constexpr int kTileThreads = 384;
+constexpr int kTileItemCost = 1;  // of an item, in tiles: some 8000 cycles against 7000
 // Registers a thread: at launch, and what each warpgroup sets; the three come
 // to the launch's total (the host checks that the build has it).
 constexpr int kTileLaunchRegs = 80, kTileSoftmaxRegs = 120, kTileLoadRegs = 72, kTileIssueRegs = 48;
@@ -142,8 +143,6 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
     const int group = p.H / p.Hkv;
     volatile int *abort_flag = &sh.abort_flag;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    clear_tail<T>(p);
-
     // ---- set-up: barriers, tensor memory, this CTA's share
     if (tid == 0) {
         mbar_init(&sh.q_full, 128);
@@ -173,7 +172,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
         tmem_alloc(&sh.tmem, C::kTmemCols);
         tmem_relinquish();
     }
-    find_share<kTileRows, 128, kTileThreads>(p, sh.sum, sh.share);
+    find_share<kTileRows, 128, kTileItemCost, kTileThreads>(p, sh.sum, sh.share);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -189,7 +188,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                 const int i = seg & 1;
                 if (seg >= 2 && !mbar_wait(&sh.seg_empty[i], ((seg >> 1) - 1) & 1, abort_flag)) break;
                 Segment &s = sh.seg[i];
-                more = next_segment<kTileRows, 128>(p, sh.share, s);
+                more = next_segment<kTileRows, 128, kTileItemCost>(p, sh.share, s);
                 if (!more) s.tile0 = s.tile1 = 0;
                 mbar_arrive(&sh.seg_full[i]);
             }
@@ -553,7 +552,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                 if (real && !whole) sa.part_lse[slot * kTileRows + tid] = lse2;
                 // Begun here, ended by a later CTA.
                 if (tid == 0 && tile0 == 0 && !whole)
-                    sa.desc[blockIdx.x] = StreamDesc{s.b, s.item, s.last_cta - static_cast<int>(blockIdx.x) + 1, 0};
+                    sa.desc[blockIdx.x] = StreamDesc{s.last_cta - static_cast<int>(blockIdx.x) + 1, s.r.first, s.h, s.row0, s.n_rows, {}};
                 tc_fence_before();
             }
             __syncwarp();
@@ -569,6 +568,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
         tmem_dealloc(tmem, C::kTmemCols);
     }
     if (tid == 0 && *abort_flag && !skip) report_device_error(PMKL_DEVERR_TIMEOUT);
+    clear_tail<T>(p);
 }
 
 }  // namespace paged

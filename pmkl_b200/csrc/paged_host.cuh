@@ -133,9 +133,11 @@ long long share_grid(long long resident, long long most, long long items, long l
 
 // Workspace addresses and alignments of the shared-out kernels.
 template <typename T>
-paged::StreamArgs shared_args(const paged::AttnArgs &a, void *workspace, int ctas, int rows) {
+paged::StreamArgs shared_args(const paged::AttnArgs &a, void *workspace, int ctas, int rows, int tile_keys) {
     paged::StreamArgs p{};
     p.a = a;
+    p.d_col = tile_keys / a.block;
+    p.d_row = tile_keys % a.block;
     constexpr long long kVec = 16 / sizeof(T);
     p.vec_q = aligned16(a.q) && a.q_st[0] % kVec == 0 && a.q_st[1] % kVec == 0;
     p.vec_o = aligned16(a.o) && a.o_st[0] % kVec == 0 && a.o_st[1] % kVec == 0;
@@ -157,7 +159,7 @@ int launch_join(const paged::StreamArgs &p, long long grid, cudaStream_t stream)
     const long long rows = std::min<long long>(ROWS, static_cast<long long>(p.a.H / p.a.Hkv) * p.a.max_q);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(grid), static_cast<unsigned>(std::min<long long>(rows, 16)));
-    cfg.blockDim = dim3(D);
+    cfg.blockDim = dim3(paged::kJoinThreads);
     cfg.stream = stream;
     cudaLaunchAttribute early{};
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -198,7 +200,7 @@ int launch_stream(const paged::AttnArgs &a, void *workspace, cudaStream_t stream
     auto kernel = paged::paged_attention_stream_kernel<T, D, NT>;
     const int per_sm = occupancy.get(kernel, C::kThreads, C::kSmemBytes);
     if (per_sm < 1) return PMKL_ERR_LAUNCH;
-    const paged::StreamArgs p = shared_args<T>(a, workspace, paged::kMaxStreamCtas, C::kRows);
+    const paged::StreamArgs p = shared_args<T>(a, workspace, paged::kMaxStreamCtas, C::kRows, C::kTileKeys);
     const long long tiles = std::max<long long>(
         1, (static_cast<long long>(a.max_blocks) * a.block + C::kTileKeys - 1) / C::kTileKeys);
     const long long row_tiles = (static_cast<long long>(a.H / a.Hkv) * a.max_q + C::kRows - 1) / C::kRows;
@@ -232,7 +234,7 @@ int launch_tile(const paged::AttnArgs &a, void *workspace, cudaStream_t stream) 
     // Tensor memory holds two CTAs an SM.
     const int per_sm = 2 + 0 * occupancy.get(kernel, paged::kTileThreads, C::kSmemBytes);
     if (per_sm < 1) return PMKL_ERR_LAUNCH;
-    const paged::StreamArgs p = shared_args<T>(a, workspace, paged::kMaxTileCtas, paged::kTileRows);
+    const paged::StreamArgs p = shared_args<T>(a, workspace, paged::kMaxTileCtas, paged::kTileRows, 128);
     const long long tiles = std::max<long long>(1, (static_cast<long long>(a.max_blocks) * a.block + 127) / 128);
     const long long row_tiles = (static_cast<long long>(a.H / a.Hkv) * a.max_q + 127) / 128;
     const long long grid = share_grid(static_cast<long long>(sm_count()) * per_sm, paged::kMaxTileCtas,

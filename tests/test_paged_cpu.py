@@ -104,3 +104,18 @@ def test_plain_forms():
     seq, starts, slots, left, status, table = ref.plan([5, 0], [4, 2], [[7, 8, -1], [-1] * 3], [1, 2, 3], 3, 4, 7)
     assert (seq, starts, left, status) == ([9, 2], [0, 4, 6], 1, [0, 0])
     assert table == [[7, 8, 3], [2, -1, -1]] and slots == [33, 34, 35, 12, 8, 9, -1]
+
+
+def test_walk_over_shares(tmp_path):
+    """The device code that hands an attention's tiles out to CTAs, run on the host: every tile once, in order."""
+    import subprocess
+    from pathlib import Path
+
+    from pmkl_b200 import build
+
+    repo = Path(__file__).resolve().parent.parent
+    exe = tmp_path / "walk_test"
+    subprocess.run([build._nvcc(), *build.NVCC_ARCH, "-O1", "-std=c++17", "-I", str(build.INCLUDE), "-I", str(build.CSRC),
+                    str(repo / "tests" / "cpp" / "walk_test.cu"), "-o", str(exe)], check=True)
+    out = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert out.returncode == 0 and "walk ok" in out.stdout, out.stdout

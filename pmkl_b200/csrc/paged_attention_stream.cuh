@@ -117,18 +117,25 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-// Streaming loads: a step reads the cache once.
-template <int BYTES>
-struct Bytes {
-    uint32_t w[BYTES / 4];
-};
-__device__ __forceinline__ void load_bytes(Bytes<16> &r, const uint8_t *p) {
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3])
-                 : "l"(p));
+// Asynchronous copies to shared memory: 16 bytes past L1 (a step reads the cache
+// once), or 4.
+__device__ __forceinline__ void copy16(uint32_t to, const void *from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
-__device__ __forceinline__ void load_bytes(Bytes<8> &r, const uint8_t *p) {
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(r.w[0]), "=r"(r.w[1]) : "l"(p));
+__device__ __forceinline__ void copy4(uint32_t to, const void *from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copies_wait_but_one() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
+__device__ __forceinline__ uint4 shared16(uint32_t at) {
+    uint4 r;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at) : "memory");
+    return r;
+}
+__device__ __forceinline__ uint2 shared8(uint32_t at) {
+    uint2 r;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(at) : "memory");
+    return r;
 }
 
 // 16 bytes, or zeros where `there` is false: predicated, not branched around.
@@ -152,9 +159,14 @@ struct StreamCfg {
     static constexpr int kTileKeys = 16 * kWarps;  // keys a CTA takes at a time
     static constexpr int kItemCost = 3;            // of an item, in tiles: some 8000 cycles against 2450 (16 x 4096 keys)
     static constexpr int kRowPitch = D + 32;  // 4 floats behind every D / 8: a warp's float4 stores meet no bank twice
-    // The warps' sums; the query operands, 8 bytes a lane and step, for two fp16 parts.
-    static constexpr int kAccBytes = kWarps * kRows * kRowPitch * 4;
-    static constexpr int kSmemBytes = kAccBytes + 2 * NT * (D / 16) * 32 * 8;
+    // Two stages of 16 keys and values a warp, and their scales.
+    static constexpr int kStageBytes = 2 * 16 * D + 16;
+    static constexpr int kDataBytes = kWarps * 2 * kStageBytes;
+    // The warps' sums: one warp each, or (16 and 32 rows) two adding to one.
+    static constexpr int kSlots = NT == 1 ? kWarps : kWarps / 2;
+    static constexpr int kAccBytes = kSlots * kRows * kRowPitch * 4;
+    // The query operands, 8 bytes a lane and step, for two fp16 parts.
+    static constexpr int kSmemBytes = kDataBytes + kAccBytes + 2 * NT * (D / 16) * 32 * 8;
 };
 
 __host__ __device__ constexpr size_t partial_workspace(int ctas, int rows, int D) {
@@ -365,7 +377,8 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
     constexpr int kHalves = D / 64;  // 16-byte loads of a key row
     constexpr int kMt = D / 16;      // 16-row tiles of O^T
     constexpr int kVBytes = D / 8;   // bytes of a V row a thread
-    extern __shared__ __align__(16) float s_acc[];
+    extern __shared__ __align__(16) uint8_t s_dyn[];
+    float *const s_acc = reinterpret_cast<float *>(s_dyn + C::kDataBytes);
     __shared__ float s_m[kStreamWarps][C::kRows], s_l[kStreamWarps][C::kRows];
     __shared__ alignas(8) int s_lim[C::kRows];  // keys that a row sees
     __shared__ uint32_t s_nan[C::kRows][D / 32];  // columns of a row that are NaN, where s_any_nan
@@ -388,62 +401,60 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
     if (tid == 0) s_more[0] = next_segment<C::kRows, kTileKeys, C::kItemCost>(p, s_share, s_segs[0]);
     __syncthreads();
 
-    // ---- this warp's keys: 16 of every tile, one tile ahead in registers.
-    // Column of the table and row in the page of the next ones, advanced without a division.
+    // ---- this warp's keys: 16 of every tile, two tiles in shared memory, copied
+    // there asynchronously; a table entry ahead of that.  16-byte chunks of a row
+    // are exchanged by the row so that the reads below meet no bank twice: chunk c
+    // of row r of the keys is at c ^ 4 (r % 2), of the values at c ^ 2 (r / 2 % 4)
+    // (head size 128; at 64 the values' at c ^ (r / 2 % 4)).
+    constexpr int kPerRow = D / 16, kCopies = D / 32;  // chunks of a row; copies a lane and side
+    const uint32_t s_stage = static_cast<uint32_t>(__cvta_generic_to_shared(s_dyn)) + warp * 2 * C::kStageBytes;
+    const int c_row = lane / kPerRow, c_chunk = lane % kPerRow;  // (rows c_row, c_row + 32 / kPerRow, ...)
     const int *entry = nullptr;  // of the table, of the next lookup
-    int key = 0, key_end = 0, row = 0, page = -1, page_next = -1, row_next = 0;
+    int key = 0, key_end = 0, row = 0, ahead = -1;
+    bool there = false, there_next = false;
+    uint32_t stage = 0;
     const uint8_t *k_mine = nullptr, *v_mine = nullptr;
-    float ks = 0.f, vs = 1.f;
-    Bytes<16> kr[2][kHalves];
-    Bytes<kVBytes> vr[4];
+    const auto look_up = [&]() -> int { return __ldg(entry); };  // the table's entry of the next tile to copy
+    // Copies the tile whose entry is x to stage st and steps on; true where its page is one.
     // (strides of the cache are below 2^31 bytes here, offsets 64-bit)
-    const auto load_k = [&](int pg, int rw) {
-        const uint8_t *at = k_mine + static_cast<long long>(pg) * sa.k_page + static_cast<long long>(rw) * sa.k_row;
+    const auto copy_tile = [&](int x, uint32_t st, const Segment &sg) -> bool {
+        const bool ok = static_cast<unsigned>(x) < static_cast<unsigned>(p.num_blocks);
+        if (ok) {
+            const uint8_t *k = k_mine + static_cast<long long>(x) * sa.k_page + static_cast<long long>(row) * sa.k_row;
+            const uint8_t *v = v_mine + static_cast<long long>(x) * sa.v_page + static_cast<long long>(row) * sa.v_row;
+            const uint32_t to = s_stage + st * C::kStageBytes;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int hf = 0; hf < kHalves; ++hf) load_bytes(kr[i][hf], at + i * 8LL * sa.k_row + hf * 64);
-    };
-    const auto load_v = [&](int pg, int rw) {
-        const uint8_t *at = v_mine + static_cast<long long>(pg) * sa.v_page + static_cast<long long>(rw) * sa.v_row;
-        load_bytes(vr[0], at);
-        load_bytes(vr[1], at + sa.v_row);
-        load_bytes(vr[2], at + 8LL * sa.v_row);
-        load_bytes(vr[3], at + 9LL * sa.v_row);
-    };
-    const auto load_scales = [&](int pg, const Segment &sg) {
-        const int at = pg * p.Hkv + *static_cast<const volatile int *>(&sg.h);  // (pages times heads fit 31 bits)
-        ks = __ldg(p.k.scale + at);
-        vs = __ldg(p.v.scale + at);
-    };
-    const auto look_up = [&]() -> int {  // the table's entry, then a step on
-        const int x = __ldg(entry);
+            for (int i = 0; i < kCopies; ++i) {
+                const int r = c_row + i * (32 / kPerRow);
+                copy16(to + r * D + (D == 128 ? (c_chunk ^ (r & 1) << 2) : c_chunk) * 16, k + i * (32 / kPerRow) * static_cast<long long>(sa.k_row));
+                copy16(to + 16 * D + r * D + (D == 128 ? (c_chunk ^ (r >> 1 & 3) << 1) : (c_chunk ^ (r >> 1 & 3))) * 16,
+                       v + i * (32 / kPerRow) * static_cast<long long>(sa.v_row));
+            }
+            if (lane < 2) copy4(to + 32 * D + lane * 4, (lane ? p.v.scale : p.k.scale) + x * p.Hkv + sg.h);
+        }
         entry += sa.d_col;
         row += sa.d_row;
         if (row >= p.block) row -= p.block, ++entry;
-        return x;
+        return ok;
     };
-    const auto valid = [&](int x) { return static_cast<unsigned>(x) < static_cast<unsigned>(p.num_blocks); };
-    const auto begin = [&](const Segment &sg) {  // the first loads of a segment
+    const auto begin = [&](const Segment &sg) {  // the first copies of a segment
         key = sg.tile0 * kTileKeys + warp * 16;
         key_end = min(sg.tile1 * kTileKeys, sg.lim_max);
         const int col = key / p.block;
         row = key - col * p.block;
         entry = p.table + sg.b * p.table_stride + col;
-        k_mine = p.k.base + sg.h * p.k.s[1] + g * p.k.s[2] + t * 16;
-        v_mine = p.v.base + sg.h * p.v.s[1] + 2 * t * p.v.s[2] + g * kVBytes;
-        page = page_next = -1;
-        if (key < key_end) {
-            const int rw = row;
-            page = look_up();
-            row_next = row;
-            if (key + kTileKeys < key_end) page_next = look_up();
-            if (valid(page)) {
-                load_k(page, rw);
-                load_scales(page, sg);
-                load_v(page, rw);
-            }
-        }
+        k_mine = p.k.base + sg.h * p.k.s[1] + c_row * p.k.s[2] + c_chunk * 16;
+        v_mine = p.v.base + sg.h * p.v.s[1] + c_row * p.v.s[2] + c_chunk * 16;
+        there = there_next = false;
+        stage = 0;
+        int x0 = -1, x1 = -1;
+        if (key < key_end) x0 = look_up();
+        if (key + kTileKeys < key_end) x1 = __ldg(entry + sa.d_col + (row + sa.d_row >= p.block ? 1 : 0));
+        if (key < key_end) there = copy_tile(x0, 0, sg);
+        copies_commit();
+        if (key + kTileKeys < key_end) there_next = copy_tile(x1, 1, sg);
+        copies_commit();
+        if (key + 2 * kTileKeys < key_end) ahead = look_up();
     };
 
     // Query rows of a segment as they are in memory: warp 0 loads them with the
@@ -544,29 +555,34 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
             return *static_cast<const volatile float *>(&s_qscale[n * 8 + 2 * t + c]);
         };
         for (; key < key_end; key += kTileKeys) {
-            const bool there = valid(page);
-            const bool more = key + kTileKeys < key_end, next = more && valid(page_next);
-            float s[NT][4];
+            copies_wait_but_one();
+            __syncwarp();
+            const uint32_t at = s_stage + stage * C::kStageBytes;
             if (there) {
                 // S^T: 16 keys, NT x 8 queries
+                float s[NT][4];
 #pragma unroll
                 for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
-                for (int x = 0; x < kSteps; ++x) {
-                    const uint32_t lo = kr[0][x >> 2].w[x & 3], hi = kr[1][x >> 2].w[x & 3];
-                    const uint32_t a0 = e4m3x2_to_h2(lo), a2 = e4m3x2_to_h2_hi(lo);
-                    const uint32_t a1 = e4m3x2_to_h2(hi), a3 = e4m3x2_to_h2_hi(hi);
+                for (int hf = 0; hf < kHalves; ++hf) {
+                    const int c = (hf * 4 + t) ^ (D == 128 ? (g & 1) << 2 : 0);
+                    const uint4 k0 = shared16(at + g * D + c * 16), k8 = shared16(at + (g + 8) * D + c * 16);
+                    const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w8[4] = {k8.x, k8.y, k8.z, k8.w};
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t a0 = e4m3x2_to_h2(w0[i]), a2 = e4m3x2_to_h2_hi(w0[i]);
+                        const uint32_t a1 = e4m3x2_to_h2(w8[i]), a3 = e4m3x2_to_h2_hi(w8[i]);
 #pragma unroll
-                        for (int part = 0; part < kParts; ++part) {
-                            const uint2 q2 = s_q[((part * NT + n) * kSteps + x) * 32];
-                            mma16816(s[n], a0, a1, a2, a3, q2.x, q2.y);
-                        }
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int part = 0; part < kParts; ++part) {
+                                const uint2 q2 = s_q[((part * NT + n) * kSteps + hf * 4 + i) * 32];
+                                mma16816(s[n], a0, a1, a2, a3, q2.x, q2.y);
+                            }
+                    }
                 }
-            }
-            if (next) load_k(page_next, row_next);
-            if (there) {
+                const uint2 scales = shared8(at + 32 * D);
+                const float ks = __uint_as_float(scales.x), vs = __uint_as_float(scales.y);
                 const float vs_ok = value_scale(vs);
                 const float lv = log2_fast(vs_ok), inv_vs = rcp_fast(vs_ok);
                 const bool edge = key + 16 > lim_min;
@@ -631,35 +647,48 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
                         pf[kParts - 1][n][1] = transpose8x8(h2_bits(p2 - ch.x, p3 - ch.y));
                     }
                 }
+                uint32_t vr[4][kVBytes / 4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = 2 * t + (i & 1) + (i >> 1) * 8;
+                    const uint32_t v_at = at + 16 * D + r * D;
+                    if constexpr (D == 128) {
+                        const uint4 x = shared16(v_at + (g ^ t << 1) * 16);
+                        vr[i][0] = x.x, vr[i][1] = x.y, vr[i][kVBytes / 4 - 2] = x.z, vr[i][kVBytes / 4 - 1] = x.w;
+                    } else {
+                        const uint2 x = shared8(v_at + ((g >> 1) ^ t) * 16 + (g & 1) * 8);
+                        vr[i][0] = x.x, vr[i][1] = x.y;
+                    }
+                }
                 if (edge) {
                     // Rows behind the last key: zero.
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         if (key + 2 * t + (i & 1) + (i >> 1) * 8 >= lim_max)
 #pragma unroll
-                            for (int x = 0; x < kVBytes / 4; ++x) vr[i].w[x] = 0;
+                            for (int x = 0; x < kVBytes / 4; ++x) vr[i][x] = 0;
                     // NaN in rows that some queries do not see.
                     uint32_t nan = 0;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
 #pragma unroll
-                        for (int x = 0; x < kVBytes / 4; ++x) nan |= nan_bits(vr[i].w[x]);
+                        for (int x = 0; x < kVBytes / 4; ++x) nan |= nan_bits(vr[i][x]);
                     if (__any_sync(0xffffffffu, nan != 0)) {
                         if (lane < sg.n_rows) mark_nan(p, p.table + sg.b * p.table_stride, sg.h, key, min(key + 16, s_lim[lane]), s_nan[lane]);
                         if (lane == 0) s_any_nan = 1;
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
 #pragma unroll
-                            for (int x = 0; x < kVBytes / 4; ++x) vr[i].w[x] = without_nan(vr[i].w[x]);
+                            for (int x = 0; x < kVBytes / 4; ++x) vr[i][x] = without_nan(vr[i][x]);
                     }
                 }
                 // O^T += V^T P^T
 #pragma unroll
                 for (int x = 0; x < kVBytes / 4; ++x) {
-                    const uint32_t e0 = __byte_perm(vr[0].w[x], vr[1].w[x], 0x5140);  // dims 4x, 4x + 1 of keys 2t, 2t + 1
-                    const uint32_t o0 = __byte_perm(vr[0].w[x], vr[1].w[x], 0x7362);  // dims 4x + 2, 4x + 3
-                    const uint32_t e1 = __byte_perm(vr[2].w[x], vr[3].w[x], 0x5140);  // of keys 2t + 8, 2t + 9
-                    const uint32_t o1 = __byte_perm(vr[2].w[x], vr[3].w[x], 0x7362);
+                    const uint32_t e0 = __byte_perm(vr[0][x], vr[1][x], 0x5140);  // dims 4x, 4x + 1 of keys 2t, 2t + 1
+                    const uint32_t o0 = __byte_perm(vr[0][x], vr[1][x], 0x7362);  // dims 4x + 2, 4x + 3
+                    const uint32_t e1 = __byte_perm(vr[2][x], vr[3][x], 0x5140);  // of keys 2t + 8, 2t + 9
+                    const uint32_t o1 = __byte_perm(vr[2][x], vr[3][x], 0x7362);
                     const uint32_t a0 = e4m3x2_to_h2(e0), a1 = e4m3x2_to_h2_hi(e0);
                     const uint32_t a2 = e4m3x2_to_h2(e1), a3 = e4m3x2_to_h2_hi(e1);
                     const uint32_t c0 = e4m3x2_to_h2(o0), c1 = e4m3x2_to_h2_hi(o0);
@@ -673,38 +702,66 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
                         }
                 }
             }
-            if (next) {
-                load_scales(page_next, sg);
-                load_v(page_next, row_next);
-            }
-            page = page_next;
-            row_next = row;
-            if (key + 2 * kTileKeys < key_end) page_next = look_up();
+            __syncwarp();  // the stage has been read
+            bool more = false;
+            if (key + 2 * kTileKeys < key_end) more = copy_tile(ahead, stage, sg);
+            copies_commit();
+            there = there_next;
+            there_next = more;
+            stage ^= 1;
+            if (key + 3 * kTileKeys < key_end) ahead = look_up();
         }
 
-        // ---- the next segment's first loads, then the warps join
+        // ---- the next segment's first copies, then the warps join
         if (s_more[turn ^ 1]) begin(s_segs[turn ^ 1]);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const int rw = n * 8 + 2 * t + c;
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], o);
                 if (g == 0) {
-                    s_m[warp][rw] = m[n][c];
-                    s_l[warp][rw] = l[n][c];
-                }
-                if (rw < sg.n_rows) {
-                    float4 *at = reinterpret_cast<float4 *>(s_acc + (warp * C::kRows + rw) * C::kRowPitch + g * (D / 8 + 4));
-#pragma unroll
-                    for (int x = 0; x < kMt / 2; ++x)
-                        at[x] = make_float4(acc[2 * x][n][c], acc[2 * x][n][c + 2], acc[2 * x + 1][n][c],
-                                            acc[2 * x + 1][n][c + 2]);
+                    s_m[warp][n * 8 + 2 * t + c] = m[n][c];
+                    s_l[warp][n * 8 + 2 * t + c] = l[n][c];
                 }
             }
+        const auto store_sums = [&](bool scaled, bool add) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int rw = n * 8 + 2 * t + c;
+                    if (rw >= sg.n_rows) continue;
+                    float fix = 1.f;
+                    if (scaled) {
+                        float top = s_m[0][rw];
+#pragma unroll
+                        for (int w = 1; w < kStreamWarps; ++w) top = fmaxf(top, s_m[w][rw]);
+                        fix = exp2_fast(m[n][c] - top);
+                    }
+                    float4 *to = reinterpret_cast<float4 *>(s_acc + (warp % C::kSlots * C::kRows + rw) * C::kRowPitch + g * (D / 8 + 4));
+#pragma unroll
+                    for (int x = 0; x < kMt / 2; ++x) {
+                        float4 v = make_float4(acc[2 * x][n][c] * fix, acc[2 * x][n][c + 2] * fix, acc[2 * x + 1][n][c] * fix,
+                                               acc[2 * x + 1][n][c + 2] * fix);
+                        if (add) {
+                            const float4 o = to[x];
+                            v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+                        }
+                        to[x] = v;
+                    }
+                }
+        };
+        constexpr bool kTwoRounds = C::kSlots < kStreamWarps;
+        if constexpr (!kTwoRounds) store_sums(false, false);
         if (s_more[turn ^ 1]) begin_queries(s_segs[turn ^ 1]);
         __syncthreads();
+        if constexpr (kTwoRounds) {  // the maxima are known: each warp scales its sums, the second half adds
+            if (warp < C::kSlots) store_sums(true, false);
+            __syncthreads();
+            if (warp >= C::kSlots) store_sums(true, true);
+            __syncthreads();
+        }
         const bool whole = sg.tile0 == 0 && sg.tile1 == sg.tiles;
         const int slot = 2 * blockIdx.x + (sg.tile0 == 0 ? 1 : 0);
         for (int i = tid; i < sg.n_rows * D; i += kStreamThreads) {
@@ -719,8 +776,11 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
             for (int w = 0; w < kStreamWarps; ++w) {
                 const float fix = exp2_fast(s_m[w][rw] - top);
                 sum = fmaf(fix, s_l[w][rw], sum);
-                x = fmaf(fix, from[w * C::kRows * C::kRowPitch], x);
+                if (!kTwoRounds) x = fmaf(fix, from[w * C::kRows * C::kRowPitch], x);
             }
+            if constexpr (kTwoRounds)
+#pragma unroll
+                for (int w = 0; w < C::kSlots; ++w) x += from[w * C::kRows * C::kRowPitch];
             x *= sum == 0.f ? 0.f : 1.f / sum;
             if (s_any_nan && (s_nan[rw][d >> 5] >> (d & 31) & 1u)) x = NAN;
             const float lse2 = sum == 0.f ? -INFINITY : top + log2f(sum);

@@ -93,8 +93,46 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
 // side, so that a token's whole row is read at about one time.
 constexpr int kSpanMax = 32;
 
-// Shares of one 16-byte vector: its largest finite magnitude, and its elements
-// divided by a power of two as 8-bit floats.
+// The largest magnitude of 16-byte vectors, kept as the elements are: fp32, or
+// two 16-bit maxima side by side (one instruction for two elements).  NaN is
+// passed over; an infinity stays, and the caller then looks again by element.
+template <typename T>
+struct Largest;
+template <>
+struct Largest<float> {
+    float m = 0.f;
+    __device__ __forceinline__ void add(const uint4 &u) {
+        m = fmaxf(fmaxf(fmaxf(m, fabsf(__uint_as_float(u.x))), fabsf(__uint_as_float(u.y))),
+                  fmaxf(fabsf(__uint_as_float(u.z)), fabsf(__uint_as_float(u.w))));
+    }
+    __device__ __forceinline__ float get() const { return m; }
+};
+template <>
+struct Largest<__half> {
+    __half2 m = __float2half2_rn(0.f);
+    __device__ __forceinline__ static __half2 mag(uint32_t w) {
+        w &= 0x7FFF7FFFu;
+        return *reinterpret_cast<const __half2 *>(&w);
+    }
+    __device__ __forceinline__ void add(const uint4 &u) {
+        m = __hmax2(__hmax2(m, __hmax2(mag(u.x), mag(u.y))), __hmax2(mag(u.z), mag(u.w)));
+    }
+    __device__ __forceinline__ float get() const { return fmaxf(__low2float(m), __high2float(m)); }
+};
+template <>
+struct Largest<__nv_bfloat16> {
+    __nv_bfloat162 m = __float2bfloat162_rn(0.f);
+    __device__ __forceinline__ static __nv_bfloat162 mag(uint32_t w) {
+        w &= 0x7FFF7FFFu;
+        return *reinterpret_cast<const __nv_bfloat162 *>(&w);
+    }
+    __device__ __forceinline__ void add(const uint4 &u) {
+        m = __hmax2(__hmax2(m, __hmax2(mag(u.x), mag(u.y))), __hmax2(mag(u.z), mag(u.w)));
+    }
+    __device__ __forceinline__ float get() const { return fmaxf(__low2float(m), __high2float(m)); }
+};
+
+// The largest finite magnitude of a vector, element by element.
 template <typename T>
 __device__ __forceinline__ float vec_amax(const uint4 &u) {
     const T *e = reinterpret_cast<const T *>(&u);
@@ -104,24 +142,35 @@ __device__ __forceinline__ float vec_amax(const uint4 &u) {
     return a;
 }
 
+// The two elements of a word as fp32.
+template <typename T>
+__device__ __forceinline__ float2 word_floats(uint32_t w);
+template <>
+__device__ __forceinline__ float2 word_floats<__half>(uint32_t w) {
+    return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+template <>
+__device__ __forceinline__ float2 word_floats<__nv_bfloat16>(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+
 __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d) {
     uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
     uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
     return lo | hi << 16;
 }
 
+// A vector's elements times `inv` as 8-bit floats.
 template <typename T>
 __device__ __forceinline__ void vec_store(uint8_t *dst, const uint4 &u, float inv) {
-    const T *e = reinterpret_cast<const T *>(&u);
-    uint32_t w[4 / sizeof(T)];
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(4 / sizeof(T)); ++i)
-        w[i] = pack_e4m3(Elem<T>::to_float(e[4 * i]) * inv, Elem<T>::to_float(e[4 * i + 1]) * inv,
-                         Elem<T>::to_float(e[4 * i + 2]) * inv, Elem<T>::to_float(e[4 * i + 3]) * inv);
-    if constexpr (sizeof(T) == 4)
-        *reinterpret_cast<uint32_t *>(dst) = w[0];
-    else
-        *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<uint32_t *>(dst) = pack_e4m3(__uint_as_float(u.x) * inv, __uint_as_float(u.y) * inv,
+                                                       __uint_as_float(u.z) * inv, __uint_as_float(u.w) * inv);
+    } else {
+        const float2 a = word_floats<T>(u.x), b = word_floats<T>(u.y), c = word_floats<T>(u.z), d = word_floats<T>(u.w);
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_e4m3(a.x * inv, a.y * inv, b.x * inv, b.y * inv),
+                                                     pack_e4m3(c.x * inv, c.y * inv, d.x * inv, d.y * inv));
+    }
 }
 
 template <typename T, int WPU, int NV>
@@ -178,7 +227,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_vec_kernel(const 
         uint8_t *dst = c.base + page * c.s[0] + h * c.s[1] + col;
 
         uint4 v[NV];
-        float amax = 0.f;
+        Largest<T> largest;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int i = row_first + k * row_step;
@@ -186,9 +235,17 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_vec_kernel(const 
             if (active && i < n) v[k] = *reinterpret_cast<const uint4 *>(x + i * x_row);
         }
         for (int i = row_first + NV * row_step; active && i < n; i += row_step)
-            amax = fmaxf(amax, vec_amax<T>(*reinterpret_cast<const uint4 *>(x + i * x_row)));
+            largest.add(*reinterpret_cast<const uint4 *>(x + i * x_row));
 #pragma unroll
-        for (int k = 0; k < NV; ++k) amax = fmaxf(amax, vec_amax<T>(v[k]));
+        for (int k = 0; k < NV; ++k) largest.add(v[k]);
+        float amax = largest.get();
+        if (__any_sync(0xffffffffu, !(amax <= 3.402823466e38f))) {
+            // Infinities: the finite elements alone count.
+            amax = 0.f;
+#pragma unroll 1
+            for (int i = row_first; active && i < n; i += row_step)
+                amax = fmaxf(amax, vec_amax<T>(*reinterpret_cast<const uint4 *>(x + i * x_row)));
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
         if constexpr (WPU > 1) {

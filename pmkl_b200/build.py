@@ -93,7 +93,7 @@ def build_ext(force: bool = False, verbose: bool = False) -> Path:
         *[f"-I{p}" for p in cpp.include_paths()],
         f"-I{sysconfig.get_paths()['include']}", f"-I{cuda_home / 'include'}", f"-I{INCLUDE}",
         str(src),
-        f"-L{torch_lib}", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python",
+        f"-L{torch_lib}", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
         f"-L{LIB_DIR}", "-lpmkl_b200", "-Wl,-rpath,$ORIGIN/../../lib",
         "-o", str(tmp),
     ]

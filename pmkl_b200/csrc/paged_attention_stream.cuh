@@ -470,14 +470,16 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
                (sg.h * group + (real ? rw - i * group : 0)) * p.q_st[1] + t * 16;
     };
     const auto begin_queries = [&](const Segment &sg) {
-        if (!kEarly || warp != 0 || !sa.vec_q) return;
+        if constexpr (kEarly) {
+            if (warp != 0 || !sa.vec_q) return;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const T *q = query_row(sg, n);
+            for (int n = 0; n < NT; ++n) {
+                const T *q = query_row(sg, n);
 #pragma unroll
-            for (int i = 0; i < kQVecs; ++i)
-                q_raw[n][i] = *reinterpret_cast<const uint4 *>(q + i / static_cast<int>(sizeof(T)) * 64 +
-                                                               i % static_cast<int>(sizeof(T)) * (16 / sizeof(T)));
+                for (int i = 0; i < kQVecs; ++i)
+                    q_raw[n][i] = *reinterpret_cast<const uint4 *>(q + i / static_cast<int>(sizeof(T)) * 64 +
+                                                                   i % static_cast<int>(sizeof(T)) * (16 / sizeof(T)));
+            }
         }
     };
 

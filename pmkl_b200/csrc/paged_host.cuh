@@ -12,6 +12,19 @@
 namespace pmkl_b200 {
 namespace {
 
+// SMs of the current device, asked once a device.
+int cached_sm_count() {
+    static std::atomic<int> known[kMaxDevices];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) {
+        cudaGetLastError();
+        return sm_count();
+    }
+    int n = known[dev].load(std::memory_order_relaxed);
+    if (n == 0) known[dev].store(n = sm_count(), std::memory_order_relaxed);
+    return n;
+}
+
 // Calls f with a null pointer of the element type that `dtype` names.
 template <typename F>
 int with_dtype(int dtype, F f) {
@@ -22,7 +35,7 @@ int with_dtype(int dtype, F f) {
 
 unsigned blocks_for(long long units, long long per_block, int blocks_per_sm) {
     const long long need = (units + per_block - 1) / per_block;
-    const long long cap = static_cast<long long>(sm_count()) * blocks_per_sm;
+    const long long cap = static_cast<long long>(cached_sm_count()) * blocks_per_sm;
     return static_cast<unsigned>(need < cap ? need : cap);
 }
 
@@ -64,7 +77,7 @@ template <typename T, int WPU, int NV>
 int launch_append_vec(const paged::AppendArgs &p, cudaStream_t stream) {
     // Tokens a CTA: 32 (two pages of 16 rows, four runs with keys and values),
     // fewer where that would leave SMs without a CTA.
-    const long long share = static_cast<long long>(p.tokens) * p.kv_heads / (4LL * sm_count());
+    const long long share = static_cast<long long>(p.tokens) * p.kv_heads / (4LL * cached_sm_count());
     const int span = static_cast<int>(std::min<long long>(paged::kSpanMax, std::max<long long>(2, share)));
     const long long grid = (static_cast<long long>(p.tokens) + span - 1) / span * p.kv_heads;
     if (grid > 0x7FFFFFFFLL) return PMKL_ERR_INVALID_SHAPE;
@@ -204,7 +217,7 @@ int launch_stream(const paged::AttnArgs &a, void *workspace, cudaStream_t stream
     const long long tiles = std::max<long long>(
         1, (static_cast<long long>(a.max_blocks) * a.block + C::kTileKeys - 1) / C::kTileKeys);
     const long long row_tiles = (static_cast<long long>(a.H / a.Hkv) * a.max_q + C::kRows - 1) / C::kRows;
-    const long long grid = share_grid(static_cast<long long>(sm_count()) * per_sm, paged::kMaxStreamCtas,
+    const long long grid = share_grid(static_cast<long long>(cached_sm_count()) * per_sm, paged::kMaxStreamCtas,
                                       static_cast<long long>(a.batch) * a.Hkv * row_tiles, tiles);
     kernel<<<static_cast<unsigned>(grid), C::kThreads, C::kSmemBytes, stream>>>(p);
     const int rc = launch_status();
@@ -231,13 +244,15 @@ int launch_tile(const paged::AttnArgs &a, void *workspace, cudaStream_t stream) 
     static Occupancy occupancy;
     auto kernel = paged::paged_attention_tile_kernel<T, D>;
     if (!tile_launchable<T, D>()) return PMKL_ERR_UNSUPPORTED;
-    // Tensor memory holds two CTAs an SM.
-    const int per_sm = 2 + 0 * occupancy.get(kernel, paged::kTileThreads, C::kSmemBytes);
-    if (per_sm < 1) return PMKL_ERR_LAUNCH;
+    // Shared memory, registers and tensor memory hold two CTAs an SM (the
+    // occupancy call says one of a kernel that allocates tensor memory; 296 CTAs
+    // were measured to run together).
+    constexpr int per_sm = 2;
+    if (occupancy.get(kernel, paged::kTileThreads, C::kSmemBytes) < 1) return PMKL_ERR_LAUNCH;
     const paged::StreamArgs p = shared_args<T>(a, workspace, paged::kMaxTileCtas, paged::kTileRows, 128);
     const long long tiles = std::max<long long>(1, (static_cast<long long>(a.max_blocks) * a.block + 127) / 128);
     const long long row_tiles = (static_cast<long long>(a.H / a.Hkv) * a.max_q + 127) / 128;
-    const long long grid = share_grid(static_cast<long long>(sm_count()) * per_sm, paged::kMaxTileCtas,
+    const long long grid = share_grid(static_cast<long long>(cached_sm_count()) * per_sm, paged::kMaxTileCtas,
                                       static_cast<long long>(a.batch) * a.Hkv * row_tiles, tiles);
     kernel<<<static_cast<unsigned>(grid), paged::kTileThreads, C::kSmemBytes, stream>>>(p);
     const int rc = launch_status();

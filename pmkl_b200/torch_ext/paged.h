@@ -3,7 +3,24 @@
 // Included by fused_self_attention.cpp.  No reference counterpart.
 #pragma once
 
+#include <ATen/cuda/EmptyTensor.h>
+
 namespace {
+
+// At the small end these calls are bound by what the host does: outputs come
+// straight from the allocator, and several from one allocation.
+at::Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType type, const at::Device &dev) {
+    return at::detail::empty_cuda(sizes, type, dev, c10::nullopt);
+}
+
+// Elements [from, from + n) of a contiguous vector, sharing its memory.
+at::Tensor part_of(const at::Tensor &base, int64_t from, int64_t n) {
+    auto impl = c10::make_intrusive<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(base.storage()),
+                                                     base.key_set(), base.dtype());
+    impl->set_storage_offset(from);
+    impl->set_sizes_contiguous({n});
+    return at::Tensor(std::move(impl));
+}
 
 void check_i32(const at::Tensor &t, const char *name, int64_t dims, const at::Device &dev) {
     TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == dims, name, " must be an int32 tensor of ", dims,
@@ -65,12 +82,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> paged_pla
     TORCH_CHECK(block_size >= 1 && block_size <= INT32_MAX && max_tokens >= 0 && max_tokens <= INT32_MAX,
                 "paged_plan: block_size must be positive and max_tokens not negative");
     const c10::cuda::CUDAGuard guard(dev);
-    // One allocation for the int32 outputs: this call is bound by latency.
-    const auto opts = cached_lens.options();
-    at::Tensor ints = at::empty({3 * batch + 2}, opts);
-    at::Tensor slot_map = at::empty({max_tokens}, opts.dtype(at::kLong));
-    at::Tensor seq_lens = ints.narrow(0, 0, batch), status = ints.narrow(0, batch, batch);
-    at::Tensor starts = ints.narrow(0, 2 * batch, batch + 1), left = ints.narrow(0, 3 * batch + 1, 1);
+    const at::Tensor ints = new_tensor({3 * batch + 2}, at::kInt, dev);
+    at::Tensor slot_map = new_tensor({max_tokens}, at::kLong, dev);
+    at::Tensor seq_lens = part_of(ints, 0, batch), status = part_of(ints, batch, batch);
+    at::Tensor starts = part_of(ints, 2 * batch, batch + 1), left = part_of(ints, 3 * batch + 1, 1);
     cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
     const int rc = pmkl_paged_plan(
         cached_lens.data_ptr<int>(), new_lens.data_ptr<int>(), block_table.data_ptr<int>(),
@@ -139,12 +154,12 @@ std::tuple<at::Tensor, at::Tensor> paged_attention_fw(
     const auto kst = cache_strides(k_cache), vst = cache_strides(v_cache);
     const int T = static_cast<int>(q.size(0)), H = static_cast<int>(q.size(1)), D = static_cast<int>(q.size(2));
     const int Hkv = static_cast<int>(k_cache.size(1)), dt = pmkl_dtype_of(q.scalar_type());
-    at::Tensor out = at::empty(q.sizes(), q.options());
-    at::Tensor lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
+    at::Tensor out = new_tensor(q.sizes(), q.scalar_type(), dev);
+    at::Tensor lse = new_tensor({q.size(0), q.size(1)}, at::kFloat, dev);
     const size_t ws_bytes = pmkl_paged_attention_workspace_size(T, static_cast<int>(batch), H, Hkv, D,
                                                                 static_cast<int>(max_query_len), dt);
     at::Tensor ws;
-    if (ws_bytes > 0) ws = at::empty({static_cast<int64_t>(ws_bytes)}, q.options().dtype(at::kByte));
+    if (ws_bytes > 0) ws = new_tensor({static_cast<int64_t>(ws_bytes)}, at::kByte, dev);
     cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
     const int rc = pmkl_paged_attention(
         qc.data_ptr(), qs, k_cache.data_ptr(), v_cache.data_ptr(), kst.data(), vst.data(), k_scale.data_ptr<float>(),

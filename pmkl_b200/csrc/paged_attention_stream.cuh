@@ -391,6 +391,7 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
     const AttnArgs &p = sa.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int group = p.H / p.Hkv;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     uint2 *const s_q = reinterpret_cast<uint2 *>(s_acc + C::kAccBytes / 4) + lane;  // [part][n][step][lane]
 

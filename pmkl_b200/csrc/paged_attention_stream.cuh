@@ -12,15 +12,19 @@
 //     item.  Each CTA finds its share from the lengths itself.  Items that lie
 //     in one CTA are written at once; the others leave normalised partial rows
 //     and their log-sums in the workspace, joined in the list's order by a
-//     second kernel (no atomics: the same bits on every run).
-//   * A warp takes 16 keys at a time, straight from global memory into the
-//     registers that the tensor cores read, with no shared memory between: a
-//     sum over D may run in any order, so thread (g, t) = (lane / 4, lane % 4)
-//     loads 16 consecutive bytes of keys g and g + 8 and the queries are laid
-//     out to match; and output rows may come in any order, so for V it loads 16
+//     second kernel (no atomics: the same bits on every run).  Two or more
+//     shares a resident CTA balance no better than they cost (B200, 16 x 4096
+//     keys, 32 heads: 99 us with one, 104 with two, 111 with three).
+//   * A warp takes 16 keys at a time, copied asynchronously to shared memory of
+//     its own two tiles ahead (4 KB a tile at head size 128, 64 KB an SM under
+//     way), and reads them as the operands of the tensor cores: a sum over D may
+//     run in any order, so thread (g, t) = (lane / 4, lane % 4) takes 16
+//     consecutive bytes of keys g and g + 8 and the queries are laid out to
+//     match; and output rows may come in any order, so for V it takes 16
 //     consecutive bytes of keys 2t, 2t + 1, 2t + 8, 2t + 9 and pairs up the
 //     bytes of neighbouring keys.  e4m3 values are exact in fp16, which is what
-//     the products take.
+//     the products take.  (Loads into registers instead ran as fast where the
+//     compiler kept them apart and up to 18 % slower where it did not.)
 //   * S^T = K Q^T puts keys in rows and queries in columns; its result is
 //     turned into the operand of O^T = V^T P^T by a transposing matrix move.
 //   * Queries are exact in fp16 too: each row is divided by a power of two that
@@ -30,6 +34,16 @@
 //     rounded to fp16 for the product, and the sum of the softmax takes p' / vs
 //     in fp32.  M is a bound that is raised only when some w passes it by 2^8
 //     (voted per warp), so most tiles reduce nothing across lanes.
+//
+// mma.sync and not tcgen05: 8 to 32 query rows leave most of a 128-row tcgen05
+// tile empty, and the cache's bytes are the bound.  B200, device time: 16 x 4096
+// keys, 32 heads of 128 (538 MB): 99.5 us, 5.41 TB/s (0.82 of the measured copy
+// bandwidth; a CTA's loop over tiles alone runs at 7.6 TB/s, the rest is its
+// start of some 8000 cycles, the change of items and the join); 64 requests of
+// 1..16384 keys, 32/8 heads (939 MB): 184 us, 5.10 TB/s; one request of 131071
+// keys, 32/8 heads (269 MB): 61 us; 8 x 1024 keys, 16 heads of 64: 13.7 us and
+// 2 x 128 keys, 4 heads, fp32: 6.1 us, bound by the latency of what comes before
+// the first key (lengths, share, table, queries) and of the join.
 //
 // Rows behind a request's last key may hold anything: their scores are set to
 // -inf by selection and their values to zero.  A key that some rows see and

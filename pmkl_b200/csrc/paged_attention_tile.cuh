@@ -25,6 +25,16 @@
 // Tensor memory (256 columns a CTA): S [0, 128), O [128, 128 + D); P takes S's
 // upper half: scores 64..127 are held in registers when it is written.
 //
+// What bounds it: each CTA's chain (S 600 cycles, softmax 3300, P V 600, and the
+// hand-overs), some 7000 cycles a tile with two CTAs an SM, against 1024 cycles
+// of tensor work.  B200: chunks of 700..1024 tokens over 3001..8192 keys, 32/8
+// heads of 128 (bf16): 561 us, 530 TFLOP/s (0.32 of the measured bf16 rate); 1..5
+// tokens over 500..8192 keys, 32/4 heads (fp16): 65 us, where the loads' latency
+// is the chain (a half tile of keys and one of values a CTA under way).
+// Tried and not kept: weights against the last reference with a second pass
+// where the maximum passes it (P would wait in registers: spills); one CTA an SM
+// (1098 us against 736 at that step).
+//
 // NaN and rows behind the last key: as in the stream kernel.  Values in tiles
 // at the diagonal are searched for NaN; where there is one, the product gets
 // zeros and the rows that see the key note its columns.

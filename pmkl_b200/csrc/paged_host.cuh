@@ -254,7 +254,6 @@ int launch_tile(const paged::AttnArgs &a, void *workspace, cudaStream_t stream) 
     using C = paged::TileCfg<D>;
     static Occupancy occupancy;
     auto kernel = paged::paged_attention_tile_kernel<T, D>;
-    if (!tile_launchable<T, D>()) return PMKL_ERR_UNSUPPORTED;
     // Shared memory, registers and tensor memory hold two CTAs an SM (the
     // occupancy call says one of a kernel that allocates tensor memory; 296 CTAs
     // were measured to run together).
@@ -271,11 +270,18 @@ int launch_tile(const paged::AttnArgs &a, void *workspace, cudaStream_t stream) 
     return launch_join<T, D, paged::kTileRows>(p, grid, stream);
 }
 
-// The tcgen05 kernel from this many rows a K/V head on (16-bit queries).
-constexpr int kTileMinRows = 17;
+// The tcgen05 kernel from this many rows a K/V head on (16-bit queries).  B200, 16
+// requests of 500..8192 keys, 4 K/V heads of 128: 24 rows 59.8 us streaming, 60.4
+// here; 32 rows 66.8 and 63.0; 64 rows 107 and 75.
+constexpr int kTileMinRows = 25;
 
 int paged_attention_impl(const paged::AttnArgs &p, int dtype, int kernel, void *workspace, cudaStream_t stream) {
-    const bool can_stream = stream_applies(p), can_tile = can_stream && dtype != PMKL_DTYPE_F32;
+    const bool can_stream = stream_applies(p);
+    const bool can_tile =
+        can_stream && (dtype == PMKL_DTYPE_F16
+                           ? (p.D == 64 ? tile_launchable<__half, 64>() : tile_launchable<__half, 128>())
+                           : dtype == PMKL_DTYPE_BF16 && (p.D == 64 ? tile_launchable<__nv_bfloat16, 64>()
+                                                                    : tile_launchable<__nv_bfloat16, 128>()));
     if (kernel == PMKL_PAGED_STREAM && !can_stream) return PMKL_ERR_UNSUPPORTED;
     if (kernel == PMKL_PAGED_TCGEN05 && !can_tile) return PMKL_ERR_UNSUPPORTED;
     if (can_stream && kernel != PMKL_PAGED_SIMT && p.batch > 0 && p.max_q > 0) {
@@ -408,6 +414,9 @@ int pmkl_paged_attention(const void *q, const int64_t *q_strides, const void *k_
     if (heads > 0 && (kv_heads == 0 || heads % kv_heads != 0)) return PMKL_ERR_INVALID_SHAPE;
     if (batch > 1 && table_stride < max_blocks) return PMKL_ERR_INVALID_SHAPE;
     if (!query_starts && tokens != batch) return PMKL_ERR_INVALID_SHAPE;
+    // Rows of a request that share a K/V head are counted in 31 bits.
+    if (heads > 0 && static_cast<long long>(max_query_len) * (heads / kv_heads) > 0x3FFFFFFFLL)
+        return PMKL_ERR_INVALID_SHAPE;
     if (tokens == 0 || heads == 0 || hidden == 0) return PMKL_OK;
     if (hidden > 256) return PMKL_ERR_UNSUPPORTED;
     if (!q || !o) return PMKL_ERR_NULL_POINTER;

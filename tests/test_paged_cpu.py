@@ -58,6 +58,7 @@ def test_attention_argument_errors():
     assert attend(stride=3) == -1
     assert attend(tokens=3, starts=None) == -1  # one token a request
     assert attend(block=0) == -1
+    assert attend(max_q=0x7FFFFFFF, heads=8, kv=1) == -1  # rows of a K/V head past 31 bits
     assert attend(dtype=5) == -2
     assert attend(kernel=77) == -5
     assert attend(hidden=257) == -5

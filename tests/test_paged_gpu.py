@@ -393,6 +393,50 @@ def test_attention_nan_in_later_tokens(kernel, dtype, D):
     assert torch.equal(out.isnan().cpu(), want) and torch.equal(lse.isnan().cpu(), want[:, :, 0])
 
 
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_attention_keys_and_values_in_different_layouts(kernel):
+    prob = list(problem([70, 200], [2, 1], 4, 2, 64, 16, F16, seed=13))
+    prob[1] = prob[1].transpose(1, 2).contiguous().transpose(1, 2)  # keys: rows outside the heads
+    big = torch.zeros(prob[2].shape[0], 2, 16, 2 * 64, dtype=torch.uint8)  # values: every other 64 bytes of a row
+    big[..., 64:] = prob[2].view(torch.uint8)
+    prob[2] = big.view(torch.float8_e4m3fn)[..., 64:]
+    check(tuple(prob), kernel=kernel)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("D,rows_first", [(128, False), (64, True)])
+def test_cache_past_32_bit_offsets(kernel, D, rows_first):
+    """Pages whose bytes lie past 2^32: written by paged_append and read back by the attention, against a small cache."""
+    Hkv, block = 4, 64
+    pages = (9 << 29) // (Hkv * block * D)  # 4.5 GiB
+    shape = (pages, block, Hkv, D) if rows_first else (pages, Hkv, block, D)
+    cache = torch.empty(shape, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    cache = cache.transpose(1, 2) if rows_first else cache
+    scale = torch.ones(pages, Hkv, device="cuda")
+    x = values((150, Hkv, D), BF16, 14)
+    far = [pages - 1, 3, pages - 2]
+    slots = torch.tensor([p * block + i for p in far for i in range(block)][:150], device="cuda")
+    paged_append(x, x, slots, cache, cache, scale, scale)  # keys and values share one cache here
+    near, near_scale = torch.zeros(3, Hkv, block, D, device="cuda").to(torch.float8_e4m3fn), torch.ones(3, Hkv, device="cuda")
+    paged_append(x, x, torch.arange(150, device="cuda"), near, near, near_scale, near_scale)
+    q = values((2, 8, D), BF16, 15)
+    a = pmkl_pytorch_ext.paged_attention_fw(q, cache, cache, scale, scale, i32([far]), i32([150]), i32([0, 2]), 2, True, 0.0, kernel)
+    b = pmkl_pytorch_ext.paged_attention_fw(q, near, near, near_scale, near_scale, i32([[0, 1, 2]]), i32([150]), i32([0, 2]), 2,
+                                            True, 0.0, kernel)
+    for got, want in zip(a, b):
+        assert torch.equal(got, want) and got.isfinite().all()
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_many_requests(kernel, dtype):
+    """More requests than a CTA has threads, most of them short, some empty."""
+    r = random.Random(16)
+    lens = [r.choice([0, 1, 5, 16, 40]) for _ in range(600)] + [700]
+    news = [r.choice([0, 1, 1, 2]) for _ in lens]
+    check(problem(lens, news, 2, 1, 64, 16, dtype, seed=17), kernel=kernel)
+
+
 # ---------------------------------------------------------------- refusals
 def test_refusals():
     q, kc, vc, ks, vs, table, lens, starts = problem([20], [1], 4, 2, 64, 16, F16, seed=8)
@@ -432,3 +476,14 @@ def test_refusals():
     for bad in ((i32([1]), i32([1, 2]), 16, 8), (i32([1]), i32([1]), 0, 8), (i32([1]), i32([1]), 16, -1), (n.long(), n, 16, 8)):
         with pytest.raises(RuntimeError):
             paged_plan(bad[0], bad[1], t, i32([1]), i32([1]), bad[2], bad[3])
+
+
+def test_example_runs():
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    example = Path(__file__).resolve().parent.parent / "examples" / "paged_decode.py"
+    out = subprocess.run([sys.executable, str(example), "--steps", "12", "--check"], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0, out.stdout + out.stderr
+    assert "12 steps" in out.stdout

@@ -472,30 +472,23 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
         if (key + 2 * kTileKeys < key_end) ahead = look_up();
     };
 
-    // Query rows of a segment as they are in memory: warp 0 loads them with the
-    // segment's first keys, where one row tile's fit the registers (rows of 16-byte
-    // vectors; others are read when laid out).
+    // Query rows: warp n lays the n-th 8 out; it loads them as they are in memory
+    // with the segment's first keys (rows of 16-byte vectors; others when laid out).
     constexpr int kQVecs = kHalves * sizeof(T);
-    constexpr bool kEarly = NT == 1;
-    uint4 q_raw[NT][kQVecs];
-    const auto query_row = [&](const Segment &sg, int n) -> const T * {
-        const bool real = n * 8 + g < sg.n_rows;
-        const int rw = sg.row0 + n * 8 + g, i = rw / group;
+    uint4 q_raw[kQVecs];
+    const auto query_row = [&](const Segment &sg) -> const T * {
+        const bool real = warp * 8 + g < sg.n_rows;
+        const int rw = sg.row0 + warp * 8 + g, i = rw / group;
         return static_cast<const T *>(p.q) + (sg.r.first + (real ? i : 0)) * p.q_st[0] +
                (sg.h * group + (real ? rw - i * group : 0)) * p.q_st[1] + t * 16;
     };
     const auto begin_queries = [&](const Segment &sg) {
-        if constexpr (kEarly) {
-            if (warp != 0 || !sa.vec_q) return;
+        if (warp >= NT || !sa.vec_q) return;
+        const T *q = query_row(sg);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const T *q = query_row(sg, n);
-#pragma unroll
-                for (int i = 0; i < kQVecs; ++i)
-                    q_raw[n][i] = *reinterpret_cast<const uint4 *>(q + i / static_cast<int>(sizeof(T)) * 64 +
-                                                                   i % static_cast<int>(sizeof(T)) * (16 / sizeof(T)));
-            }
-        }
+        for (int i = 0; i < kQVecs; ++i)
+            q_raw[i] = *reinterpret_cast<const uint4 *>(q + i / static_cast<int>(sizeof(T)) * 64 +
+                                                        i % static_cast<int>(sizeof(T)) * (16 / sizeof(T)));
     };
 
     if (s_more[0]) {
@@ -504,23 +497,20 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
     }
     for (int turn = 0; s_more[turn]; turn ^= 1) {
         const Segment &sg = s_segs[turn];
-        // ---- the last warp walks on, the first lays the queries out as operands of S^T
-        if (tid == kStreamThreads - 32) s_more[turn ^ 1] = next_segment<C::kRows, kTileKeys, C::kItemCost>(p, s_share, s_segs[turn ^ 1]);
-        if (warp == 0) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
+        // ---- the last warp walks on, the first ones lay the queries out as operands of S^T
+        if (tid == kStreamThreads - 32)
+            s_more[turn ^ 1] = next_segment<C::kRows, kTileKeys, C::kItemCost>(p, s_share, s_segs[turn ^ 1]);
+        if (warp < NT) {
+            const int n = warp;
+            {
                 const bool real = n * 8 + g < sg.n_rows;
                 float x[kHalves][16];
-                if (!kEarly) {
-                    const T *q = query_row(sg, n);
-#pragma unroll
-                    for (int hf = 0; hf < kHalves; ++hf) load_q16(x[hf], q + hf * 64, sa.vec_q != 0);
-                } else if (sa.vec_q) {
-                    const T *y = reinterpret_cast<const T *>(q_raw[n]);
+                if (sa.vec_q) {
+                    const T *y = reinterpret_cast<const T *>(q_raw);
 #pragma unroll
                     for (int j = 0; j < kHalves * 16; ++j) x[j >> 4][j & 15] = Elem<T>::to_float(y[j]);
                 } else {
-                    const T *q = query_row(sg, n);
+                    const T *q = query_row(sg);
 #pragma unroll
                     for (int j = 0; j < kHalves * 16; ++j)
                         x[j >> 4][j & 15] = Elem<T>::to_float(q[(j >> 4) * 64 + (j & 15)]);
@@ -825,67 +815,53 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
 }
 
 // Joins the partial rows of the item that CTA blockIdx.x of the kernel before
-// began and did not end: rows blockIdx.y, blockIdx.y + gridDim.y, ... of its
-// row tile, a thread a column, the segments shared out over groups of D threads.
+// began and did not end: a warp a row, each lane D / 32 neighbouring columns.
 constexpr int kJoinThreads = 256;
 
 template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(const __grid_constant__ StreamArgs sa) {
-    constexpr int kGroups = kJoinThreads / D, kWarps = kJoinThreads / 32;
-    __shared__ float s_w[kMaxStreamCtas], s_top[kWarps], s_sum[kWarps], s_x[kGroups][D];
+    constexpr int kCols = D / 32;
     const AttnArgs &p = sa.a;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, d = tid % D, part = tid / D;
-    const int group = p.H / p.Hkv;
+    const int lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int n = sa.desc[blockIdx.x].segments;
-    if (n == 0) return;
     const StreamDesc desc = sa.desc[blockIdx.x];
-    const auto slot = [&](int i) { return i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i); };
-    for (int rw = blockIdx.y; rw < desc.n_rows; rw += gridDim.y) {
-        float top = -INFINITY;
-        for (int i = tid; i < n; i += kJoinThreads) {
-            const float x = sa.part_lse[slot(i) * ROWS + rw];
-            s_w[i] = x;
-            top = fmaxf(top, x);
+    const int n = desc.segments, rw = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5);
+    if (n == 0 || rw >= desc.n_rows) return;
+    // Part i lies in slot 2c + 1 of the CTA that began the item (i = 0), in slot 2c of those after it.
+    const auto slot = [&](int i) { return i == 0 ? 2 * static_cast<int>(blockIdx.x) + 1 : 2 * (static_cast<int>(blockIdx.x) + i); };
+    float top = -INFINITY;
+    for (int i = lane; i < n; i += 32) top = fmaxf(top, sa.part_lse[slot(i) * ROWS + rw]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, x[kCols] = {};
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        const float w = i0 + lane < n ? exp2_fast(sa.part_lse[slot(i0 + lane) * ROWS + rw] - base) : 0.f;
+        sum += w;
+        const int here = min(32, n - i0);
+#pragma unroll 8
+        for (int i = 0; i < here; ++i) {
+            const float wi = __shfl_sync(0xffffffffu, w, i);
+            const float *from = sa.part_o + (static_cast<long long>(slot(i0 + i)) * ROWS + rw) * D + lane * kCols;
+            if constexpr (kCols == 4) {
+                const float4 v = *reinterpret_cast<const float4 *>(from);
+                x[0] = fmaf(wi, v.x, x[0]), x[1] = fmaf(wi, v.y, x[1]), x[2] = fmaf(wi, v.z, x[2]), x[3] = fmaf(wi, v.w, x[3]);
+            } else {
+                const float2 v = *reinterpret_cast<const float2 *>(from);
+                x[0] = fmaf(wi, v.x, x[0]), x[1] = fmaf(wi, v.y, x[1]);
+            }
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (lane == 0) s_top[warp] = top;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_top[w]);
-        const float base = top == -INFINITY ? 0.f : top;
-        float sum = 0.f;
-        for (int i = tid; i < n; i += kJoinThreads) {
-            const float w = exp2_fast(s_w[i] - base);
-            s_w[i] = w;
-            sum += w;
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) s_sum[warp] = sum;
-        __syncthreads();
-        sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) sum += s_sum[w];
-        float x = 0.f;
-#pragma unroll 16
-        for (int i = part; i < n; i += kGroups)
-            x = fmaf(s_w[i], sa.part_o[(static_cast<long long>(slot(i)) * ROWS + rw) * D + d], x);
-        s_x[part][d] = x;
-        __syncthreads();
-        if (part == 0) {
-#pragma unroll
-            for (int k = 1; k < kGroups; ++k) x += s_x[k][d];
-            x *= sum == 0.f ? 0.f : 1.f / sum;
-            const int row = desc.row0 + rw, tok = row / group, head = desc.h * group + row - tok * group;
-            const long long token = desc.first + tok;
-            static_cast<T *>(p.o)[token * p.o_st[0] + head * p.o_st[1] + d] = Elem<T>::from_float(x);
-            if (p.lse && d == 0)
-                p.lse[token * p.H + head] = sum == 0.f ? -INFINITY : (base + log2f(sum)) * 0.6931471805599453f;
-        }
-        __syncthreads();  // the row's values have been read
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int group = p.H / p.Hkv, row = desc.row0 + rw, tok = row / group, head = desc.h * group + row - tok * group;
+    const long long token = desc.first + tok;
+    T *o = static_cast<T *>(p.o) + token * p.o_st[0] + head * p.o_st[1] + lane * kCols;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) o[c] = Elem<T>::from_float(x[c] * inv);
+    if (p.lse && lane == 0)
+        p.lse[token * p.H + head] = sum == 0.f ? -INFINITY : (base + log2f(sum)) * 0.6931471805599453f;
 }
 
 }  // namespace paged

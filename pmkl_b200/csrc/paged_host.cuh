@@ -194,7 +194,7 @@ template <typename T, int D, int ROWS>
 int launch_join(const paged::StreamArgs &p, long long grid, cudaStream_t stream) {
     const long long rows = std::min<long long>(ROWS, static_cast<long long>(p.a.H / p.a.Hkv) * p.a.max_q);
     return launch_early(paged::paged_attention_join_kernel<T, D, ROWS>,
-                        dim3(static_cast<unsigned>(grid), static_cast<unsigned>(std::min<long long>(rows, 16))),
+                        dim3(static_cast<unsigned>(grid), static_cast<unsigned>((rows + 7) / 8)),  // a warp a row
                         paged::kJoinThreads, 0, p, stream);
 }
 

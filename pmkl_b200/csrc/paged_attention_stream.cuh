@@ -37,12 +37,12 @@
 //
 // mma.sync and not tcgen05: 8 to 32 query rows leave most of a 128-row tcgen05
 // tile empty, and the cache's bytes are the bound.  B200, device time: 16 x 4096
-// keys, 32 heads of 128 (538 MB): 99.5 us, 5.41 TB/s (0.82 of the measured copy
+// keys, 32 heads of 128 (538 MB): 101 us, 5.33 TB/s (0.81 of the measured copy
 // bandwidth; a CTA's loop over tiles alone runs at 7.6 TB/s, the rest is its
 // start of some 8000 cycles, the change of items and the join); 64 requests of
-// 1..16384 keys, 32/8 heads (939 MB): 184 us, 5.10 TB/s; one request of 131071
-// keys, 32/8 heads (269 MB): 61 us; 8 x 1024 keys, 16 heads of 64: 13.7 us and
-// 2 x 128 keys, 4 heads, fp32: 6.1 us, bound by the latency of what comes before
+// 1..16384 keys, 32/8 heads (939 MB): 188 us, 5.0 TB/s; one request of 131071
+// keys, 32/8 heads (269 MB): 62 us; 8 x 1024 keys, 16 heads of 64: 13.7 us and
+// 2 x 128 keys, 4 heads, fp32: 6.2 us, bound by the latency of what comes before
 // the first key (lengths, share, table, queries) and of the join.
 //
 // Rows behind a request's last key may hold anything: their scores are set to

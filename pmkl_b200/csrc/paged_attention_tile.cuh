@@ -26,11 +26,12 @@
 // upper half: scores 64..127 are held in registers when it is written.
 //
 // What bounds it: each CTA's chain (S 600 cycles, softmax 3300, P V 600, and the
-// hand-overs), some 7000 cycles a tile with two CTAs an SM, against 1024 cycles
-// of tensor work.  B200: chunks of 700..1024 tokens over 3001..8192 keys, 32/8
-// heads of 128 (bf16): 561 us, 530 TFLOP/s (0.32 of the measured bf16 rate); 1..5
-// tokens over 500..8192 keys, 32/4 heads (fp16): 65 us, where the loads' latency
-// is the chain (a half tile of keys and one of values a CTA under way).
+// hand-overs), some 6000 cycles a tile with two CTAs an SM, against 1024 cycles
+// of tensor work.  B200, device time: chunks of 700..1024 tokens over 3001..8192
+// keys, 32/8 heads of 128 (bf16): 481 us, 618 TFLOP/s (0.38 of the measured bf16
+// rate); 1..5 tokens over 500..8192 keys, 32/4 heads (fp16): 53 us, where the
+// loads' latency is the chain (a half tile of keys and one of values a CTA under
+// way).
 // Tried and not kept: weights against the last reference with a second pass
 // where the maximum passes it (P would wait in registers: spills); one CTA an SM
 // (1098 us against 736 at that step).
@@ -50,8 +51,10 @@ constexpr int kTileRows = 128;
 constexpr int kTileThreads = 384;
 constexpr int kTileItemCost = 1;  // of an item, in tiles: some 8000 cycles against 7000
 // Registers a thread: at launch, and what each warpgroup sets; the three come
-// to the launch's total (the host checks that the build has it).
-constexpr int kTileLaunchRegs = 80, kTileSoftmaxRegs = 120, kTileLoadRegs = 72, kTileIssueRegs = 48;
+// to the launch's total (the host checks that the build has it).  B200, chunk
+// workload above: 120/64/56 and 120/72/48 481 us, 112/72/56 492, 128/72/40 564,
+// 128/80/32 653; 16 x 1..5 tokens: 52.7, 54.4, 55.2, 62, 68.5.
+constexpr int kTileLaunchRegs = 80, kTileSoftmaxRegs = 120, kTileLoadRegs = 64, kTileIssueRegs = 56;
 static_assert(kTileSoftmaxRegs + kTileLoadRegs + kTileIssueRegs == 3 * kTileLaunchRegs, "register split");
 constexpr int kMaxTileCtas = 320;  // partials in the workspace: 148 SMs with 2 CTAs
 

@@ -271,9 +271,11 @@ int launch_tile(const paged::AttnArgs &a, void *workspace, cudaStream_t stream) 
 }
 
 // The tcgen05 kernel from this many rows a K/V head on (16-bit queries).  B200, 16
-// requests of 500..8192 keys, 4 K/V heads of 128: 24 rows 59.8 us streaming, 60.4
-// here; 32 rows 66.8 and 63.0; 64 rows 107 and 75.
-constexpr int kTileMinRows = 25;
+// requests of 500..8192 keys, 4 K/V heads of 128: 32 rows 47.8 us streaming, 53.8
+// here; 40 rows (a second row tile, which reads the keys again) 70.5 and 57.8; 64
+// rows 76 and 60.  One request of 131071 keys: 32 rows 58.0 and 68.1, 40 rows
+// 90 and 71.5; head size 64, the 16 requests: 34.1 and 38.7, 52.3 and 42.8.
+constexpr int kTileMinRows = 33;
 
 int paged_attention_impl(const paged::AttnArgs &p, int dtype, int kernel, void *workspace, cudaStream_t stream) {
     const bool can_stream = stream_applies(p);

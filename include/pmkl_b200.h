@@ -399,7 +399,7 @@ int pmkl_paged_attention(const void *q, const int64_t *q_strides, const void *k_
                          void *workspace, size_t workspace_bytes, int kernel, void *stream);
 
 /* Workspace bytes of pmkl_paged_attention for these sizes (0 for an empty
- * problem).  Host only. */
+ * problem; max_query_len 0 counts as 1).  Host only. */
 size_t pmkl_paged_attention_workspace_size(int tokens, int batch, int heads, int kv_heads, int hidden,
                                            int max_query_len, int dtype);
 

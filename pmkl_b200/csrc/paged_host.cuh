@@ -387,9 +387,11 @@ int pmkl_paged_append(const void *k, const void *v, const int64_t *k_new_strides
 
 size_t pmkl_paged_attention_workspace_size(int tokens, int batch, int heads, int kv_heads, int hidden,
                                            int max_query_len, int dtype) {
-    if (tokens <= 0 || batch <= 0 || heads <= 0 || kv_heads <= 0 || hidden <= 0 || max_query_len <= 0 ||
+    if (tokens <= 0 || batch <= 0 || heads <= 0 || kv_heads <= 0 || hidden <= 0 || max_query_len < 0 ||
         heads % kv_heads != 0 || !dtype_valid(dtype))
         return 0;
+    // 0 as well as 1: one token a request where no query_starts are given, whatever the limit says.
+    if (max_query_len == 0) max_query_len = 1;
     if (hidden != 64 && hidden != 128) return 0;  // the CUDA-core kernel needs none
     // What the largest of the kernels that may be asked for needs.
     const size_t stream =
@@ -416,6 +418,8 @@ int pmkl_paged_attention(const void *q, const int64_t *q_strides, const void *k_
     if (heads > 0 && (kv_heads == 0 || heads % kv_heads != 0)) return PMKL_ERR_INVALID_SHAPE;
     if (batch > 1 && table_stride < max_blocks) return PMKL_ERR_INVALID_SHAPE;
     if (!query_starts && tokens != batch) return PMKL_ERR_INVALID_SHAPE;
+    // One value for the sizes, the workspace and the launch.
+    if (!query_starts) max_query_len = 1;
     // Rows of a request that share a K/V head are counted in 31 bits.
     if (heads > 0 && static_cast<long long>(max_query_len) * (heads / kv_heads) > 0x3FFFFFFFLL)
         return PMKL_ERR_INVALID_SHAPE;
@@ -454,7 +458,7 @@ int pmkl_paged_attention(const void *q, const int64_t *q_strides, const void *k_
     p.num_blocks = num_blocks;
     p.block = block_size;
     p.max_blocks = max_blocks;
-    p.max_q = query_starts ? max_query_len : 1;
+    p.max_q = max_query_len;
     p.causal = is_causal ? 1 : 0;
     p.scale = scale > 0.f ? scale : 1.0f / sqrtf(static_cast<float>(hidden));
     return paged_attention_impl(p, dtype, kernel, workspace, static_cast<cudaStream_t>(stream));

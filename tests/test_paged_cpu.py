@@ -74,6 +74,21 @@ def test_workspace_size_is_zero_for_empty_or_bad_sizes():
     assert f(2, 2, 4, 2, 64, 1, 2) % 256 == 0
 
 
+@pytest.mark.parametrize("hidden", [64, 128])
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_workspace_is_asked_for_whatever_max_query_len(hidden, dtype):
+    """Without query_starts a request has one token, and the workspace of one, also where max_query_len says 0."""
+    f = pmkl_b200.capi().pmkl_paged_attention_workspace_size
+    need = f(2, 2, 4, 2, hidden, 1, dtype)
+    assert need > 0 and f(2, 2, 4, 2, hidden, 0, dtype) == need
+    for max_q in (0, 1):
+        for starts in (None, FAKE):
+            assert attend(hidden=hidden, dtype=dtype, max_q=max_q, starts=starts, ws=None, ws_bytes=0) == -3
+            assert attend(hidden=hidden, dtype=dtype, max_q=max_q, starts=starts, ws_bytes=need - 1) == -9
+    # an upper limit far above the one token is no reason to refuse
+    assert attend(hidden=hidden, dtype=dtype, heads=8, kv=1, max_q=0x7FFFFFFF, starts=None, ws=None) == -3
+
+
 def test_binding_refuses_cpu_tensors():
     from pmkl_function import paged_append, paged_attention, paged_plan
 

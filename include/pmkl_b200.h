@@ -387,7 +387,8 @@ int pmkl_paged_append(const void *k, const void *v, const int64_t *k_new_strides
  * A row that sees no key gets o = 0 and lse = -inf, and so do rows of q past
  * query_starts[batch].  Rows of a page behind seq_len may hold anything, NaN
  * included.  Scales are positive; the scale of a page of values outside
- * 2^-64 .. 2^64 counts as the nearer of the two.  Scores, softmax and sums
+ * 2^-64 .. 2^64 counts as the nearer of the two, one of a page of keys below
+ * 2^-64 as 2^-64.  Scores, softmax and sums
  * are fp32, o is rounded once.
  */
 int pmkl_paged_attention(const void *q, const int64_t *q_strides, const void *k_cache, const void *v_cache,

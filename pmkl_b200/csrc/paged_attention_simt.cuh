@@ -75,6 +75,24 @@ __device__ __forceinline__ float value_scale(float s) {
     return fminf(fmaxf(s, 5.421010862427522e-20f), 1.8446744073709552e19f);  // 2^-64, 2^64
 }
 
+// The scale of a page of keys: no smaller than what paged_append writes, so that
+// its product with a row's factor is not 0 (below).
+__device__ __forceinline__ float key_scale(float s) {
+    return s < 5.421010862427522e-20f ? 5.421010862427522e-20f : s;  // 2^-64; NaN stays
+}
+
+// Query rows are held in fp16 over a power of two 2^e, and a score is the raw
+// product times the row's factor (2^e * c, c the score scale in log2 units) and
+// the page's key scale.  Returns the e that brings the row's largest value to
+// 2^7 .. 2^8, or, for rows so small (0 among them) that the factor would fall below 2^-85, the e
+// that keeps it there: times a key scale it is then never 0 in fp32, and -inf
+// in masked places stays -inf.  Such a row loses 2^-25 * 2^-85 of its values,
+// 2^-30 in a score over the largest keys.
+__device__ __forceinline__ int query_exponent(float amax, float c) {
+    const int least = max(-100, 127 - 85 - static_cast<int>(__float_as_uint(c) >> 23));
+    return min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127 - 7, least), 126);
+}
+
 // The rare path of the kernels whose products would spread a NaN value as 0 *
 // NaN: sets in `cols` (a bit a column) the columns that hold NaN in the rows
 // [key, end) of request row `table`, K/V head h.
@@ -138,7 +156,7 @@ __global__ void __launch_bounds__(kSimtThreads) paged_attention_simt_kernel(cons
                     float dot = 0.f;
                     for (int d = 0; d < p.D; ++d) dot = fmaf(qs[d], e4m3_to_float(k[d]), dot);
                     const long long at = static_cast<long long>(page) * p.Hkv + hk;
-                    s = dot * p.k.scale[at];
+                    s = dot * key_scale(p.k.scale[at]);
                     vs = value_scale(p.v.scale[at]);
                     vrow = page * p.v.s[0] + hk * p.v.s[1] + row * p.v.s[2];
                 }

@@ -524,8 +524,8 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
                 }
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                // The power of two that brings the row's largest value to 2^7 .. 2^8.
-                const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127 - 7, -100), 126);
+                const float c = p.scale * 1.4426950408889634f;
+                const int e = query_exponent(amax, c);
                 const float down = exp2_int(-e);
 #pragma unroll
                 for (int s = 0; s < kSteps; ++s) {
@@ -542,7 +542,7 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
                     }
                 }
                 if (t == 0) {
-                    s_qscale[n * 8 + g] = exp2_int(e) * p.scale * 1.4426950408889634f;
+                    s_qscale[n * 8 + g] = exp2_int(e) * c;
                     s_lim[n * 8 + g] = real ? visible(p, sg.r, (sg.row0 + n * 8 + g) / group) : sg.r.keys;
                 }
             }
@@ -590,7 +590,7 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
                     }
                 }
                 const uint2 scales = shared8(at + 32 * D);
-                const float ks = __uint_as_float(scales.x), vs = __uint_as_float(scales.y);
+                const float ks = key_scale(__uint_as_float(scales.x)), vs = __uint_as_float(scales.y);
                 const float vs_ok = value_scale(vs);
                 const float lv = log2_fast(vs_ok), inv_vs = rcp_fast(vs_ok);
                 const bool edge = key + 16 > lim_min;

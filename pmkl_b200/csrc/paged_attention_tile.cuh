@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                         from = reinterpret_cast<unsigned long long>(cache.base) + x * cache.s[0] + h * cache.s[1] +
                                row * cache.s[2];
                         const long long at = static_cast<long long>(x) * p.Hkv + h;
-                        ks = __ldg(p.k.scale + at);
+                        ks = key_scale(__ldg(p.k.scale + at));
                         vs = value_scale(__ldg(p.v.scale + at));
                     }
                     const int i = it % kAhead;
@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
             const bool real = tid < s.n_rows;
             const int tok = real ? rr / group : 0, head = s.h * group + (real ? rr - tok * group : 0);
             const T *q = static_cast<const T *>(p.q) + (s.r.first + tok) * p.q_st[0] + head * p.q_st[1];
-            // The row's largest value, then the row over the power of two that brings it to 2^7 .. 2^8.
+            // The row's largest value, then the row over its power of two.
             float amax = 0.f;
             if (real)
 #pragma unroll 1
@@ -400,8 +400,9 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
 #pragma unroll
                     for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(x[i]));
                 }
-            const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127 - 7, -100), 126);
-            const float down = exp2_int(-e), up = exp2_int(e) * p.scale * 1.4426950408889634f;
+            const float log2_scale = p.scale * 1.4426950408889634f;
+            const int e = query_exponent(amax, log2_scale);
+            const float down = exp2_int(-e), up = exp2_int(e) * log2_scale;
 #pragma unroll 1
             for (int c = 0; c < D; c += 16) {
                 float x[16];

@@ -460,7 +460,8 @@ int pmkl_paged_attention(const void *q, const int64_t *q_strides, const void *k_
     p.max_blocks = max_blocks;
     p.max_q = max_query_len;
     p.causal = is_causal ? 1 : 0;
-    p.scale = scale > 0.f ? scale : 1.0f / sqrtf(static_cast<float>(hidden));
+    // (below the normal numbers a score scale is as good as the smallest of them)
+    p.scale = scale > 0.f ? fmaxf(scale, 1.17549435e-38f) : 1.0f / sqrtf(static_cast<float>(hidden));
     return paged_attention_impl(p, dtype, kernel, workspace, static_cast<cudaStream_t>(stream));
 }
 

@@ -437,6 +437,43 @@ def test_attention_many_requests(kernel, dtype):
     check(problem(lens, news, 2, 1, 64, 16, dtype, seed=17), kernel=kernel)
 
 
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("H,Hkv,D", [(4, 2, 64), (4, 1, 128)])
+def test_attention_zero_queries_over_zero_keys(kernel, dtype, H, Hkv, D):
+    """Zero keys, appended (their pages get the smallest scale), under zero and other queries: the mean of the values."""
+    block, lens, news = 16, [1, 17, 129, 160, 40], [1, 1, 1, 5, 40]
+    width = max(-(-n // block) for n in lens)
+    table, slots, pages = [], [], 0
+    for n in lens:
+        k = -(-n // block)
+        table.append([pages + j for j in range(k)] + [-1] * (width - k))
+        slots += [pages * block + i for i in range(n)]
+        pages += k
+    kc, vc = (torch.zeros(pages, Hkv, block, D, device="cuda").to(torch.float8_e4m3fn) for _ in range(2))
+    ks, vs = torch.ones(pages, Hkv, device="cuda"), torch.ones(pages, Hkv, device="cuda")
+    paged_append(torch.zeros(len(slots), Hkv, D, device="cuda", dtype=dtype), values((len(slots), Hkv, D), dtype, 20),
+                 torch.tensor(slots, device="cuda"), kc, vc, ks, vs)
+    assert (ks == 2.0 ** -64).all()
+    starts = [0]
+    for n in news:
+        starts.append(starts[-1] + n)
+    q = torch.zeros(starts[-1], H, D, dtype=dtype)
+    q[:, 1] = values((starts[-1], D), dtype, 21).cpu()
+    check((q, kc.cpu(), vc.cpu(), ks.cpu(), vs.cpu(), table, lens, starts), kernel=kernel)
+    check((q, kc.cpu(), vc.cpu(), ks.cpu(), vs.cpu(), table, lens, starts), kernel=kernel, scale=1e-30)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_small_queries_over_large_keys(kernel, dtype):
+    """Queries near 2^-66 over keys near 2^66, near 2^50 over 2^-50: ordinary scores; keys of scale 0 are keys of 0."""
+    q, kc, vc, ks, vs, table, lens, starts = problem([700, 90], [1, 5], 4, 2, 128, 16, dtype, seed=26)
+    check((q * 2.0 ** -66, kc, vc, ks * 2.0 ** 66, vs, table, lens, starts), kernel=kernel)
+    check((q * 2.0 ** 50, kc, vc, ks * 2.0 ** -50, vs, table, lens, starts), kernel=kernel)
+    check((q, kc, vc, torch.where(ks.isnan(), ks, 0.0), vs, table, lens, starts), kernel=kernel)
+
+
 # ---------------------------------------------------------------- refusals
 def test_refusals():
     q, kc, vc, ks, vs, table, lens, starts = problem([20], [1], 4, 2, 64, 16, F16, seed=8)

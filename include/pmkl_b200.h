@@ -388,8 +388,14 @@ int pmkl_paged_append(const void *k, const void *v, const int64_t *k_new_strides
  * query_starts[batch].  Rows of a page behind seq_len may hold anything, NaN
  * included.  Scales are positive; the scale of a page of values outside
  * 2^-64 .. 2^64 counts as the nearer of the two, one of a page of keys below
- * 2^-64 as 2^-64.  Scores, softmax and sums
- * are fp32, o is rounded once.
+ * 2^-64 as 2^-64.
+ *
+ * Scores, their exponentials and all sums are fp32, o is rounded once.  On the
+ * tensor cores (hidden 64 and 128) queries and weights are operands in fp16:
+ * 16-bit queries lose at most 2^-32 of their row's largest value, weights 2^-11
+ * of themselves or 2^-32 of the row's largest, whichever is more.  fp32 queries
+ * and their weights go in two parts: 2^-22 of themselves, or 2^-32 of the
+ * largest query value and 2^-38 of the largest weight.
  */
 int pmkl_paged_attention(const void *q, const int64_t *q_strides, const void *k_cache, const void *v_cache,
                          const int64_t *k_strides, const int64_t *v_strides, const float *k_scale,

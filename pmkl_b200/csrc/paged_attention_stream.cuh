@@ -27,13 +27,17 @@
 //     compiler kept them apart and up to 18 % slower where it did not.)
 //   * S^T = K Q^T puts keys in rows and queries in columns; its result is
 //     turned into the operand of O^T = V^T P^T by a transposing matrix move.
-//   * Queries are exact in fp16 too: each row is divided by a power of two that
-//     brings its largest value near 2^7 (16-bit types); fp32 queries and
-//     weights are split in two fp16 parts.
+//   * 16-bit queries go to fp16 over a power of two that brings the row's largest
+//     value near 2^7: exact but for what lies below 2^-32 of it.  fp32 queries
+//     and weights are split in two fp16 parts (2^-22 of themselves).
 //   * A page's value scale enters the exponent: w = s + log2 vs, p' = 2^(w - M)
 //     rounded to fp16 for the product, and the sum of the softmax takes p' / vs
-//     in fp32.  M is a bound that is raised only when some w passes it by 2^8
-//     (voted per warp), so most tiles reduce nothing across lanes.
+//     in fp32.  M is such that weights go up to 2^15, so that small ones keep what
+//     fp16 has below: it is raised only when some w would pass that, to where the
+//     largest is 2^7 (voted per warp), so most tiles reduce nothing across lanes.
+//     What a weight may lose beside 2^-11 of itself is then 2^-32 of the largest.
+//     fp32 queries raise M to where the largest weight is 2^13: 2^-22 of a weight
+//     or 2^-38 of the largest.
 //
 // mma.sync and not tcgen05: 8 to 32 query rows leave most of a 128-row tcgen05
 // tile empty, and the cache's bytes are the bound.  B200, device time: 16 x 4096
@@ -114,6 +118,12 @@ __device__ __forceinline__ float2 h2_floats(uint32_t v) { return __half22float2(
 // A running maximum before its first score: far below all, and finite, so that
 // differences with it are numbers.
 constexpr float kNoMax = -1e30f;
+
+// Weights are 2^(w - M) up to 2^kTopExp, where fp16 ends; M is raised to where the
+// largest is 2^lift.
+constexpr float kTopExp = 15.f;
+template <typename T>
+constexpr float kLift = sizeof(T) == 4 ? 13.f : 7.f;
 
 __device__ __forceinline__ float rcp_fast(float x) {
     float y;
@@ -621,7 +631,7 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
                 exponents();
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
-                    raise = raise || fmaxf(fmaxf(z[n][0], z[n][1]), fmaxf(z[n][2], z[n][3])) > 8.f;
+                    raise = raise || fmaxf(fmaxf(z[n][0], z[n][1]), fmaxf(z[n][2], z[n][3])) > kTopExp;
                 if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
@@ -630,7 +640,7 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
                             float top = fmaf(fmaxf(s[n][c], s[n][c + 2]), q_scale(n, c) * ks, lv);
 #pragma unroll
                             for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                            top = fmaxf(top, m[n][c]);
+                            top = fmaxf(top - kLift<T>, m[n][c]);
                             const float fix = exp2_fast(m[n][c] - top);
                             m[n][c] = top;
                             l[n][c] *= fix;

@@ -19,9 +19,9 @@
 //     be issued over P, and its completion tells that P V is done;
 //   * warps 0-3, a thread a row: the running maximum and sum.  A page's key
 //     scale and the row's factor make one factor for 16 scores, its value scale
-//     enters the exponent (as in the stream kernel); O is rescaled only when
-//     the reference rises by more than 2^8.  They also load the queries and
-//     write the results.
+//     enters the exponent; weights go up to 2^15, and the reference is raised, and
+//     O rescaled, only when one would pass that (as in the stream kernel).  They
+//     also load the queries and write the results.
 // Tensor memory (256 columns a CTA): S [0, 128), O [128, 128 + D); P takes S's
 // upper half: scores 64..127 are held in registers when it is written.
 //
@@ -461,8 +461,9 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                     if (edge) mask(a, 64), mask(b, 96);
                     gather(a, 64);
                     gather(b, 96);
-                    const bool raise = top > m + 8.f;
+                    const bool raise = top > m + kTopExp;
                     if (__any_sync(0xffffffffu, raise)) {
+                        top -= kLift<T>;
                         const float fix = !raise || m == -INFINITY ? (raise ? 0.f : 1.f) : exp2_fast(m - top);
                         if (raise) m = top;
                         l *= fix;

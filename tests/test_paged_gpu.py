@@ -474,6 +474,41 @@ def test_attention_small_queries_over_large_keys(kernel, dtype):
     check((q, kc, vc, torch.where(ks.isnan(), ks, 0.0), vs, table, lens, starts), kernel=kernel)
 
 
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_one_strong_key_over_many_weak(kernel, dtype, D):
+    """One key of value zero, 19 nats above 64 Ki others: what is left of the output is theirs.
+
+    A weight is rounded against the largest one at 2^7 (16-bit queries; 2^13 with
+    fp32 queries, in two parts): 2^-25 at the lower end of fp16, so 2^-32 (2^-38)
+    of the largest value a key, beside the relative errors that out_bound has."""
+    needs(kernel, dtype, D)
+    block, n, batch = 128, 1 << 16, 300  # (as many requests as CTAs: a CTA sees a request whole)
+    g = torch.Generator().manual_seed(22)
+    pages = n // block
+    k = torch.zeros(pages, 1, block, D)
+    k[:, 0, :, 1] = torch.randn(pages, block, generator=g)
+    v = 1 + 0.25 * torch.randn(pages, 1, block, D, generator=g)
+    k[6, 0, 9, 0], k[6, 0, 9, 1], v[6, 0, 9] = 8.0, 0.0, 0.0
+    kc, vc = k.to(torch.float8_e4m3fn), v.to(torch.float8_e4m3fn)
+    ones = torch.ones(pages, 1)
+    q = torch.zeros(1, 1, D)
+    q[0, 0, 0], q[0, 0, 1] = 19.0, 4.0
+    q = q.to(dtype)
+    order = list(range(pages))
+    want, lse, weight = ref.attention(q, kc, vc, ones, ones, [order], [n], [0, 1], scale=0.125)
+    table = i32([order, order[::-1]]).repeat(batch // 2, 1)  # the strong key early and late
+    out, got_lse = pmkl_pytorch_ext.paged_attention_fw(
+        q.cuda().repeat(batch, 1, 1), kc.cuda(), vc.cuda(), ones.cuda(), ones.cuda(), table, i32([n] * batch), None, 1, True,
+        0.125, kernel)
+    rel, floor = (2.0 ** -20, 2.0 ** -38) if dtype == F32 else (2.0 ** -11, 2.0 ** -32)
+    bound = (rel + 2.0 ** -15) * weight + n * floor * float(vc.float().abs().max()) + 0.5 * ref.ulp(want, dtype)
+    err = (out.cpu().double() - want).abs()
+    assert (err <= bound).all(), f"err {err.max():.3e} of {float(want.abs().max()):.3e}, worst err / bound {(err / bound).max():.3f}"
+    assert ((got_lse.cpu().double() - lse).abs() <= ref.lse_bound(lse)).all()
+
+
 # ---------------------------------------------------------------- refusals
 def test_refusals():
     q, kc, vc, ks, vs, table, lens, starts = problem([20], [1], 4, 2, 64, 16, F16, seed=8)

@@ -115,9 +115,9 @@ __device__ __forceinline__ uint32_t h2_bits(float lo, float hi) {
 }
 __device__ __forceinline__ float2 h2_floats(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
 
-// A running maximum before its first score: far below all, and finite, so that
-// differences with it are numbers.
-constexpr float kNoMax = -1e30f;
+// A running maximum before its first score: no fp32 number is below it, and it is
+// finite, so that differences with it are numbers.
+constexpr float kNoMax = -3.402823466e38f;
 
 // Weights are 2^(w - M) up to 2^kTopExp, where fp16 ends; M is raised to where the
 // largest is 2^lift.
@@ -614,30 +614,25 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
                         if (key + g + 8 >= lim.y) s[n][3] = -INFINITY;
                     }
                 }
-                // z = w - M: the weight's exponent, value scale included, against the reference
-                float z[NT][4];
+                // w: the weight's exponent, value scale included.  Rounded before M is
+                // taken from it: in one step the difference would keep the rounding of
+                // M, which passes 1 where scores pass 2^24.
                 bool raise = false;
-                const auto exponents = [&]() {
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        const float f0 = q_scale(n, 0) * ks, f1 = q_scale(n, 1) * ks;
-                        const float o0 = lv - m[n][0], o1 = lv - m[n][1];
-                        z[n][0] = fmaf(s[n][0], f0, o0);
-                        z[n][1] = fmaf(s[n][1], f1, o1);
-                        z[n][2] = fmaf(s[n][2], f0, o0);
-                        z[n][3] = fmaf(s[n][3], f1, o1);
-                    }
-                };
-                exponents();
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-                    raise = raise || fmaxf(fmaxf(z[n][0], z[n][1]), fmaxf(z[n][2], z[n][3])) > kTopExp;
+                for (int n = 0; n < NT; ++n) {
+                    const float f0 = q_scale(n, 0) * ks, f1 = q_scale(n, 1) * ks;
+                    s[n][0] = fmaf(s[n][0], f0, lv);
+                    s[n][1] = fmaf(s[n][1], f1, lv);
+                    s[n][2] = fmaf(s[n][2], f0, lv);
+                    s[n][3] = fmaf(s[n][3], f1, lv);
+                    raise = raise || fmaxf(s[n][0], s[n][2]) - m[n][0] > kTopExp || fmaxf(s[n][1], s[n][3]) - m[n][1] > kTopExp;
+                }
                 if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            float top = fmaf(fmaxf(s[n][c], s[n][c + 2]), q_scale(n, c) * ks, lv);
+                            float top = fmaxf(s[n][c], s[n][c + 2]);
 #pragma unroll
                             for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                             top = fmaxf(top - kLift<T>, m[n][c]);
@@ -647,13 +642,12 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
 #pragma unroll
                             for (int x = 0; x < kMt; ++x) acc[x][n][c] *= fix, acc[x][n][c + 2] *= fix;
                         }
-                    exponents();
                 }
                 uint32_t pf[kParts][NT][2];  // P^T, keys along the operand's rows
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const float p0 = exp2_fast(z[n][0]), p1 = exp2_fast(z[n][1]);
-                    const float p2 = exp2_fast(z[n][2]), p3 = exp2_fast(z[n][3]);
+                    const float p0 = exp2_fast(s[n][0] - m[n][0]), p1 = exp2_fast(s[n][1] - m[n][1]);
+                    const float p2 = exp2_fast(s[n][2] - m[n][0]), p3 = exp2_fast(s[n][3] - m[n][1]);
                     l[n][0] = fmaf(p0 + p2, inv_vs, l[n][0]);
                     l[n][1] = fmaf(p1 + p3, inv_vs, l[n][1]);
                     const uint32_t a = h2_bits(p0, p1), c = h2_bits(p2, p3);

@@ -21,7 +21,13 @@
 //     scale and the row's factor make one factor for 16 scores, its value scale
 //     enters the exponent; weights go up to 2^15, and the reference is raised, and
 //     O rescaled, only when one would pass that (as in the stream kernel).  They
-//     also load the queries and write the results.
+//     also load the queries and write the results.  Score and reference meet in
+//     one multiply-add, which is exact enough while the reference is below 2^20;
+//     beyond, the exponents are formed in two steps beforehand (two steps for all:
+//     498 us against 476 on the chunks below).  What is seldom needed (masks,
+//     rescaling, those exponents) goes through tensor memory in rolled loops: the
+//     warps' code has to stay in the instruction cache (masks in registers and
+//     an unrolled rescaling, 6 KB more: prompts of 1000 tokens 489 us against 461).
 // Tensor memory (256 columns a CTA): S [0, 128), O [128, 128 + D); P takes S's
 // upper half: scores 64..127 are held in registers when it is written.
 //
@@ -77,6 +83,10 @@ struct TileCfg {
 
 constexpr int kAhead = 4;
 
+// References up to here: what the multiply-add of a score with its reference may
+// be off, four roundings of it, stays below 2^-2 (weights below fp16's largest).
+constexpr float kExactRef = 1048576.f;
+
 struct TileShared {
     uint64_t q_full, k_full, k_empty, v_full, v_empty, s_full, p_full, o_full, drained;
     uint64_t seg_full[2], seg_empty[2], page_full[kAhead], page_empty[kAhead];
@@ -87,8 +97,9 @@ struct TileShared {
     // Of four tiles' groups of 16 keys: where they begin (0: no page) in the keys
     // and the values; key scale, log2 of the value scale (-inf: no page).
     unsigned long long from[kAhead][2][8];
-    float2 scale[kAhead][8];
-    float inv_vs[kAhead][8];
+    // The last: (1, 0) and 0, for scores that are exponents already.
+    float2 scale[kAhead + 1][8];
+    float inv_vs[kAhead + 1][8];
     int nan[2];          // the tile's values held NaN: tile number of the CTA + 1
     alignas(16) uint32_t nan_cols[kTileRows][4];  // columns of a row that are NaN (see above)
     long long sum[kTileThreads / 32];
@@ -176,6 +187,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
             mbar_init(&sh.page_empty[i], 8);  // four softmax and four loading warps
         }
         sh.nan[0] = sh.nan[1] = 0;
+        for (int i = 0; i < 8; ++i) sh.scale[kAhead][i] = make_float2(1.f, 0.f), sh.inv_vs[kAhead][i] = 0.f;
         // Once any CTA has given up a wait, later CTAs skip their work.
         sh.abort_flag = (*reinterpret_cast<volatile unsigned int *>(&g_device_error) != 0u) ? 1 : 0;
         sa.desc[blockIdx.x].segments = 0;
@@ -402,7 +414,8 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                 }
             const float log2_scale = p.scale * 1.4426950408889634f;
             const int e = query_exponent(amax, log2_scale);
-            const float down = exp2_int(-e), up = exp2_int(e) * log2_scale;
+            const float down = exp2_int(-e);
+            const float row_up = exp2_int(e) * log2_scale;
 #pragma unroll 1
             for (int c = 0; c < D; c += 16) {
                 float x[16];
@@ -420,7 +433,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
 
             const int lim = real ? visible(p, s.r, tok) : s.r.keys;
             const bool busy = warp * 32 < s.n_rows;  // some row of this warp is one
-            float m = -INFINITY, l = 0.f;
+            float m = kNoMax, l = 0.f;
             *reinterpret_cast<uint4 *>(sh.nan_cols[tid]) = make_uint4(0, 0, 0, 0);
             for (int j = tile0; j < tile1; ++j, ++it) {
                 if (!(ok = wait_warp(&sh.s_full, it & 1, abort_flag))) break;
@@ -428,21 +441,29 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                 if (!(ok = wait_warp(&sh.page_full[it % kAhead], it / kAhead & 1, abort_flag))) break;
                 tc_fence_after();
                 if (busy) {
-                    const float2 *scale = sh.scale[it % kAhead];
-                    const float *inv_vs = sh.inv_vs[it % kAhead];
+                    int page = it % kAhead;  // of the scales
+                    float up = row_up;
                     const int seen = lim - j * 128;  // columns of this tile that the row sees
                     const bool edge = j * 128 + 128 > lim_min;
                     uint32_t a[32], b[32];
-                    const auto mask = [&](uint32_t (&r)[32], int base) {
+                    if (edge) {
+                        // What the row does not see, as -inf in its scores' place.
+#pragma unroll 1
+                        for (int x = 0; x < 128; x += 16) {
+                            uint32_t r[16];
+                            tmem_ld16(lanes + C::kColS + x, r);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (base + i >= seen) r[i] = 0xFF800000u;  // -inf
-                    };
+                            for (int i = 0; i < 16; ++i)
+                                if (x + i >= seen) r[i] = 0xFF800000u;  // -inf
+                            tmem_st16(lanes + C::kColS + x, r);
+                        }
+                        tmem_wait_st();
+                    }
                     float top = -INFINITY;
                     const auto gather = [&](uint32_t (&r)[32], int base) {
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
-                            const float2 sc = scale[base / 16 + x];
+                            const float2 sc = sh.scale[page][base / 16 + x];
                             top = fmaxf(top, fmaf(max16(r + 16 * x), up * sc.x, sc.y));
                         }
                     };
@@ -451,24 +472,23 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                     tmem_ld32(lanes + C::kColS + 32, b);
                     tmem_arrived(a);
                     tmem_arrived(b);
-                    if (edge) mask(a, 0), mask(b, 32);
                     gather(a, 0);
                     gather(b, 32);
                     tmem_ld32(lanes + C::kColS + 64, a);
                     tmem_ld32(lanes + C::kColS + 96, b);
                     tmem_arrived(a);
                     tmem_arrived(b);
-                    if (edge) mask(a, 64), mask(b, 96);
                     gather(a, 64);
                     gather(b, 96);
-                    const bool raise = top > m + kTopExp;
-                    if (__any_sync(0xffffffffu, raise)) {
+                    const bool raise = top - m > kTopExp;
+                    float ref = m;  // what comes off the exponents
+                    if (__any_sync(0xffffffffu, raise || fabsf(m) > kExactRef)) {
                         top -= kLift<T>;
-                        const float fix = !raise || m == -INFINITY ? (raise ? 0.f : 1.f) : exp2_fast(m - top);
+                        const float fix = raise ? exp2_fast(m - top) : 1.f;
                         if (raise) m = top;
                         l *= fix;
-                        if (j > tile0) {
-#pragma unroll
+                        if (j > tile0 && __any_sync(0xffffffffu, raise)) {
+#pragma unroll 1
                             for (int x = 0; x < D / 16; ++x) {
                                 uint32_t o[16];
                                 tmem_ld16(lanes + C::kColO + x * 16, o);
@@ -477,13 +497,40 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                                 tmem_st16(lanes + C::kColO + x * 16, o);
                             }
                         }
+                        ref = m;
+                        if (__any_sync(0xffffffffu, fabsf(m) > kExactRef && m != kNoMax)) {
+                            // The exponents take the scores' place, and go through the rest as they are.
+#pragma unroll 1
+                            for (int x = 0; x < 8; ++x) {
+                                uint32_t r[16];
+                                tmem_ld16(lanes + C::kColS + x * 16, r);
+                                const float2 sc = sh.scale[page][x];
+                                const float lv = sc.y == -INFINITY ? 0.f : sc.y;
+                                float sum = 0.f;
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) {
+                                    const float z = fmaf(__uint_as_float(r[i]), up * sc.x, sc.y) - ref;
+                                    sum += exp2_fast(z - lv);
+                                    r[i] = __float_as_uint(z);
+                                }
+                                l += sum;
+                                tmem_st16(lanes + C::kColS + x * 16, r);
+                            }
+                            tmem_wait_st();
+                            tmem_ld32(lanes + C::kColS + 64, a);
+                            tmem_ld32(lanes + C::kColS + 96, b);
+                            tmem_arrived(a);
+                            tmem_arrived(b);
+                            page = kAhead;
+                            up = 1.f;
+                            ref = 0.f;
+                        }
                     }
-                    const float base_m = m == -INFINITY ? 0.f : m;
                     const auto weigh = [&](uint32_t (&r)[32], int base) {
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
-                            const float2 sc = scale[base / 16 + x];
-                            const float2 f = make_float2(up * sc.x, up * sc.x), off = make_float2(sc.y - base_m, sc.y - base_m);
+                            const float2 sc = sh.scale[page][base / 16 + x];
+                            const float2 f = make_float2(up * sc.x, up * sc.x), off = make_float2(sc.y - ref, sc.y - ref);
                             float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
                             for (int i = 0; i < 8; ++i) {
@@ -493,7 +540,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                                 sum.x += w.x, sum.y += w.y;
                                 r[8 * x + i] = h2_bits(w.x, w.y);
                             }
-                            l = fmaf(sum.x + sum.y, inv_vs[base / 16 + x], l);
+                            l = fmaf(sum.x + sum.y, sh.inv_vs[page][base / 16 + x], l);
                         }
                         tmem_st16(lanes + C::kColP + base / 2, r);
                     };
@@ -503,7 +550,6 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                     tmem_ld32(lanes + C::kColS + 32, b);
                     tmem_arrived(a);
                     tmem_arrived(b);
-                    if (edge) mask(a, 0), mask(b, 32);
                     weigh(a, 0);
                     weigh(b, 32);
                     tmem_wait_st();

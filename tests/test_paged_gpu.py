@@ -509,6 +509,30 @@ def test_attention_one_strong_key_over_many_weak(kernel, dtype, D):
     assert ((got_lse.cpu().double() - lse).abs() <= ref.lse_bound(lse)).all()
 
 
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("dtype,exponent,key_exponent", [(F32, 103, 0), (F32, 122, 0), (F32, 23, 6), (F16, 14, 30), (BF16, 103, 0),
+                                                         (BF16, 27, 4)])
+def test_attention_scores_far_from_zero(kernel, dtype, exponent, key_exponent):
+    """Scores of both signs between 1e9 and 1e38, where one key (or three equal ones of a page) leads by an eighth.
+
+    fp32 scores of this size differ by more than their rounding or not at all, so
+    the output is the leaders' mean; lse is off by their relative rounding, 2^-15
+    at most."""
+    needs(kernel, dtype)
+    q, kc, vc, ks, vs, table, lens, starts = problem([1, 3, 200], [1, 1, 20], 2, 1, 64, 16, dtype, seed=23)
+    kc = torch.where(kc.view(torch.uint8) == 0x7F, kc.view(torch.uint8), 0x38)  # ones where written
+    kc[table[2][77 // 16], 0, 77 % 16] = 0x39  # 1.125
+    kc[table[2][101 // 16], 0, 101 % 16] = 0x36  # 0.875
+    kc, ks = kc.view(torch.float8_e4m3fn), torch.where(ks.isnan(), ks, 2.0 ** key_exponent)
+    for sign in (1, -1):
+        q = torch.full_like(q, sign * 2.0 ** exponent)
+        want, lse, weight = ref.attention(q, kc, vc, ks, vs, table, lens, starts)
+        out, got = pmkl_pytorch_ext.paged_attention_fw(q.cuda(), kc.cuda(), vc.cuda(), ks.cuda(), vs.cuda(), i32(table), i32(lens),
+                                                       i32(starts), 20, True, 0.0, kernel)
+        assert ((out.cpu().double() - want).abs() <= ref.out_bound(want, weight, lse, dtype, 200)).all()
+        assert ((got.cpu().double() - lse).abs() <= 2.0 ** -15 * lse.abs()).all()
+
+
 # ---------------------------------------------------------------- refusals
 def test_refusals():
     q, kc, vc, ks, vs, table, lens, starts = problem([20], [1], 4, 2, 64, 16, F16, seed=8)

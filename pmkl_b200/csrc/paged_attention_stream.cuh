@@ -37,7 +37,8 @@
 //     largest is 2^7 (voted per warp), so most tiles reduce nothing across lanes.
 //     What a weight may lose beside 2^-11 of itself is then 2^-32 of the largest.
 //     fp32 queries raise M to where the largest weight is 2^13: 2^-22 of a weight
-//     or 2^-38 of the largest.
+//     or 2^-38 of the largest.  Where vs is small and another page's large, p' may
+//     be 0 and p' / vs not: pages of small vs add 2^(w - M - log2 vs) to the sum.
 //
 // mma.sync and not tcgen05: 8 to 32 query rows leave most of a 128-row tcgen05
 // tile empty, and the cache's bytes are the bound.  B200, device time: 16 x 4096
@@ -125,6 +126,11 @@ constexpr float kTopExp = 15.f;
 template <typename T>
 constexpr float kLift = sizeof(T) == 4 ? 13.f : 7.f;
 
+// log2 of the value scales below which the sum's terms come from exponents of their
+// own.  From there on, 2^(7 - 32 - 64) in front of a weight, one of 2^-37 of the
+// largest is still a normal number, whatever the scale of the other pages.
+constexpr float kSmallScale = -32.f;
+
 __device__ __forceinline__ float rcp_fast(float x) {
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -140,6 +146,10 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+
+// The square root of 2^x: sums as large as 1 / vs are multiplied by it twice where
+// 2^x itself would be 0 (x down to -252).
+__device__ __forceinline__ float exp2_half(float x) { return exp2_fast(0.5f * x); }
 
 // Asynchronous copies to shared memory: 16 bytes past L1 (a step reads the cache
 // once), or 4.
@@ -636,9 +646,9 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
 #pragma unroll
                             for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                             top = fmaxf(top - kLift<T>, m[n][c]);
-                            const float fix = exp2_fast(m[n][c] - top);
+                            const float half = exp2_half(m[n][c] - top), fix = half * half;
                             m[n][c] = top;
-                            l[n][c] *= fix;
+                            l[n][c] = l[n][c] * half * half;
 #pragma unroll
                             for (int x = 0; x < kMt; ++x) acc[x][n][c] *= fix, acc[x][n][c + 2] *= fix;
                         }
@@ -648,8 +658,13 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
                 for (int n = 0; n < NT; ++n) {
                     const float p0 = exp2_fast(s[n][0] - m[n][0]), p1 = exp2_fast(s[n][1] - m[n][1]);
                     const float p2 = exp2_fast(s[n][2] - m[n][0]), p3 = exp2_fast(s[n][3] - m[n][1]);
-                    l[n][0] = fmaf(p0 + p2, inv_vs, l[n][0]);
-                    l[n][1] = fmaf(p1 + p3, inv_vs, l[n][1]);
+                    if (lv < kSmallScale) {
+                        l[n][0] += exp2_fast(s[n][0] - m[n][0] - lv) + exp2_fast(s[n][2] - m[n][0] - lv);
+                        l[n][1] += exp2_fast(s[n][1] - m[n][1] - lv) + exp2_fast(s[n][3] - m[n][1] - lv);
+                    } else {
+                        l[n][0] = fmaf(p0 + p2, inv_vs, l[n][0]);
+                        l[n][1] = fmaf(p1 + p3, inv_vs, l[n][1]);
+                    }
                     const uint32_t a = h2_bits(p0, p1), c = h2_bits(p2, p3);
                     pf[0][n][0] = transpose8x8(a);
                     pf[0][n][1] = transpose8x8(c);
@@ -750,8 +765,9 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
             float sum = 0.f, fix[kStreamWarps];
 #pragma unroll
             for (int w = 0; w < kStreamWarps; ++w) {
-                fix[w] = exp2_fast(s_m[w][rw] - top);
-                sum = fmaf(fix[w], s_l[w][rw], sum);
+                const float half = exp2_half(s_m[w][rw] - top);
+                fix[w] = half * half;
+                sum = fmaf(half, half * s_l[w][rw], sum);
             }
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
@@ -846,9 +862,9 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
                 float sum = 0.f, x = 0.f;
 #pragma unroll
                 for (int w = 0; w < kStreamWarps; ++w) {
-                    const float fix = exp2_fast(s_m[w][rw] - top);
-                    sum = fmaf(fix, s_l[w][rw], sum);
-                    x = fmaf(fix, from[w * C::kRows * C::kRowPitch], x);
+                    const float half = exp2_half(s_m[w][rw] - top);
+                    sum = fmaf(half, half * s_l[w][rw], sum);
+                    x = fmaf(half * half, from[w * C::kRows * C::kRowPitch], x);
                 }
                 x *= sum == 0.f ? 0.f : 1.f / sum;
                 if (s_any_nan && (s_nan[rw][d >> 5] >> (d & 31) & 1u)) x = NAN;

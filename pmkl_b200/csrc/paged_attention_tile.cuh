@@ -24,7 +24,8 @@
 //     also load the queries and write the results.  Score and reference meet in
 //     one multiply-add, which is exact enough while the reference is below 2^20;
 //     beyond, the exponents are formed in two steps beforehand (two steps for all:
-//     498 us against 476 on the chunks below).  What is seldom needed (masks,
+//     498 us against 476 on the chunks below), as they are where a page's value
+//     scale is small.  What is seldom needed (masks,
 //     rescaling, those exponents) goes through tensor memory in rolled loops: the
 //     warps' code has to stay in the instruction cache (masks in registers and
 //     an unrolled rescaling, 6 KB more: prompts of 1000 tokens 489 us against 461).
@@ -100,6 +101,7 @@ struct TileShared {
     // The last: (1, 0) and 0, for scores that are exponents already.
     float2 scale[kAhead + 1][8];
     float inv_vs[kAhead + 1][8];
+    int small[kAhead];   // some group's value scale is below kSmallScale
     int nan[2];          // the tile's values held NaN: tile number of the CTA + 1
     alignas(16) uint32_t nan_cols[kTileRows][4];  // columns of a row that are NaN (see above)
     long long sum[kTileThreads / 32];
@@ -249,13 +251,16 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                         ks = key_scale(__ldg(p.k.scale + at));
                         vs = value_scale(__ldg(p.v.scale + at));
                     }
+                    const float lv = there ? log2f(vs) : -INFINITY;
+                    const int small = __any_sync(0xffffffffu, there && lv < kSmallScale);
                     const int i = it % kAhead;
                     if (it >= kAhead && !(ok = wait_warp(&sh.page_empty[i], (it / kAhead - 1) & 1, abort_flag))) break;
                     if (lane < 16) sh.from[i][lane >> 3][lane & 7] = from;
                     if (lane < 8) {
-                        sh.scale[i][lane] = make_float2(ks, there ? log2f(vs) : -INFINITY);
+                        sh.scale[i][lane] = make_float2(ks, lv);
                         sh.inv_vs[i][lane] = 1.f / vs;
                     }
+                    if (lane == 0) sh.small[i] = small;
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sh.page_full[i]);
                     x = x_next;
@@ -482,11 +487,12 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                     gather(b, 96);
                     const bool raise = top - m > kTopExp;
                     float ref = m;  // what comes off the exponents
-                    if (__any_sync(0xffffffffu, raise || fabsf(m) > kExactRef)) {
+                    const bool small = sh.small[page] != 0;
+                    if (__any_sync(0xffffffffu, raise || fabsf(m) > kExactRef || small)) {
                         top -= kLift<T>;
-                        const float fix = raise ? exp2_fast(m - top) : 1.f;
+                        const float half = raise ? exp2_half(m - top) : 1.f, fix = half * half;
                         if (raise) m = top;
-                        l *= fix;
+                        l = l * half * half;
                         if (j > tile0 && __any_sync(0xffffffffu, raise)) {
 #pragma unroll 1
                             for (int x = 0; x < D / 16; ++x) {
@@ -498,7 +504,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                             }
                         }
                         ref = m;
-                        if (__any_sync(0xffffffffu, fabsf(m) > kExactRef && m != kNoMax)) {
+                        if (__any_sync(0xffffffffu, (fabsf(m) > kExactRef && m != kNoMax) || small)) {
                             // The exponents take the scores' place, and go through the rest as they are.
 #pragma unroll 1
                             for (int x = 0; x < 8; ++x) {

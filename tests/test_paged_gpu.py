@@ -533,6 +533,19 @@ def test_attention_scores_far_from_zero(kernel, dtype, exponent, key_exponent):
         assert ((got.cpu().double() - lse).abs() <= 2.0 ** -15 * lse.abs()).all()
 
 
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("low,high", [(-64, 64), (-64, 20), (-20, 64)])
+def test_attention_value_scales_at_the_ends_of_their_range(kernel, dtype, low, high):
+    """Pages of values at both ends of 2^-64 .. 2^64: each key counts in the sum, whatever its page's scale."""
+    for seed in range(3):
+        prob = problem([700, 33, 1500, 257], [1, 1, 2, 40], 4, 2, 128, 16, dtype, seed=30 + seed)
+        vs = prob[4]
+        g = torch.Generator().manual_seed(seed)
+        vs.copy_(torch.where(vs.isnan(), vs, torch.exp2(torch.where(torch.rand(vs.shape, generator=g) < 0.5, low, high).float())))
+        check(prob, kernel=kernel)
+
+
 # ---------------------------------------------------------------- refusals
 def test_refusals():
     q, kc, vc, ks, vs, table, lens, starts = problem([20], [1], 4, 2, 64, 16, F16, seed=8)

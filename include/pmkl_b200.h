@@ -375,8 +375,8 @@ int pmkl_paged_append(const void *k, const void *v, const int64_t *k_new_strides
  *   seq_lens     : [batch] int32 rows in the cache, the step's own included.
  *   query_starts : [batch + 1] int32; NULL: one token a request (tokens ==
  *                  batch).
- *   max_query_len: no request has more tokens in the step (rows past it are
- *                  not written).
+ *   max_query_len: tokens of the longest request in the step, or more; it
+ *                  chooses the kernel.  A wrong one costs time, not results.
  *   is_causal    : token i of a request's n sees the keys up to its own place,
  *                  seq_len - n + i; otherwise all of them.
  *   scale        : score scale; <= 0 for 1/sqrt(hidden).
@@ -384,8 +384,8 @@ int pmkl_paged_append(const void *k, const void *v, const int64_t *k_new_strides
  *                  pmkl_paged_attention_workspace_size(...) bytes, 256-byte
  *                  aligned; contents on entry do not matter.
  *
- * A row that sees no key gets o = 0 and lse = -inf, and so do rows of q past
- * query_starts[batch].  Rows of a page behind seq_len may hold anything, NaN
+ * A row that sees no key gets o = 0 and lse = -inf, and so do rows of q before
+ * query_starts[0] and from query_starts[batch] on.  Rows of a page behind seq_len may hold anything, NaN
  * included.  Scales are positive; the scale of a page of values outside
  * 2^-64 .. 2^64 counts as the nearer of the two, one of a page of keys below
  * 2^-64 as 2^-64.

@@ -22,14 +22,15 @@ struct AttnArgs {
     long long table_stride;
     const int *seq_lens, *query_starts;
     float *lse;
-    int tokens, batch, H, Hkv, D, num_blocks, block, max_blocks, max_q, causal;
+    int tokens, batch, H, Hkv, D, num_blocks, block, max_blocks, causal;
+    int max_q;  // rows of a request that launches are sized for; a request may have more
     float scale;
 };
 
 // Rows and keys of request b, kept within the tensors whatever the device
 // arrays hold.
 struct Request {
-    int first, rows, keys;  // first row of q, rows (at most max_q), rows in the cache
+    int first, rows, keys;  // first row of q, rows, rows in the cache
     int shift;              // row i sees keys j <= i + shift
 };
 
@@ -44,9 +45,9 @@ __host__ __device__ __forceinline__ Request request_of(const AttnArgs &p, int b)
     const long long cap = min(static_cast<long long>(p.max_blocks) * p.block, 0x7FFFFFFFLL - 4096);
     const int len = max(0, p.seq_lens[b]);
     r.first = begin;
-    r.rows = min(end - begin, p.max_q);
+    r.rows = end - begin;
     r.keys = static_cast<int>(len < cap ? len : cap);
-    r.shift = r.keys - (end - begin);
+    r.shift = r.keys - r.rows;
     return r;
 }
 
@@ -55,15 +56,18 @@ __host__ __device__ __forceinline__ int visible(const AttnArgs &p, const Request
     return p.causal ? min(r.keys, max(0, i + r.shift + 1)) : r.keys;
 }
 
-// Rows of q that belong to no request: o = 0, lse = -inf.  Called by the whole
-// grid (128 threads and more a CTA).
+// Rows of q that belong to no request, before the first and behind the last: o =
+// 0, lse = -inf.  Called by the whole grid (128 threads and more a CTA).
 template <typename T>
-__device__ __forceinline__ void clear_tail(const AttnArgs &p) {
+__device__ __forceinline__ void clear_unused(const AttnArgs &p) {
     if (!p.query_starts) return;
-    const int used = min(max(p.query_starts[p.batch], 0), p.tokens);
-    const long long n = static_cast<long long>(p.tokens - used) * p.H;
+    const int first = min(max(p.query_starts[0], 0), p.tokens);
+    const int used = min(max(p.query_starts[p.batch], first), p.tokens);
+    const long long n = static_cast<long long>(first + p.tokens - used) * p.H;
     for (long long i = blockIdx.x; i < n; i += gridDim.x) {
-        const long long t = used + i / p.H, h = i % p.H;
+        const long long h = i % p.H;
+        long long t = i / p.H;
+        if (t >= first) t += used - first;
         T *o = static_cast<T *>(p.o) + t * p.o_st[0] + h * p.o_st[1];
         for (int d = threadIdx.x; d < p.D; d += blockDim.x) o[d] = Elem<T>::from_float(0.f);
         if (p.lse && threadIdx.x == 0) p.lse[t * p.H + h] = -INFINITY;
@@ -127,92 +131,94 @@ __global__ void __launch_bounds__(kSimtThreads) paged_attention_simt_kernel(cons
     __shared__ float part[kWarps][256];
     __shared__ float ms[kWarps], ls[kWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    clear_tail<T>(p);
+    clear_unused<T>(p);
     const long long units = static_cast<long long>(p.batch) * p.max_q * p.H;
     for (long long u = blockIdx.x; u < units; u += gridDim.x) {
         const int h = static_cast<int>(u % p.H);
         const long long bi = u / p.H;
-        const int b = static_cast<int>(bi / p.max_q), i = static_cast<int>(bi % p.max_q);
+        const int b = static_cast<int>(bi / p.max_q);
         const Request r = request_of(p, b);
-        if (i >= r.rows) continue;
         const int hk = h / (p.H / p.Hkv);
-        const int keys = visible(p, r, i);
-        const T *q = static_cast<const T *>(p.q) + (r.first + i) * p.q_st[0] + h * p.q_st[1];
-        __syncthreads();  // the row before has been read
-        for (int d = threadIdx.x; d < p.D; d += kSimtThreads) qs[d] = Elem<T>::to_float(q[d]) * p.scale;
-        __syncthreads();
-        float m = -INFINITY, l = 0.f, acc[kSimtCols] = {};
-        for (long long j0 = warp * 32; j0 < keys; j0 += kWarps * 32) {
-            const long long j = j0 + lane;
-            float s = -INFINITY, vs = 0.f;
-            long long vrow = 0;
-            bool there = j < keys;
-            if (there) {
-                const int page = p.table[b * p.table_stride + j / p.block];
-                there = page >= 0 && page < p.num_blocks;
+        for (long long row = bi % p.max_q; row < r.rows; row += p.max_q) {
+            const int i = static_cast<int>(row);
+            const int keys = visible(p, r, i);
+            const T *q = static_cast<const T *>(p.q) + (r.first + i) * p.q_st[0] + h * p.q_st[1];
+            __syncthreads();  // the row before has been read
+            for (int d = threadIdx.x; d < p.D; d += kSimtThreads) qs[d] = Elem<T>::to_float(q[d]) * p.scale;
+            __syncthreads();
+            float m = -INFINITY, l = 0.f, acc[kSimtCols] = {};
+            for (long long j0 = warp * 32; j0 < keys; j0 += kWarps * 32) {
+                const long long j = j0 + lane;
+                float s = -INFINITY, vs = 0.f;
+                long long vrow = 0;
+                bool there = j < keys;
                 if (there) {
-                    const long long row = j % p.block;
-                    const uint8_t *k = p.k.base + page * p.k.s[0] + hk * p.k.s[1] + row * p.k.s[2];
-                    float dot = 0.f;
-                    for (int d = 0; d < p.D; ++d) dot = fmaf(qs[d], e4m3_to_float(k[d]), dot);
-                    const long long at = static_cast<long long>(page) * p.Hkv + hk;
-                    s = dot * key_scale(p.k.scale[at]);
-                    vs = value_scale(p.v.scale[at]);
-                    vrow = page * p.v.s[0] + hk * p.v.s[1] + row * p.v.s[2];
+                    const int page = p.table[b * p.table_stride + j / p.block];
+                    there = page >= 0 && page < p.num_blocks;
+                    if (there) {
+                        const long long at_row = j % p.block;
+                        const uint8_t *k = p.k.base + page * p.k.s[0] + hk * p.k.s[1] + at_row * p.k.s[2];
+                        float dot = 0.f;
+                        for (int d = 0; d < p.D; ++d) dot = fmaf(qs[d], e4m3_to_float(k[d]), dot);
+                        const long long at = static_cast<long long>(page) * p.Hkv + hk;
+                        s = dot * key_scale(p.k.scale[at]);
+                        vs = value_scale(p.v.scale[at]);
+                        vrow = page * p.v.s[0] + hk * p.v.s[1] + at_row * p.v.s[2];
+                    }
+                }
+                float top = s;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                top = fmaxf(top, m);
+                const float base = top == -INFINITY ? 0.f : top;
+                const float fix = expf(m - base);
+                const float e = there ? expf(s - base) : 0.f;
+                float sum = e;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                m = top;
+                l = l * fix + sum;
+#pragma unroll
+                for (int c = 0; c < kSimtCols; ++c) acc[c] *= fix;
+                const float w = e * vs;
+                const unsigned int mine = __ballot_sync(0xffffffffu, there);
+                for (int x = 0; x < 32; ++x) {
+                    const float wx = __shfl_sync(0xffffffffu, w, x);
+                    const long long at = __shfl_sync(0xffffffffu, vrow, x);
+                    if (!((mine >> x) & 1u)) continue;  // a row that is not there may hold anything
+#pragma unroll
+                    for (int c = 0; c < kSimtCols; ++c) {
+                        const int d = c * 32 + lane;
+                        if (d < p.D) acc[c] = fmaf(wx, e4m3_to_float(p.v.base[at + d]), acc[c]);
+                    }
                 }
             }
-            float top = s;
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            top = fmaxf(top, m);
+            for (int c = 0; c < kSimtCols; ++c) part[warp][c * 32 + lane] = acc[c];
+            if (lane == 0) ms[warp] = m, ls[warp] = l;
+            __syncthreads();
+            float top = ms[0];
+#pragma unroll
+            for (int w = 1; w < kWarps; ++w) top = fmaxf(top, ms[w]);
             const float base = top == -INFINITY ? 0.f : top;
-            const float fix = expf(m - base);
-            const float e = there ? expf(s - base) : 0.f;
-            float sum = e;
+            float sum = 0.f, f[kWarps];
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            m = top;
-            l = l * fix + sum;
-#pragma unroll
-            for (int c = 0; c < kSimtCols; ++c) acc[c] *= fix;
-            const float w = e * vs;
-            const unsigned int mine = __ballot_sync(0xffffffffu, there);
-            for (int x = 0; x < 32; ++x) {
-                const float wx = __shfl_sync(0xffffffffu, w, x);
-                const long long at = __shfl_sync(0xffffffffu, vrow, x);
-                if (!((mine >> x) & 1u)) continue;  // a row that is not there may hold anything
-#pragma unroll
-                for (int c = 0; c < kSimtCols; ++c) {
-                    const int d = c * 32 + lane;
-                    if (d < p.D) acc[c] = fmaf(wx, e4m3_to_float(p.v.base[at + d]), acc[c]);
-                }
+            for (int w = 0; w < kWarps; ++w) {
+                f[w] = expf(ms[w] - base);
+                sum += f[w] * ls[w];
             }
+            // A sum of 0 is a row without keys; a NaN goes through to the output.
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            T *o = static_cast<T *>(p.o) + (r.first + i) * p.o_st[0] + h * p.o_st[1];
+            for (int d = threadIdx.x; d < p.D; d += kSimtThreads) {
+                float x = 0.f;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) x = fmaf(f[w], part[w][d], x);
+                o[d] = Elem<T>::from_float(x * inv);
+            }
+            if (p.lse && threadIdx.x == 0)
+                p.lse[static_cast<long long>(r.first + i) * p.H + h] = sum == 0.f ? -INFINITY : base + logf(sum);
         }
-#pragma unroll
-        for (int c = 0; c < kSimtCols; ++c) part[warp][c * 32 + lane] = acc[c];
-        if (lane == 0) ms[warp] = m, ls[warp] = l;
-        __syncthreads();
-        float top = ms[0];
-#pragma unroll
-        for (int w = 1; w < kWarps; ++w) top = fmaxf(top, ms[w]);
-        const float base = top == -INFINITY ? 0.f : top;
-        float sum = 0.f, f[kWarps];
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            f[w] = expf(ms[w] - base);
-            sum += f[w] * ls[w];
-        }
-        // A sum of 0 is a row without keys; a NaN goes through to the output.
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        T *o = static_cast<T *>(p.o) + (r.first + i) * p.o_st[0] + h * p.o_st[1];
-        for (int d = threadIdx.x; d < p.D; d += kSimtThreads) {
-            float x = 0.f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) x = fmaf(f[w], part[w][d], x);
-            o[d] = Elem<T>::from_float(x * inv);
-        }
-        if (p.lse && threadIdx.x == 0)
-            p.lse[static_cast<long long>(r.first + i) * p.H + h] = sum == 0.f ? -INFINITY : base + logf(sum);
     }
 }
 

@@ -890,7 +890,7 @@ __global__ void __launch_bounds__(StreamCfg<D, NT>::kThreads, NT == 1 ? 2 : 1) p
         }
         __syncthreads();  // the queries, sums and segment may be written over
     }
-    clear_tail<T>(p);
+    clear_unused<T>(p);
 }
 
 // Joins the partial rows of the item that CTA blockIdx.x of the kernel before

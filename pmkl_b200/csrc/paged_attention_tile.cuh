@@ -635,7 +635,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
         tmem_dealloc(tmem, C::kTmemCols);
     }
     if (tid == 0 && *abort_flag && !skip) report_device_error(PMKL_DEVERR_TIMEOUT);
-    clear_tail<T>(p);
+    clear_unused<T>(p);
 }
 
 }  // namespace paged

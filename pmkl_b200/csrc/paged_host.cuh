@@ -63,6 +63,10 @@ bool packed_strides(long long (&st)[2], const int64_t *given, int heads, int hid
     return true;
 }
 
+// The tokens a request that kernel and launch are chosen for: at least one, and
+// no more than there are.
+int query_len(int max_query_len, int tokens) { return std::max(1, std::min(max_query_len, tokens)); }
+
 int paged_plan_impl(const paged::PlanArgs &a, cudaStream_t stream) {
     paged::PlanArgs p = a;
     // 512 slots a CTA (1024: 8.9 us for 66 Ki tokens of 1024 requests against 6.7)
@@ -138,7 +142,9 @@ bool stream_applies(const paged::AttnArgs &p) {
             if (s % 16 != 0) return false;
         if (c->s[0] > 0x7FFFFFFF || c->s[2] > 0x7FFFFFFF / 16) return false;
     }
-    return static_cast<long long>(p.num_blocks) * p.Hkv <= 0x7FFFFFFF;
+    // Rows of a request that share a K/V head, and pages' scales, are counted in 31 bits.
+    return static_cast<long long>(p.tokens) * (p.H / p.Hkv) <= 0x3FFFFFFF &&
+           static_cast<long long>(p.num_blocks) * p.Hkv <= 0x7FFFFFFF;
 }
 
 // Grid of a kernel that shares out `items` of at most `tiles` tiles each over
@@ -192,7 +198,8 @@ int launch_early(K kernel, dim3 grid, int threads, int smem, const paged::Stream
 
 template <typename T, int D, int ROWS>
 int launch_join(const paged::StreamArgs &p, long long grid, cudaStream_t stream) {
-    const long long rows = std::min<long long>(ROWS, static_cast<long long>(p.a.H / p.a.Hkv) * p.a.max_q);
+    // (every row that an item may have: a request may have more tokens than max_q)
+    const long long rows = std::min<long long>(ROWS, static_cast<long long>(p.a.H / p.a.Hkv) * p.a.tokens);
     return launch_early(paged::paged_attention_join_kernel<T, D, ROWS>,
                         dim3(static_cast<unsigned>(grid), static_cast<unsigned>((rows + 7) / 8)),  // a warp a row
                         paged::kJoinThreads, 0, p, stream);
@@ -390,8 +397,7 @@ size_t pmkl_paged_attention_workspace_size(int tokens, int batch, int heads, int
     if (tokens <= 0 || batch <= 0 || heads <= 0 || kv_heads <= 0 || hidden <= 0 || max_query_len < 0 ||
         heads % kv_heads != 0 || !dtype_valid(dtype))
         return 0;
-    // 0 as well as 1: one token a request where no query_starts are given, whatever the limit says.
-    if (max_query_len == 0) max_query_len = 1;
+    max_query_len = query_len(max_query_len, tokens);
     if (hidden != 64 && hidden != 128) return 0;  // the CUDA-core kernel needs none
     // What the largest of the kernels that may be asked for needs.
     const size_t stream =
@@ -418,9 +424,7 @@ int pmkl_paged_attention(const void *q, const int64_t *q_strides, const void *k_
     if (heads > 0 && (kv_heads == 0 || heads % kv_heads != 0)) return PMKL_ERR_INVALID_SHAPE;
     if (batch > 1 && table_stride < max_blocks) return PMKL_ERR_INVALID_SHAPE;
     if (!query_starts && tokens != batch) return PMKL_ERR_INVALID_SHAPE;
-    // One value for the sizes, the workspace and the launch.
     if (!query_starts) max_query_len = 1;
-    // Rows of a request that share a K/V head are counted in 31 bits.
     if (heads > 0 && static_cast<long long>(max_query_len) * (heads / kv_heads) > 0x3FFFFFFFLL)
         return PMKL_ERR_INVALID_SHAPE;
     if (tokens == 0 || heads == 0 || hidden == 0) return PMKL_OK;
@@ -458,7 +462,7 @@ int pmkl_paged_attention(const void *q, const int64_t *q_strides, const void *k_
     p.num_blocks = num_blocks;
     p.block = block_size;
     p.max_blocks = max_blocks;
-    p.max_q = max_query_len;
+    p.max_q = query_len(max_query_len, tokens);
     p.causal = is_causal ? 1 : 0;
     // (below the normal numbers a score scale is as good as the smallest of them)
     p.scale = scale > 0.f ? fmaxf(scale, 1.17549435e-38f) : 1.0f / sqrtf(static_cast<float>(hidden));

@@ -195,7 +195,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("paged_attention_fw", &paged_attention_fw, "paged_attention_fw", pybind11::arg("q"),
           pybind11::arg("k_cache"), pybind11::arg("v_cache"), pybind11::arg("k_scale"), pybind11::arg("v_scale"),
           pybind11::arg("block_table"), pybind11::arg("seq_lens"), pybind11::arg("query_starts") = pybind11::none(),
-          pybind11::arg("max_query_len") = 1, pybind11::arg("is_causal") = true, pybind11::arg("scale") = 0.0,
+          pybind11::arg("max_query_len") = pybind11::none(), pybind11::arg("is_causal") = true, pybind11::arg("scale") = 0.0,
           pybind11::arg("kernel") = 0);
     m.attr("KERNEL_AUTO") = static_cast<int>(PMKL_ATTN_AUTO);
     m.attr("KERNEL_SIMT") = static_cast<int>(PMKL_ATTN_SIMT);

@@ -129,9 +129,11 @@ void paged_append(const at::Tensor &k, const at::Tensor &v, const at::Tensor &sl
 std::tuple<at::Tensor, at::Tensor> paged_attention_fw(
     const at::Tensor &q, const at::Tensor &k_cache, const at::Tensor &v_cache, const at::Tensor &k_scale,
     const at::Tensor &v_scale, const at::Tensor &block_table, const at::Tensor &seq_lens,
-    const c10::optional<at::Tensor> &query_starts, int64_t max_query_len, bool is_causal, double scale,
+    const c10::optional<at::Tensor> &query_starts, c10::optional<int64_t> max_len, bool is_causal, double scale,
     int64_t kernel) {
     check_packed(q, "q");
+    // Not given: one token a request without query_starts, any number with them.
+    const int64_t max_query_len = max_len.has_value() ? *max_len : (query_starts.has_value() ? q.size(0) : 1);
     const at::Device dev = q.device();
     check_cache(k_cache, k_scale, "k", dev);
     check_cache(v_cache, v_scale, "v", dev);

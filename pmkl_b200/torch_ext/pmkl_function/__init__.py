@@ -34,7 +34,7 @@ values in 8 bits (no reference counterpart); a step calls them in this order:
         cached_lens, new_lens, block_table, free_blocks, free_count, block_size, max_tokens)
     paged_append(k, v, slot_map, k_cache, v_cache, k_scale, v_scale)
     out, lse = paged_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens,
-                               query_starts=None, max_query_len=1, is_causal=True, scale=0.0)
+                               query_starts=None, max_query_len=None, is_causal=True, scale=0.0)
 
 See each function's text; ``examples/paged_decode.py`` runs them together.
 """
@@ -138,19 +138,22 @@ def paged_append(k, v, slot_map, k_cache, v_cache, k_scale, v_scale):
     pmkl_pytorch_ext.paged_append(k, v, slot_map, k_cache, v_cache, k_scale, v_scale)
 
 
-def paged_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_starts=None, max_query_len=1,
+def paged_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_starts=None, max_query_len=None,
                     is_causal=True, scale=0.0):
     """Attention of a step's queries [tokens, heads, hidden] over the cache.
 
     ``seq_lens`` [batch] counts each request's rows in the cache, the step's
     own included; request b's queries are rows ``query_starts[b]`` to
-    ``query_starts[b + 1]`` of ``q`` (without ``query_starts``: row b), at most
-    ``max_query_len`` of them, and stand at the end of its rows; with
-    ``is_causal`` each sees the keys up to its own place.  Query head h reads
-    K/V head h // (heads // kv_heads).  ``scale`` <= 0: 1/sqrt(hidden).
+    ``query_starts[b + 1]`` of ``q`` (without ``query_starts``: row b) and stand
+    at the end of its rows; with ``is_causal`` each sees the keys up to its own
+    place.  ``max_query_len``, the most tokens that a request has, chooses the
+    kernel: give it where it is far below the number of tokens (a wrong one
+    costs time, not results).  Query head h reads K/V head h // (heads //
+    kv_heads).  ``scale`` <= 0: 1/sqrt(hidden).
 
     Returns ``out`` like q and ``lse`` [tokens, heads] float32, the log of the
-    sum of the exponentials (-inf, with ``out`` 0, where no key is visible).
+    sum of the exponentials (-inf, with ``out`` 0, where no key is visible and in
+    rows of no request).
     Forward only: the cache is not differentiable."""
     return pmkl_pytorch_ext.paged_attention_fw(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens,
                                                query_starts, max_query_len, is_causal, scale)

@@ -546,6 +546,38 @@ def test_attention_value_scales_at_the_ends_of_their_range(kernel, dtype, low, h
         check(prob, kernel=kernel)
 
 
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("hint", [0, 1, 3, 70, 1 << 20])
+def test_attention_writes_every_row(kernel, dtype, hint):
+    """Whatever max_query_len says: rows past it, before the first request and behind the last one."""
+    needs(kernel, dtype)
+    for H, Hkv, D in ((4, 4, 64), (8, 1, 128)):
+        q, kc, vc, ks, vs, table, lens, starts = problem([64, 1, 200, 90], [3, 1, 33, 70], H, Hkv, D, 16, dtype, seed=24, tail=9)
+        starts = [s + 4 for s in starts]
+        want, lse, weight = ref.attention(q, kc, vc, ks, vs, table, lens, starts)
+        dev = [t.cuda() for t in (q, kc, vc, ks, vs)] + [i32(table), i32(lens), i32(starts)]
+        stale = [torch.full((n,), math.nan, device="cuda") for n in (q.numel(), q.numel() // 2, q.numel() // D)]
+        del stale  # (memory that the outputs are likely to get)
+        out, got_lse = pmkl_pytorch_ext.paged_attention_fw(*dev, hint, True, 0.0, kernel)
+        assert ((out.cpu().double() - want).abs() <= ref.out_bound(want, weight, lse, dtype, max(lens))).all()
+        empty, l = lse.isinf(), got_lse.cpu().double()
+        assert torch.equal(l.isinf(), empty) and (l[empty] < 0).all()
+        assert ((l - lse).abs()[~empty] <= ref.lse_bound(lse)[~empty]).all()
+
+
+def test_attention_without_max_query_len():
+    """The function's default covers a prompt."""
+    q, kc, vc, ks, vs, table, lens, starts = problem([64, 90], [33, 70], 4, 2, 64, 16, BF16, seed=25)
+    dev = [t.cuda() for t in (q, kc, vc, ks, vs)] + [i32(table), i32(lens)]
+    out, lse = paged_attention(*dev, i32(starts))
+    named, named_lse = paged_attention(*dev, query_starts=i32(starts), max_query_len=70)
+    want, want_lse, weight = ref.attention(q, kc, vc, ks, vs, table, lens, starts)
+    for o, l in ((out, lse), (named, named_lse)):
+        assert ((o.cpu().double() - want).abs() <= ref.out_bound(want, weight, want_lse, BF16, 90)).all()
+        assert ((l.cpu().double() - want_lse).abs() <= ref.lse_bound(want_lse)).all()
+
+
 # ---------------------------------------------------------------- refusals
 def test_refusals():
     q, kc, vc, ks, vs, table, lens, starts = problem([20], [1], 4, 2, 64, 16, F16, seed=8)

@@ -296,7 +296,7 @@ typedef enum pmkl_paged_kernel {
 typedef enum pmkl_plan_status {
     PMKL_PLAN_OK = 0,
     PMKL_PLAN_NO_BLOCKS = 1,   /* the free list has not enough pages */
-    PMKL_PLAN_NO_COLUMNS = 2,  /* the block table is too narrow */
+    PMKL_PLAN_NO_COLUMNS = 2,  /* the block table is too narrow (or the length past 2^31 - 1) */
     PMKL_PLAN_NO_TOKENS = 3,   /* its tokens go past max_tokens */
 } pmkl_plan_status;
 

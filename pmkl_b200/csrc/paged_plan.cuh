@@ -97,8 +97,9 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs
             end += n[i];
             first[i] = pages_of(c[i], block);
             const unsigned last = pages_of(c[i] + n[i], block);
-            why[i] = end > p.max_tokens ? PMKL_PLAN_NO_TOKENS
-                                        : (last > static_cast<unsigned>(p.max_blocks) ? PMKL_PLAN_NO_COLUMNS : PMKL_PLAN_OK);
+            // (a length past 31 bits fits no table either)
+            const bool wide = last > static_cast<unsigned>(p.max_blocks) || c[i] + n[i] > 0x7FFFFFFFu;
+            why[i] = end > p.max_tokens ? PMKL_PLAN_NO_TOKENS : (wide ? PMKL_PLAN_NO_COLUMNS : PMKL_PLAN_OK);
             need[i] = why[i] == PMKL_PLAN_OK ? last - first[i] : 0;
             mine += need[i];
             s_end[r1 - r0 + i] = end;

@@ -81,6 +81,16 @@ def test_plan_long_prompts_and_empty():
     assert starts.tolist() == [0] and slots.tolist() == [-1] * 4 and left.item() == 2 and seq.numel() == 0
 
 
+def test_plan_lengths_past_31_bits():
+    """A request whose length would not fit in 32 bits is left out, and the next one is not."""
+    top = 2 ** 31 - 1
+    seq, starts, slots, left, status = paged_plan(i32([top - 1, top - 1]), i32([4, 1]), i32([[5, 6, -1], [7, 8, -1]]), i32([9]),
+                                                  i32([1]), 1 << 30, 6)
+    assert status.tolist() == [2, 0] and seq.tolist() == [top - 1, top]
+    assert starts.tolist() == [0, 4, 5] and left.item() == 1
+    assert slots.tolist() == [-1] * 4 + [8 * (1 << 30) + (top - 1 - (1 << 30)), -1]
+
+
 # ---------------------------------------------------------------- append
 def run_append(xk, xv, slots, kc, vc, ks, vs):
     """paged_append on CUDA copies; caches bit for bit as the definition says."""

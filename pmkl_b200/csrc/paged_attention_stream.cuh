@@ -234,11 +234,12 @@ struct Share {
     int h, row0, at, tiles;
 };
 
-// Where share c of `shares` begins in `total` tiles.  32-bit division where it
-// does: the 64-bit one is a long routine.
+// Where share c of `shares` begins in `total` tiles (and, with the two exchanged,
+// near which share a tile lies).  32-bit division where it does: the 64-bit one is
+// a long routine.
 __host__ __device__ __forceinline__ long long share_begin(long long total, long long c, long long shares) {
     const unsigned long long n = static_cast<unsigned long long>(total) * c;
-    return (n >> 32) == 0 ? static_cast<unsigned>(n) / static_cast<unsigned>(shares) : n / shares;
+    return ((n | shares) >> 32) == 0 ? static_cast<unsigned>(n) / static_cast<unsigned>(shares) : n / shares;
 }
 __host__ __device__ __forceinline__ int quotient(long long a, long long b) {  // a, b >= 0, the result an int
     return ((a | b) >> 32) == 0 ? static_cast<unsigned>(a) / static_cast<unsigned>(b) : static_cast<int>(a / b);

@@ -135,3 +135,18 @@ def test_walk_over_shares(tmp_path):
                     str(repo / "tests" / "cpp" / "walk_test.cu"), "-o", str(exe)], check=True)
     out = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
     assert out.returncode == 0 and "walk ok" in out.stdout, out.stdout
+
+
+def test_shares_of_long_lists(tmp_path):
+    """Where the shares of more than 2^32 tiles begin, and whose a tile is."""
+    import subprocess
+    from pathlib import Path
+
+    from pmkl_b200 import build
+
+    repo = Path(__file__).resolve().parent.parent
+    exe = tmp_path / "share_test"
+    subprocess.run([build._nvcc(), *build.NVCC_ARCH, "-O1", "-std=c++17", "-I", str(build.INCLUDE), "-I", str(build.CSRC),
+                    str(repo / "tests" / "cpp" / "share_test.cu"), "-o", str(exe)], check=True)
+    out = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert out.returncode == 0 and "shares ok" in out.stdout, out.stdout

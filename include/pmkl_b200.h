@@ -381,8 +381,9 @@ int pmkl_paged_append(const void *k, const void *v, const int64_t *k_new_strides
  *                  seq_len - n + i; otherwise all of them.
  *   scale        : score scale; <= 0 for 1/sqrt(hidden).
  *   workspace    : device scratch of at least
- *                  pmkl_paged_attention_workspace_size(...) bytes, 256-byte
- *                  aligned; contents on entry do not matter.
+ *                  pmkl_paged_attention_workspace_size_ex(...) bytes for the
+ *                  kernel asked for, 256-byte aligned; contents on entry do not
+ *                  matter.
  *
  * A row that sees no key gets o = 0 and lse = -inf, and so do rows of q before
  * query_starts[0] and from query_starts[batch] on.  Rows of a page behind seq_len may hold anything, NaN
@@ -405,8 +406,13 @@ int pmkl_paged_attention(const void *q, const int64_t *q_strides, const void *k_
                          int block_size, int max_blocks, int max_query_len, int dtype, int is_causal, float scale,
                          void *workspace, size_t workspace_bytes, int kernel, void *stream);
 
-/* Workspace bytes of pmkl_paged_attention for these sizes (0 for an empty
- * problem; max_query_len 0 counts as 1).  Host only. */
+/* Workspace bytes of pmkl_paged_attention for these sizes and a pmkl_paged_kernel
+ * (0 for an empty problem; max_query_len 0 counts as 1): what the kernel that is
+ * asked for, or that PMKL_PAGED_AUTO chooses, may use.  Without `kernel`: enough
+ * for any of them (42 MB for 16-bit queries and hidden 128, where a decode step
+ * uses up to 5.3).  Host only. */
+size_t pmkl_paged_attention_workspace_size_ex(int tokens, int batch, int heads, int kv_heads, int hidden,
+                                              int max_query_len, int dtype, int kernel);
 size_t pmkl_paged_attention_workspace_size(int tokens, int batch, int heads, int kv_heads, int hidden,
                                            int max_query_len, int dtype);
 

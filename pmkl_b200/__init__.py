@@ -87,6 +87,8 @@ def capi() -> ctypes.CDLL:
             i32] * 11 + [f32, vp, sz, i32, vp]
         L.pmkl_paged_attention_workspace_size.restype = sz
         L.pmkl_paged_attention_workspace_size.argtypes = [i32] * 7
+        L.pmkl_paged_attention_workspace_size_ex.restype = sz
+        L.pmkl_paged_attention_workspace_size_ex.argtypes = [i32] * 8
         L.pmkl_status_string.restype = ctypes.c_char_p
         L.pmkl_status_string.argtypes = [i32]
         L.pmkl_version.restype = i32

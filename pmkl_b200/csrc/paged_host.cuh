@@ -284,6 +284,10 @@ int launch_tile(const paged::AttnArgs &a, void *workspace, cudaStream_t stream) 
 // 90 and 71.5; head size 64, the 16 requests: 34.1 and 38.7, 52.3 and 42.8.
 constexpr int kTileMinRows = 33;
 
+bool many_rows(int heads, int kv_heads, int max_q) {
+    return static_cast<long long>(heads / kv_heads) * max_q >= kTileMinRows;
+}
+
 int paged_attention_impl(const paged::AttnArgs &p, int dtype, int kernel, void *workspace, cudaStream_t stream) {
     const bool can_stream = stream_applies(p);
     const bool can_tile =
@@ -294,8 +298,7 @@ int paged_attention_impl(const paged::AttnArgs &p, int dtype, int kernel, void *
     if (kernel == PMKL_PAGED_STREAM && !can_stream) return PMKL_ERR_UNSUPPORTED;
     if (kernel == PMKL_PAGED_TCGEN05 && !can_tile) return PMKL_ERR_UNSUPPORTED;
     if (can_stream && kernel != PMKL_PAGED_SIMT && p.batch > 0 && p.max_q > 0) {
-        const bool many = static_cast<long long>(p.H / p.Hkv) * p.max_q >= kTileMinRows;
-        if (kernel == PMKL_PAGED_TCGEN05 || (kernel == PMKL_PAGED_AUTO && can_tile && many)) {
+        if (kernel == PMKL_PAGED_TCGEN05 || (kernel == PMKL_PAGED_AUTO && can_tile && many_rows(p.H, p.Hkv, p.max_q))) {
             if (dtype == PMKL_DTYPE_F16)
                 return p.D == 64 ? launch_tile<__half, 64>(p, workspace, stream)
                                  : launch_tile<__half, 128>(p, workspace, stream);
@@ -392,20 +395,30 @@ int pmkl_paged_append(const void *k, const void *v, const int64_t *k_new_strides
     return paged_append_impl(p, dtype, static_cast<cudaStream_t>(stream));
 }
 
-size_t pmkl_paged_attention_workspace_size(int tokens, int batch, int heads, int kv_heads, int hidden,
-                                           int max_query_len, int dtype) {
+size_t pmkl_paged_attention_workspace_size_ex(int tokens, int batch, int heads, int kv_heads, int hidden,
+                                              int max_query_len, int dtype, int kernel) {
     if (tokens <= 0 || batch <= 0 || heads <= 0 || kv_heads <= 0 || hidden <= 0 || max_query_len < 0 ||
         heads % kv_heads != 0 || !dtype_valid(dtype))
         return 0;
     max_query_len = query_len(max_query_len, tokens);
-    if (hidden != 64 && hidden != 128) return 0;  // the CUDA-core kernel needs none
-    // What the largest of the kernels that may be asked for needs.
-    const size_t stream =
-        paged::partial_workspace(paged::kMaxStreamCtas, stream_rows(heads, kv_heads, max_query_len), hidden);
-    const size_t tile = dtype == PMKL_DTYPE_F32
-                            ? 0
-                            : paged::partial_workspace(paged::kMaxTileCtas, paged::kTileRows, hidden);
-    return align256(stream > tile ? stream : tile);
+    // The CUDA-core kernel needs none.
+    if ((hidden != 64 && hidden != 128) || kernel == PMKL_PAGED_SIMT) return 0;
+    size_t need = 0;
+    // (the streaming kernel also where the tcgen05 kernel is chosen and does not fit)
+    if (kernel != PMKL_PAGED_TCGEN05)
+        need = paged::partial_workspace(paged::kMaxStreamCtas, stream_rows(heads, kv_heads, max_query_len), hidden);
+    if (dtype != PMKL_DTYPE_F32 && (kernel == PMKL_PAGED_TCGEN05 || (kernel == PMKL_PAGED_AUTO && many_rows(heads, kv_heads, max_query_len))))
+        need = std::max(need, paged::partial_workspace(paged::kMaxTileCtas, paged::kTileRows, hidden));
+    return align256(need);
+}
+
+size_t pmkl_paged_attention_workspace_size(int tokens, int batch, int heads, int kv_heads, int hidden,
+                                           int max_query_len, int dtype) {
+    size_t need = 0;
+    for (int kernel : {PMKL_PAGED_STREAM, PMKL_PAGED_TCGEN05})
+        need = std::max(need, pmkl_paged_attention_workspace_size_ex(tokens, batch, heads, kv_heads, hidden,
+                                                                     max_query_len, dtype, kernel));
+    return need;
 }
 
 int pmkl_paged_attention(const void *q, const int64_t *q_strides, const void *k_cache, const void *v_cache,
@@ -434,7 +447,7 @@ int pmkl_paged_attention(const void *q, const int64_t *q_strides, const void *k_
     if (batch > 0 && max_blocks > 0 && !block_table) return PMKL_ERR_NULL_POINTER;
     if (num_blocks > 0 && (!k_cache || !v_cache || !k_scale || !v_scale)) return PMKL_ERR_NULL_POINTER;
     const size_t need =
-        pmkl_paged_attention_workspace_size(tokens, batch, heads, kv_heads, hidden, max_query_len, dtype);
+        pmkl_paged_attention_workspace_size_ex(tokens, batch, heads, kv_heads, hidden, max_query_len, dtype, kernel);
     if (need > 0) {
         if (!workspace) return PMKL_ERR_NULL_POINTER;
         if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return PMKL_ERR_MISALIGNED;

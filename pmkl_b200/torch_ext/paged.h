@@ -158,8 +158,8 @@ std::tuple<at::Tensor, at::Tensor> paged_attention_fw(
     const int Hkv = static_cast<int>(k_cache.size(1)), dt = pmkl_dtype_of(q.scalar_type());
     at::Tensor out = new_tensor(q.sizes(), q.scalar_type(), dev);
     at::Tensor lse = new_tensor({q.size(0), q.size(1)}, at::kFloat, dev);
-    const size_t ws_bytes = pmkl_paged_attention_workspace_size(T, static_cast<int>(batch), H, Hkv, D,
-                                                                static_cast<int>(max_query_len), dt);
+    const size_t ws_bytes = pmkl_paged_attention_workspace_size_ex(
+        T, static_cast<int>(batch), H, Hkv, D, static_cast<int>(max_query_len), dt, static_cast<int>(kernel));
     at::Tensor ws;
     if (ws_bytes > 0) ws = new_tensor({static_cast<int64_t>(ws_bytes)}, at::kByte, dev);
     cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();

@@ -78,15 +78,47 @@ def test_workspace_size_is_zero_for_empty_or_bad_sizes():
 @pytest.mark.parametrize("dtype", [0, 1, 2])
 def test_workspace_is_asked_for_whatever_max_query_len(hidden, dtype):
     """Without query_starts a request has one token, and the workspace of one, also where max_query_len says 0."""
-    f = pmkl_b200.capi().pmkl_paged_attention_workspace_size
-    need = f(2, 2, 4, 2, hidden, 1, dtype)
-    assert need > 0 and f(2, 2, 4, 2, hidden, 0, dtype) == need
+    f = pmkl_b200.capi().pmkl_paged_attention_workspace_size_ex
+    need = f(2, 2, 4, 2, hidden, 1, dtype, 0)
+    assert need > 0 and f(2, 2, 4, 2, hidden, 0, dtype, 0) == need
     for max_q in (0, 1):
         for starts in (None, FAKE):
             assert attend(hidden=hidden, dtype=dtype, max_q=max_q, starts=starts, ws=None, ws_bytes=0) == -3
             assert attend(hidden=hidden, dtype=dtype, max_q=max_q, starts=starts, ws_bytes=need - 1) == -9
     # an upper limit far above the one token is no reason to refuse
     assert attend(hidden=hidden, dtype=dtype, heads=8, kv=1, max_q=0x7FFFFFFF, starts=None, ws=None) == -3
+
+
+@pytest.mark.parametrize("hidden", [64, 128])
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_workspace_size_goes_by_the_kernel(hidden, dtype):
+    """A decode step asks for no more than its kernel can use: of 640 CTAs a descriptor and twice 8 rows with their sums."""
+    import ctypes
+
+    L = pmkl_b200.capi()
+    size = lambda max_q, kernel, tokens=64: L.pmkl_paged_attention_workspace_size_ex(  # noqa: E731
+        tokens, 64, 8, 2, hidden, max_q, dtype, kernel)
+    rows = lambda ctas, n: -(-ctas * (32 + 2 * n * (hidden + 1) * 4) // 256) * 256  # noqa: E731
+    assert size(1, 0) == size(1, 2) == rows(640, 8) and size(8, 2) == rows(640, 32)
+    assert size(1, 1) == 0
+    any_of = lambda max_q: L.pmkl_paged_attention_workspace_size(64, 64, 8, 2, hidden, max_q, dtype)  # noqa: E731
+    if dtype:  # (tcgen05: 16-bit queries, from 33 rows a K/V head on)
+        assert size(1, 3) == size(9, 0) == any_of(1) == any_of(9) == rows(320, 128) and size(8, 0) == rows(640, 32)
+    else:
+        assert size(9, 0) == size(9, 2) == any_of(9) == rows(640, 32)
+    # What a call needs goes by its kernel.  Negative strides, which are looked at after the
+    # workspace, end each call before anything is launched.
+    bad = (ctypes.c_int64 * 2)(-1, -1)
+
+    def call(kernel, ws, ws_bytes):
+        return L.pmkl_paged_attention(FAKE, bad, FAKE, FAKE, None, None, FAKE, FAKE, FAKE, 4, FAKE, FAKE, FAKE, None, FAKE, 64, 64,
+                                      8, 2, hidden, 4, 16, 4, 1, dtype, 1, 0.0, ws, ws_bytes, kernel, None)
+
+    need = size(1, 0)
+    assert call(0, FAKE, need) == -1 and call(0, FAKE, need - 1) == -9 and call(0, None, need) == -3
+    assert call(1, None, 0) == -1
+    if dtype:
+        assert call(3, FAKE, need) == -9 and call(3, FAKE, size(1, 3)) == -1
 
 
 def test_binding_refuses_cpu_tensors():

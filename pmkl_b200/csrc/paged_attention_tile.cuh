@@ -25,7 +25,7 @@
 //     one multiply-add, which is exact enough while the reference is below 2^20;
 //     beyond, the exponents are formed in two steps beforehand (two steps for all:
 //     498 us against 476 on the chunks below), as they are where a page's value
-//     scale is small.  What is seldom needed (masks,
+//     scale is small and far below one before it (715 us on the chunks).  What is seldom needed (masks,
 //     rescaling, those exponents) goes through tensor memory in rolled loops: the
 //     warps' code has to stay in the instruction cache (masks in registers and
 //     an unrolled rescaling, 6 KB more: prompts of 1000 tokens 489 us against 461).
@@ -84,6 +84,11 @@ struct TileCfg {
 
 constexpr int kAhead = 4;
 
+// Powers of two that a value scale lies below the segment's largest so far, from
+// which on the sum's terms come from exponents of their own (kSmallScale, but
+// pages of zeros, whose scale is 2^-64, are then seldom among them).
+constexpr float kFarScale = 64.f;
+
 // References up to here: what the multiply-add of a score with its reference may
 // be off, four roundings of it, stays below 2^-2 (weights below fp16's largest).
 constexpr float kExactRef = 1048576.f;
@@ -101,7 +106,7 @@ struct TileShared {
     // The last: (1, 0) and 0, for scores that are exponents already.
     float2 scale[kAhead + 1][8];
     float inv_vs[kAhead + 1][8];
-    int small[kAhead];   // some group's value scale is below kSmallScale
+    int small[kAhead];   // some group's value scale is small beside the segment's largest so far
     int nan[2];          // the tile's values held NaN: tile number of the CTA + 1
     alignas(16) uint32_t nan_cols[kTileRows][4];  // columns of a row that are NaN (see above)
     long long sum[kTileThreads / 32];
@@ -238,6 +243,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                     return key < lim_max ? __ldg(table + key / p.block) : -1;
                 };
                 int x = look_up(tile0);
+                float lv_top = -INFINITY;  // the largest log2 of a value scale so far
                 for (int j = tile0; j < tile1; ++j, ++it) {
                     const int x_next = j + 1 < tile1 ? look_up(j + 1) : -1;
                     const int row = (j * 128 + (lane & 7) * 16) % p.block;
@@ -252,7 +258,10 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                         vs = value_scale(__ldg(p.v.scale + at));
                     }
                     const float lv = there ? log2f(vs) : -INFINITY;
-                    const int small = __any_sync(0xffffffffu, there && lv < kSmallScale);
+                    lv_top = fmaxf(lv_top, lv);
+#pragma unroll
+                    for (int o = 1; o < 8; o <<= 1) lv_top = fmaxf(lv_top, __shfl_xor_sync(0xffffffffu, lv_top, o));
+                    const int small = __any_sync(0xffffffffu, there && lv_top - lv > kFarScale);
                     const int i = it % kAhead;
                     if (it >= kAhead && !(ok = wait_warp(&sh.page_empty[i], (it / kAhead - 1) & 1, abort_flag))) break;
                     if (lane < 16) sh.from[i][lane >> 3][lane & 7] = from;

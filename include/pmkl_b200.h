@@ -329,7 +329,8 @@ typedef enum pmkl_plan_status {
  * fit max_blocks is left out and takes no page.  Of the others request b gets
  * its pages when the pages that the requests up to b need together are there
  * (requests that need none always pass).  The sum of new_lens must stay below
- * 2^31.
+ * 2^31.  The rows of a request that was left out have no key and value in the
+ * cache: what an attention computes for them means nothing.
  */
 int pmkl_paged_plan(const int32_t *cached_lens, const int32_t *new_lens, int32_t *block_table, int64_t table_stride,
                     const int32_t *free_blocks, const int32_t *free_count, int free_capacity, int batch,
@@ -340,8 +341,8 @@ int pmkl_paged_plan(const int32_t *cached_lens, const int32_t *new_lens, int32_t
  * Writes new keys and values into the cache as 8-bit floats.
  *
  *   k, v     : [tokens, kv_heads, hidden] of `dtype`, element strides
- *              (token, head) kv_strides_k / kv_strides_v, NULL = contiguous,
- *              hidden contiguous.
+ *              (token, head) k_new_strides / v_new_strides, NULL =
+ *              contiguous, hidden contiguous.
  *   slot_map : [tokens] int64; tokens with a slot outside the cache (-1) are
  *              skipped.
  *

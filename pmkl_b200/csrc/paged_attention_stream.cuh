@@ -7,7 +7,7 @@
 // bound, so the kernel is built to keep loads in flight and nothing else.
 //
 //   * Work is the list of all (request, K/V head, row tile) items, each cut in
-//     tiles of 128 keys; a grid of resident CTAs takes equal shares of the
+//     tiles of 16 keys a warp (128 keys; 192 with 9 to 16 rows); a grid of resident CTAs takes equal shares of the
 //     list, whatever the lengths, a CTA's share beginning and ending inside an
 //     item.  Each CTA finds its share from the lengths itself.  Items that lie
 //     in one CTA are written at once; the others leave normalised partial rows
@@ -42,12 +42,12 @@
 //
 // mma.sync and not tcgen05: 8 to 32 query rows leave most of a 128-row tcgen05
 // tile empty, and the cache's bytes are the bound.  B200, device time: 16 x 4096
-// keys, 32 heads of 128 (538 MB): 101 us, 5.33 TB/s (0.81 of the measured copy
+// keys, 32 heads of 128 (538 MB): 102 us, 5.27 TB/s (0.80 of the measured copy
 // bandwidth; a CTA's loop over tiles alone runs at 7.6 TB/s, the rest is its
 // start of some 8000 cycles, the change of items and the join); 64 requests of
 // 1..16384 keys, 32/8 heads (939 MB): 188 us, 5.0 TB/s; one request of 131071
-// keys, 32/8 heads (269 MB): 62 us; 8 x 1024 keys, 16 heads of 64: 13.7 us and
-// 2 x 128 keys, 4 heads, fp32: 6.2 us, bound by the latency of what comes before
+// keys, 32/8 heads (269 MB): 62 us; 8 x 1024 keys, 16 heads of 64: 14.0 us and
+// 2 x 128 keys, 4 heads, fp32: 6.4 us, bound by the latency of what comes before
 // the first key (lengths, share, table, queries) and of the join.
 //
 // Rows behind a request's last key may hold anything: their scores are set to

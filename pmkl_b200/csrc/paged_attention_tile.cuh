@@ -28,14 +28,14 @@
 //     scale is small and far below one before it (715 us on the chunks).  What is seldom needed (masks,
 //     rescaling, those exponents) goes through tensor memory in rolled loops: the
 //     warps' code has to stay in the instruction cache (masks in registers and
-//     an unrolled rescaling, 6 KB more: prompts of 1000 tokens 489 us against 461).
+//     an unrolled rescaling, 5 KB more: prompts of 1000 tokens 489 us against 461).
 // Tensor memory (256 columns a CTA): S [0, 128), O [128, 128 + D); P takes S's
 // upper half: scores 64..127 are held in registers when it is written.
 //
 // What bounds it: each CTA's chain (S 600 cycles, softmax 3300, P V 600, and the
 // hand-overs), some 6000 cycles a tile with two CTAs an SM, against 1024 cycles
 // of tensor work.  B200, device time: chunks of 700..1024 tokens over 3001..8192
-// keys, 32/8 heads of 128 (bf16): 481 us, 618 TFLOP/s (0.38 of the measured bf16
+// keys, 32/8 heads of 128 (bf16): 478 us, 622 TFLOP/s (0.38 of the measured bf16
 // rate); 1..5 tokens over 500..8192 keys, 32/4 heads (fp16): 53 us, where the
 // loads' latency is the chain (a half tile of keys and one of values a CTA under
 // way).

@@ -278,10 +278,11 @@ int launch_tile(const paged::AttnArgs &a, void *workspace, cudaStream_t stream) 
 }
 
 // The tcgen05 kernel from this many rows a K/V head on (16-bit queries).  B200, 16
-// requests of 500..8192 keys, 4 K/V heads of 128: 32 rows 47.8 us streaming, 53.8
-// here; 40 rows (a second row tile, which reads the keys again) 70.5 and 57.8; 64
-// rows 76 and 60.  One request of 131071 keys: 32 rows 58.0 and 68.1, 40 rows
-// 90 and 71.5; head size 64, the 16 requests: 34.1 and 38.7, 52.3 and 42.8.
+// requests of 500..8192 keys, 4 K/V heads of 128: 32 rows 48.8 us streaming, 53.0
+// here; 40 rows (a second row tile, which reads the keys again) 73.5 and 57.1; 64
+// rows 78 and 60.  One request of 131071 keys, 8 K/V heads: 32 rows 95.9 and
+// 101.3, 40 rows 167 and 109; head size 64, the 16 requests: 36.3 and 38.6, 55.3
+// and 42.4.
 constexpr int kTileMinRows = 33;
 
 bool many_rows(int heads, int kv_heads, int max_q) {

@@ -121,7 +121,8 @@ def paged_plan(cached_lens, new_lens, block_table, free_blocks, free_count, bloc
     block_size + row of each token, -1 behind the last), ``free_count`` [1] (a
     new tensor: pages left) and ``status`` [batch]: 0, or why the request was
     left out, with no page taken and -1 for its tokens (1 not enough free
-    pages, 2 ``block_table`` too narrow, 3 past ``max_tokens``)."""
+    pages, 2 ``block_table`` too narrow or the length past 2^31 - 1, 3 past
+    ``max_tokens``); what an attention computes for its tokens means nothing."""
     return pmkl_pytorch_ext.paged_plan(cached_lens, new_lens, block_table, free_blocks, free_count, block_size,
                                        max_tokens)
 
@@ -134,7 +135,11 @@ def paged_append(k, v, slot_map, k_cache, v_cache, k_scale, v_scale):
     float32 [pages, kv_heads], powers of two.  ``slot_map`` int64 as from
     ``paged_plan``; tokens with a slot of -1 are skipped.  All four cache
     tensors are updated in place: the scale of a page grows with its rows, and
-    rows written earlier are then rounded again to the larger scale."""
+    rows written earlier are then rounded again to the larger scale.
+
+    Tokens that follow one another in a page's rows are written together; a page
+    may get one such run a call (``paged_plan``'s slot maps are so): two runs in
+    one page would race on its scale."""
     pmkl_pytorch_ext.paged_append(k, v, slot_map, k_cache, v_cache, k_scale, v_scale)
 
 

@@ -132,8 +132,6 @@ std::tuple<at::Tensor, at::Tensor> paged_attention_fw(
     const c10::optional<at::Tensor> &query_starts, c10::optional<int64_t> max_len, bool is_causal, double scale,
     int64_t kernel) {
     check_packed(q, "q");
-    // Not given: one token a request without query_starts, any number with them.
-    const int64_t max_query_len = max_len.has_value() ? *max_len : (query_starts.has_value() ? q.size(0) : 1);
     const at::Device dev = q.device();
     check_cache(k_cache, k_scale, "k", dev);
     check_cache(v_cache, v_scale, "v", dev);
@@ -148,6 +146,8 @@ std::tuple<at::Tensor, at::Tensor> paged_attention_fw(
         check_vector(*query_starts, "query_starts", batch + 1, dev);
     else
         TORCH_CHECK(q.size(0) == batch, "paged_attention: without query_starts q must have one token a request");
+    // Not given: the requests' average, since it only chooses the kernel.
+    const int64_t max_query_len = max_len.has_value() ? *max_len : (q.size(0) + batch - 1) / std::max<int64_t>(batch, 1);
     TORCH_CHECK(max_query_len >= 0 && max_query_len <= INT32_MAX, "paged_attention: max_query_len must not be negative");
     TORCH_CHECK(k_cache.size(2) >= 1, "paged_attention: pages must have rows");
     const c10::cuda::CUDAGuard guard(dev);

@@ -152,8 +152,8 @@ def paged_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens
     ``query_starts[b + 1]`` of ``q`` (without ``query_starts``: row b) and stand
     at the end of its rows; with ``is_causal`` each sees the keys up to its own
     place.  ``max_query_len``, the most tokens that a request has, chooses the
-    kernel: give it where it is far below the number of tokens (a wrong one
-    costs time, not results).  Query head h reads K/V head h // (heads //
+    kernel and nothing else (a wrong one costs time, not results); without it
+    the requests' average is taken.  Query head h reads K/V head h // (heads //
     kv_heads).  ``scale`` <= 0: 1/sqrt(hidden).
 
     Returns ``out`` like q and ``lse`` [tokens, heads] float32, the log of the
